@@ -286,6 +286,60 @@ int gncde_clip_adamw(int32_t P, float* params, const float* grads, float* m, flo
                      float b1, float b2, float eps, float weight_decay, float max_norm, float* stats,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- training step over many tensors ------------------------------------------------------------------------ */
+enum { GNCDE_DTYPE_FP32 = 0, GNCDE_DTYPE_BF16 = 1, GNCDE_DTYPE_FP16 = 2 };
+typedef struct {
+  const void* in;   /* numel values of dtype, contiguous, aligned to the value's size (may be NULL when numel is 0) */
+  void* out;        /* gncde_clip_by_global_norm only: as in; the same pointer clips in place, any other overlap with
+                       a tensor of the list is an error of the caller's */
+  int64_t numel;
+  int32_t dtype;    /* GNCDE_DTYPE_* */
+  int32_t reserved;
+} GncdeTensor;
+
+/* stats[0] = sqrt of the sum of squares over every value of every tensor, stats[1] = the largest magnitude (device
+ * fp32[2]; squares and sums in 64 bits, so stats[0] is inf only where the norm itself passes fp32; a NaN anywhere makes
+ * both NaN; an empty list gives 0, 0).  `tensors` is a HOST array, read before the call returns.  Deterministic. */
+size_t gncde_global_norm_workspace_bytes(int32_t count);
+int gncde_global_norm(int32_t count, const GncdeTensor* tensors, float* stats, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* gncde_global_norm, and out = in where stats[0] < max_norm, else in * (max_norm / stats[0]) (optax.clip_by_global_norm,
+ * optimiser_configs.py:76-84): a norm of inf leaves zeros (NaN where the value is inf), a NaN norm NaN everywhere.
+ * max_norm: positive and finite. */
+int gncde_clip_by_global_norm(int32_t count, const GncdeTensor* tensors, float max_norm, float* stats,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- linear read-out joined with its softmax cross-entropy ------------------------------------------------------
+ * With l_rv = sum_h x_rh W_vh + b_v, lse_r = log sum_v exp l_rv and S_r = sum_v y_rv:
+ *   loss_r = S_r lse_r - sum_v y_rv l_rv                     (trainer_tgb.cross_entropy_loss, trainer_tgb.py:42-60)
+ * without the logits [rows, classes] in memory: they are made tile by tile, and once more for the gradient.
+ *   x [rows, hidden], W [classes, hidden], b [classes] (may be NULL): dtype GNCDE_DTYPE_FP32 or _BF16, all the same
+ *   target by target_kind: INDEX32 / INDEX64 [rows] class indices (y_r one-hot, S_r = 1; a NEGATIVE index leaves the
+ *          row out; an index >= classes makes the row's loss, and every gradient it enters, NaN), or ROWS
+ *          [rows, classes] fp32 y
+ *   mask [rows] bytes, 0 leaves the row out (may be NULL)
+ *   loss [rows] fp32, 0 for rows left out; stats [rows, 2] fp32 (lse_r, S_r), read by the gradient
+ * A row left out changes nothing, whatever its values.  b may hold -inf (a class nothing can be); non-finite values in
+ * x (of a row that counts) or W make losses NaN or inf.  Sums, maxima and logits are fp32 (bf16 inputs: exact products,
+ * fp32 accumulation; fp32 inputs: each value as three bf16 parts, whose six leading products leave ~2^-24 of |x||W|;
+ * the parts end at 2^-133, so fp32 values below 2^-109 carry fewer bits). */
+enum { GNCDE_TARGET_INDEX32 = 0, GNCDE_TARGET_INDEX64 = 1, GNCDE_TARGET_ROWS = 2 };
+/* Workspace of the loss (grad 0) or the gradient (grad 1); 0 for sizes the entries refuse. */
+size_t gncde_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype,
+                                                  int32_t grad);
+int gncde_linear_cross_entropy(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype, const void* x,
+                               const void* W, const void* b, int32_t target_kind, const void* target,
+                               const uint8_t* mask, float* loss, float* stats, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* Gradient for the rows' cotangents g [rows] fp32, with dl_rv = g_r (S_r exp(l_rv - lse_r) - y_rv):
+ *   gx = dl W [rows, hidden], gW = dl^T x [classes, hidden], gb = sum_r dl [classes], each of dtype, each may be NULL.
+ * Deterministic (fixed order of sums, no atomics). */
+int gncde_linear_cross_entropy_grad(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype, const void* x,
+                                    const void* W, const void* b, int32_t target_kind, const void* target,
+                                    const uint8_t* mask, const float* stats, const float* g, void* gx, void* gW,
+                                    void* gb, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- input side ------------------------------------------------------------------------------ */
 /* Graph operators of misc.py:58-113 (get_graph_operator), per graph, fp32:
  *   NORM_LAP        I - D_out^-1/2 (A + I) D_in^-1/2, degrees of A + I   (default, misc.py:83-99)

@@ -1,0 +1,833 @@
+// Linear read-out joined with its softmax cross-entropy (gncde_linear_cross_entropy, .._grad).
+//
+//   l_rv = sum_h x_rh W_vh + b_v,   lse_r = log sum_v exp l_rv,   loss_r = S_r lse_r - sum_v y_rv l_rv
+//   dl_rv = g_r (S_r exp(l_rv - lse_r) - y_rv),   gx = dl W,   gW = dl^T x,   gb_v = sum_r dl_rv
+//
+// replacing log_softmax over materialised logits [rows, classes] (trainer_tgb.py:42-60) and its reverse mode.  The
+// logits are never stored: the loss keeps, per row and tile of classes, the largest logit and the sum of exponentials
+// relative to it; the gradient makes the logits once more, a piece of the classes at a time, and stores that piece's
+// dl as bf16 matrix operands.  All four products are one kernel, C^T = B A^T over operands that lie along their
+// contraction, on v_mfma_f32_16x16x32_bf16 with fp32 accumulation:
+//
+//   product   A (rows of the tile)     B (columns)          contraction   epilogue
+//   logits    W       [classes, H]     x       [rows, H]    H             largest logit, sum of exponentials
+//   logits    W piece [Vc, H]          x       [rows, H]    H             dl piece, as [rows, Vc] and [Vc, rows]
+//   gx        W^T     [H, Vc]          dl      [rows, Vc]   Vc            fp32 sums / gx
+//   gW        x^T     [H, rows]        dl^T    [Vc, rows]   rows          gW
+//
+// fp32 inputs are split into three bf16 parts each (8 bits of the significand a part, rounded to nearest: nothing is
+// lost) and the six products above 2^-24 of |a||b| are summed, smallest first: fp32-class results on the bf16 matrix
+// rate (16 times the fp32 one, so 2.7 times faster than fp32 MFMA at equal utilisation).
+#include "gncde_internal.h"
+
+#include <algorithm>
+
+namespace gncde {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kBK = 64;  // contraction per step: 128 bytes, eight 16-byte chunks a row
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+__device__ __forceinline__ float from_bf16(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+
+// x = p0 + p1 + p2 in bf16 parts.  A finite x that would round to inf (above 3.39e38) is cut instead; an inf or NaN
+// stays in p0 alone.
+template <int NP>
+__device__ __forceinline__ void split(float x, uint16_t (&p)[NP]) {
+  p[0] = to_bf16(x);
+  if (NP == 3) {
+    if ((p[0] & 0x7f80) == 0x7f80 && (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u)
+      p[0] = (uint16_t)(__float_as_uint(x) >> 16);
+    const bool whole = (p[0] & 0x7f80) != 0x7f80;
+    const float r1 = whole ? x - from_bf16(p[0]) : 0.f;
+    p[NP > 1 ? 1 : 0] = NP > 1 ? to_bf16(r1) : p[0];
+    const float r2 = r1 - from_bf16(p[NP > 1 ? 1 : 0]);
+    p[NP > 2 ? 2 : 0] = NP > 2 ? to_bf16(r2) : p[0];
+  }
+}
+
+// ---- targets and rows left out ----------------------------------------------------------------------------------
+struct Rows {
+  const void* target;
+  const uint8_t* mask;
+  int32_t kind;
+};
+
+__device__ __forceinline__ int64_t row_index(const Rows& r, int64_t n) {
+  return r.kind == GNCDE_TARGET_INDEX32 ? (int64_t) static_cast<const int32_t*>(r.target)[n]
+                                        : static_cast<const int64_t*>(r.target)[n];
+}
+
+__device__ __forceinline__ bool row_counts(const Rows& r, int64_t n) {
+  if (r.mask && r.mask[n] == 0) return false;
+  return r.kind == GNCDE_TARGET_ROWS || row_index(r, n) >= 0;
+}
+
+// ---- operand layout ---------------------------------------------------------------------------------------------
+template <bool F32>
+__device__ __forceinline__ float value(const void* p, int64_t i) {
+  return F32 ? static_cast<const float*>(p)[i] : from_bf16(static_cast<const uint16_t*>(p)[i]);
+}
+
+// src [R, H] -> planes [NP][R][Kp], zeros behind H.
+template <bool F32, int NP>
+__global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int Kp, uint16_t* __restrict__ dst) {
+  const int cpr = Kp / 8;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < R * cpr; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = e / cpr;
+    const int h0 = (int)(e - r * cpr) * 8;
+    u16x8 o[NP];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint16_t p[NP];
+      split<NP>(h0 + i < H ? value<F32>(src, r * H + h0 + i) : 0.f, p);
+#pragma unroll
+      for (int q = 0; q < NP; ++q) o[q][i] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + ((int64_t)q * R + r) * Kp + h0) = o[q];
+  }
+}
+
+// src [R, H] -> transposed planes [NP][H][Rp], zeros behind R and (LEFT) in rows left out, whatever they hold.
+template <bool F32, int NP, bool LEFT>
+__global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
+                                                     Rows rows, uint16_t* __restrict__ dst) {
+  __shared__ float t[64][65];
+  const int64_t ht = (H + 63) / 64;
+  const int64_t r0 = (blockIdx.x / ht) * 64;
+  const int h0 = (int)(blockIdx.x % ht) * 64;
+  const int c = threadIdx.x & 63, q4 = threadIdx.x >> 6;
+  for (int i = q4; i < 64; i += 4) {
+    const int64_t r = r0 + i;
+    const int h = h0 + c;
+    const bool in = r < R && h < H && (!LEFT || row_counts(rows, r));
+    t[i][c] = in ? value<F32>(src, r * H + h) : 0.f;
+  }
+  __syncthreads();
+  const int rc = (threadIdx.x & 7) * 8, hh = threadIdx.x >> 3;
+  for (int i = hh; i < 64; i += 32) {
+    const int h = h0 + i;
+    if (h >= H) continue;
+    u16x8 o[NP];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint16_t p[NP];
+      split<NP>(t[rc + j][i], p);
+#pragma unroll
+      for (int q = 0; q < NP; ++q) o[q][j] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + ((int64_t)q * H + h) * Rp + r0 + rc) = o[q];
+  }
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------
+enum { E_LSE = 0, E_DL = 1, E_OUT = 2 };
+
+struct GemmArgs {
+  const uint16_t* A;
+  const uint16_t* B;
+  int64_t lda, ldb, sa, sb;  // row and plane strides in values
+  int64_t M, N;              // rows of A and of B
+  int K;                     // contraction, a multiple of 8
+  int kt;                    // steps of kBK over K
+  int per_split;             // steps a workgroup of one split takes
+  int64_t tm, tn;            // tiles
+  // logits
+  Rows rows;
+  const void* bias;          // this piece's
+  int64_t v0, V;             // first class of the piece, classes in all
+  float2* part;              // E_LSE: [N][tm] (largest, sum of exponentials)
+  float2* part_y;            // E_LSE, label rows: [N][tm] (sum y l, sum y)
+  float* hit;                // E_LSE, indices: [N] the target's logit
+  const float* stats;        // E_DL
+  const float* g;
+  uint16_t* P;               // E_DL: planes [N][ldp]
+  uint16_t* Pt;              // planes [M][ldpt]
+  int64_t ldp, ldpt, sp, spt;
+  float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
+  // products
+  void* out;                 // E_OUT: [N][ldo]
+  float* acc;                // fp32 [split][N][lda_c]; NULL: write `out`
+  int64_t ldo, ldacc;
+  int32_t add;               // acc += instead of =
+  int32_t vec;               // out rows can be written four values at a time
+};
+
+template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32>
+__global__ void __launch_bounds__(WM* WN * 64, 1) k_xent_mm(GemmArgs a) {
+  constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
+  constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;  // 1 KB (eight rows) loads a wave
+  static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN, "tile rows divide over the waves");
+  constexpr int TILE = (BM + BN) * kBK;
+  constexpr int NSEG = NP == 1 ? 1 : 6;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Tile of this workgroup: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the tile order,
+  // and the order walks blocks of eight tiles of A by all of B: what an XCD reads at a time stays in its own cache.
+  int64_t tile_m, tile_n;
+  {
+    const int64_t nt = a.tm * a.tn, bid = blockIdx.x;
+    const int64_t q = nt >> 3, r = nt & 7, xcd = bid & 7, idx = bid >> 3;
+    const int64_t lin = xcd * q + (xcd < r ? xcd : r) + idx;
+    const int64_t grp = lin / (8 * a.tn), in = lin - grp * 8 * a.tn;
+    const int64_t gm = a.tm - grp * 8 < 8 ? a.tm - grp * 8 : 8;
+    tile_m = grp * 8 + in % gm;
+    tile_n = in / gm;
+  }
+  const int64_t m0 = tile_m * BM, n0 = tile_n * BN;
+
+  // Each lane's source chunk: row lane / 8 of the eight, chunk (lane % 8) ^ row, so that the chunk a lane of the matrix
+  // operand reads later lies in another bank for every row.
+  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) * 8;
+  const uint16_t* pa[IA];
+  const uint16_t* pb[IB];
+#pragma unroll
+  for (int i = 0; i < IA; ++i) {
+    int64_t row = m0 + (wave * IA + i) * 8 + lr;
+    row = row < a.M ? row : a.M - 1;
+    pa[i] = a.A + row * a.lda + lc;
+  }
+#pragma unroll
+  for (int i = 0; i < IB; ++i) {
+    int64_t row = n0 + (wave * IB + i) * 8 + lr;
+    row = row < a.N ? row : a.N - 1;
+    pb[i] = a.B + row * a.ldb + lc;
+  }
+  const int k_from = blockIdx.y * a.per_split;
+  const int k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
+  const int steps = (k_to - k_from) * NSEG;
+  const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero16);
+
+  auto load = [&](int s, int buf) {
+    int64_t oa = 0, ob = 0;
+    int k = s + k_from;
+    if (NSEG > 1) {
+      const int seg = s / (k_to - k_from);
+      k = s - seg * (k_to - k_from) + k_from;
+      const int ia = seg == 1 ? 2 : (seg == 2 || seg == 4) ? 1 : 0;  // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+      const int ib = seg == 0 ? 2 : (seg == 2 || seg == 3) ? 1 : 0;
+      oa = ia * a.sa;
+      ob = ib * a.sb;
+    }
+    const int kk = k * kBK;
+    const bool in = kk + lc < a.K;
+#pragma unroll
+    for (int i = 0; i < IA; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(in ? pa[i] + oa + kk : zero),
+          (__attribute__((address_space(3))) void*)(lds + buf * TILE + (wave * IA + i) * 8 * kBK), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < IB; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(in ? pb[i] + ob + kk : zero),
+          (__attribute__((address_space(3))) void*)(lds + buf * TILE + BM * kBK + (wave * IB + i) * 8 * kBK), 16, 0,
+          0);
+  };
+
+  floatx4 acc[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int fr = lane & 15, fk = lane >> 4;
+  const uint16_t* la = lds + (wm * (BM / WM) + fr) * kBK;
+  const uint16_t* lb = lds + BM * kBK + (wn * (BN / WN) + fr) * kBK;
+  const int c0 = ((fk) ^ (fr & 7)) * 8, c1 = ((4 + fk) ^ (fr & 7)) * 8;
+
+  if (steps > 0) load(0, 0);
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads are in LDS
+    __syncthreads();                     // everybody's are, and the other buffer has been read
+    if (s + 1 < steps) load(s + 1, buf ^ 1);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int c = kk ? c1 : c0;
+      bf16x8 fa[RT], fb[CT];
+#pragma unroll
+      for (int j = 0; j < CT; ++j) fb[j] = *reinterpret_cast<const bf16x8*>(lb + buf * TILE + j * 16 * kBK + c);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) fa[i] = *reinterpret_cast<const bf16x8*>(la + buf * TILE + i * 16 * kBK + c);
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  __syncthreads();
+
+  const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
+  const int64_t nb = n0 + wn * (BN / WN) + fr;
+
+  if constexpr (EPI == E_OUT) {
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const int64_t n = nb + j * 16;
+      if (n >= a.N) continue;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int64_t m = mb + i * 16;
+        if (m >= a.M) continue;
+        floatx4 v = acc[i][j];
+        if (a.acc) {
+          floatx4* p = reinterpret_cast<floatx4*>(a.acc + ((int64_t)blockIdx.y * a.N + n) * a.ldacc + m);
+          if (a.add) v += *p;
+          *p = v;
+        } else if (F32) {
+          float* p = static_cast<float*>(a.out) + n * a.ldo + m;
+          if (a.vec) {
+            *reinterpret_cast<floatx4*>(p) = v;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (m + q < a.M) p[q] = v[q];
+          }
+        } else {
+          uint16_t* p = static_cast<uint16_t*>(a.out) + n * a.ldo + m;
+          const u16x4 o = {to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+          if (a.vec) {
+            *reinterpret_cast<u16x4*>(p) = o;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (m + q < a.M) p[q] = o[q];
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // logits: bias, classes behind the last at -inf
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t m = mb + i * 16 + q;
+      const float bv = m < a.M ? (a.bias ? value<F32>(a.bias, m) : 0.f) : 0.f;
+#pragma unroll
+      for (int j = 0; j < CT; ++j) acc[i][j][q] = m < a.M ? acc[i][j][q] + bv : -INFINITY;
+    }
+
+  if constexpr (EPI == E_LSE) {
+    float* sm = reinterpret_cast<float*>(lds);  // [4][WM][BN]
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const int64_t n = nb + j * 16;
+      const bool in = n < a.N && row_counts(a.rows, n);
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top = fmaxf(top, acc[i][j][q]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, dot = 0.f, mass = 0.f;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * kLog2e);
+      if (a.rows.kind == GNCDE_TARGET_ROWS) {
+        if (in) {
+          const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int64_t m = mb + i * 16 + q;
+              const float yv = m < a.M ? y[m] : 0.f;
+              mass += yv;
+              dot += yv == 0.f ? 0.f : yv * acc[i][j][q];  // a class at -inf without mass adds nothing
+            }
+        }
+        dot += __shfl_xor(dot, 16);
+        dot += __shfl_xor(dot, 32);
+        mass += __shfl_xor(mass, 16);
+        mass += __shfl_xor(mass, 32);
+      } else if (in) {
+        const int64_t t = row_index(a.rows, n) - a.v0 - mb;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (t == i * 16 + q && mb + t < a.M) a.hit[n] = acc[i][j][q];
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (fk == 0) {
+        const int col = wn * (BN / WN) + j * 16 + fr;
+        sm[wm * BN + col] = top;
+        sm[(WM + wm) * BN + col] = sum;
+        sm[(2 * WM + wm) * BN + col] = dot;
+        sm[(3 * WM + wm) * BN + col] = mass;
+      }
+    }
+    __syncthreads();
+    for (int col = threadIdx.x; col < BN; col += NW * 64) {
+      if (n0 + col >= a.N) break;
+      float top = sm[col];
+#pragma unroll
+      for (int w = 1; w < WM; ++w) top = fmaxf(top, sm[w * BN + col]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, dot = 0.f, mass = 0.f;
+#pragma unroll
+      for (int w = 0; w < WM; ++w) {
+        const float tw = sm[w * BN + col];
+        sum += sm[(WM + w) * BN + col] * (tw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((tw - ref) * kLog2e));
+        dot += sm[(2 * WM + w) * BN + col];
+        mass += sm[(3 * WM + w) * BN + col];
+      }
+      a.part[(n0 + col) * a.tm + tile_m] = make_float2(top, sum);
+      if (a.rows.kind == GNCDE_TARGET_ROWS) a.part_y[(n0 + col) * a.tm + tile_m] = make_float2(dot, mass);
+    }
+    return;
+  }
+
+  if constexpr (EPI == E_DL) {
+    const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const int64_t n = nb + j * 16;
+      const bool in = n < a.N && row_counts(a.rows, n);
+      const float lse = in ? a.stats[2 * n] : 0.f, gv = in ? a.g[n] : 0.f;
+      const float gs = in ? gv * a.stats[2 * n + 1] : 0.f;
+      const int64_t t = (in && !soft) ? row_index(a.rows, n) - a.v0 - mb : -1;
+      const float* y = (in && soft) ? static_cast<const float*>(a.rows.target) + n * a.V + a.v0 : nullptr;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        uint16_t p[4][NP];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t m = mb + i * 16 + q;
+          float d = gs * __builtin_amdgcn_exp2f((acc[i][j][q] - lse) * kLog2e);
+          if (soft) d -= (in && m < a.M) ? gv * y[m] : 0.f;
+          else d -= t == i * 16 + q ? gv : 0.f;
+          d = (in && m < a.M) ? d : 0.f;
+          acc[i][j][q] = d;
+          split<NP>(d, p[q]);
+        }
+        const int64_t m = mb + i * 16;
+        if (n < a.N && m < a.ldp) {
+#pragma unroll
+          for (int s = 0; s < NP; ++s)
+            *reinterpret_cast<u16x4*>(a.P + s * a.sp + n * a.ldp + m) = u16x4{p[0][s], p[1][s], p[2][s], p[3][s]};
+        }
+        if (n < a.ldpt) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (m + q < a.M) {
+#pragma unroll
+              for (int s = 0; s < NP; ++s) a.Pt[s * a.spt + (m + q) * a.ldpt + n] = p[q][s];
+            }
+        }
+      }
+    }
+    if (a.part_b) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float s = 0.f;
+#pragma unroll
+          for (int j = 0; j < CT; ++j) s += acc[i][j][q];
+          s += __shfl_xor(s, 1);
+          s += __shfl_xor(s, 2);
+          s += __shfl_xor(s, 4);
+          s += __shfl_xor(s, 8);
+          const int64_t m = mb + i * 16 + q;
+          if (fr == 0 && m < a.M) a.part_b[(tile_n * WN + wn) * a.M + m] = s;
+        }
+    }
+  }
+}
+
+// ---- joins ------------------------------------------------------------------------------------------------------
+// One wave a row: the tiles' (largest, sum) pairs into the row's running pair; at the last piece, lse and the loss.
+__global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, const float2* __restrict__ part,
+                                                   const float2* __restrict__ part_y, const float* __restrict__ hit,
+                                                   Rows rows, int64_t V, float4* __restrict__ run, int first, int last,
+                                                   float* __restrict__ loss, float* __restrict__ stats) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  float top = -INFINITY, sum = 0.f, dot = 0.f, mass = 0.f;
+  if (!first && lane == 0) {
+    const float4 r = run[n];
+    top = r.x, sum = r.y, dot = r.z, mass = r.w;
+  }
+  for (int64_t i = lane; i < tiles; i += 64) {
+    const float2 p = part[n * tiles + i];
+    const float nt = fmaxf(top, p.x), ref = nt == -INFINITY ? 0.f : nt;
+    sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
+          p.y * (p.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p.x - ref) * kLog2e));
+    top = nt;
+    if (part_y) {
+      const float2 q = part_y[n * tiles + i];
+      dot += q.x;
+      mass += q.y;
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d);
+    const float nt = fmaxf(top, ot), ref = nt == -INFINITY ? 0.f : nt;
+    sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
+          os * (ot == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ot - ref) * kLog2e));
+    top = nt;
+    dot += __shfl_xor(dot, d);
+    mass += __shfl_xor(mass, d);
+  }
+  if (lane != 0) return;
+  if (!last) {
+    run[n] = make_float4(top, sum, dot, mass);
+    return;
+  }
+  const bool counts = row_counts(rows, n);
+  float lse = top + logf(sum);
+  if (rows.kind != GNCDE_TARGET_ROWS && counts) {
+    const bool in = row_index(rows, n) < V;
+    lse = in ? lse : NAN;
+    dot = in ? hit[n] : NAN;
+    mass = 1.f;
+  }
+  loss[n] = counts ? mass * lse - dot : 0.f;
+  stats[2 * n] = counts ? lse : 0.f;
+  stats[2 * n + 1] = counts ? mass : 0.f;
+}
+
+// out[i] = sum over splits of acc[s][i], in the split order.
+template <bool F32>
+__global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __restrict__ acc, int64_t ldacc,
+                           int64_t stride, void* __restrict__ out, int64_t ldo) {
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * M; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t n = e / M, m = e - n * M;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += acc[k * stride + n * ldacc + m];
+    if (F32) static_cast<float*>(out)[n * ldo + m] = s;
+    else static_cast<uint16_t*>(out)[n * ldo + m] = to_bf16(s);
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
+
+constexpr int64_t kCus = 256;
+constexpr int64_t kMostBlocks = int64_t(1) << 20;  // of the element-wise kernels: the rest by their loops
+constexpr int64_t kPieceBytes = int64_t(512) << 20;
+
+struct Plan {
+  int64_t N, H, V;
+  bool f32, direct_ok;  // direct_ok: sizes allow x and W as operands as they lie (the pointers decide too)
+  int np;
+  int64_t Kp, Np;
+  int64_t piece;        // classes a piece
+  int64_t bytes = 0;
+  // offsets
+  int64_t o_x = 0, o_w = 0, o_part = 0, o_party = 0, o_hit = 0, o_run = 0;
+  int64_t o_xt = 0, o_wt = 0, o_p = 0, o_pt = 0, o_gx = 0, o_gw = 0, o_b = 0;
+  int64_t gx_split = 1, gw_split = 1, ldacc = 0;
+
+  int64_t take(int64_t n) {
+    const int64_t at = bytes;
+    bytes += up(std::max<int64_t>(n, 16), 256);
+    return at;
+  }
+};
+
+struct Tile {
+  bool big;
+  int64_t bm, bn, wn;
+};
+
+// 256 x 256 tiles read the least per product; below one for every CU, 128 x 128 tiles keep more CUs at work.
+Tile tile_of(int64_t M, int64_t N) {
+  const bool big = div_up(M, 256) * div_up(N, 256) >= 200;
+  return big ? Tile{true, 256, 256, 4} : Tile{false, 128, 128, 2};
+}
+
+// Splits of the contraction so that a product of few tiles fills the chip; at least four steps each.
+int64_t split_of(int64_t M, int64_t N, int64_t kt, int np) {
+  const Tile t = tile_of(M, N);
+  const int64_t tiles = div_up(M, t.bm) * div_up(N, t.bn);
+  const int64_t want = std::max<int64_t>(1, kCus / std::max<int64_t>(tiles, 1));
+  const int64_t most = std::max<int64_t>(1, kt * (np == 1 ? 1 : 6) / 4);
+  int64_t s = std::min({want, most, kt, int64_t(64)});
+  return div_up(kt, div_up(kt, s));  // no split without a step
+}
+
+bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& p) {
+  // launches stay below 2^32 threads
+  if (N < 0 || H <= 0 || V <= 0 || N > (int64_t(1) << 24) || H > (int64_t(1) << 16) || V > (int64_t(1) << 26) ||
+      N * H > (int64_t(1) << 35) || V * H > (int64_t(1) << 35))
+    return false;
+  if (dtype != GNCDE_DTYPE_FP32 && dtype != GNCDE_DTYPE_BF16) return false;
+  p = Plan{};
+  p.N = N, p.H = H, p.V = V;
+  p.f32 = dtype == GNCDE_DTYPE_FP32;
+  p.np = p.f32 ? 3 : 1;
+  p.direct_ok = !p.f32 && H % 8 == 0;
+  p.Kp = up(H, 64), p.Np = up(std::max<int64_t>(N, 1), 64);
+  const int64_t plane = 2 * p.np;
+  // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
+  const int64_t per_class = grad ? plane * (2 * p.Np + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
+  p.piece = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256));
+  // W as it lies may still be unusable (its address): the packed piece has its place in any case.
+  p.o_x = p.take(plane * N * p.Kp);
+  p.o_w = p.take(plane * std::min(p.piece, V) * p.Kp);
+  if (!grad) {
+    p.o_part = p.take(8 * N * (p.piece / 128));
+    p.o_party = p.take(8 * N * (p.piece / 128));
+    p.o_hit = p.take(4 * N);
+    p.o_run = p.take(16 * N);
+  } else {
+    p.o_xt = p.take(plane * H * p.Np);
+    p.o_wt = p.take(plane * H * p.piece);
+    p.o_p = p.take(plane * N * p.piece);
+    p.o_pt = p.take(plane * p.piece * p.Np);
+    p.ldacc = up(H, 4);
+    const int64_t vc = std::min(p.piece, V);
+    p.gx_split = split_of(H, N, div_up(vc, kBK), p.np);
+    p.gw_split = split_of(H, vc, p.Np / kBK, p.np);
+    p.o_gx = p.take(4 * p.gx_split * N * p.ldacc);
+    p.o_gw = p.take(p.gw_split > 1 ? 4 * p.gw_split * vc * p.ldacc : 0);
+    p.o_b = p.take(4 * 4 * div_up(N, 256) * vc);  // tile columns times waves across, of either tile size
+  }
+  return true;
+}
+
+template <int EPI, bool F32>
+void mm(const GemmArgs& in, int64_t splits, hipStream_t st) {
+  constexpr int NP = F32 ? 3 : 1;
+  GemmArgs a = in;
+  const Tile t = tile_of(a.M, a.N);
+  a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
+  a.kt = (int)div_up(a.K, kBK);
+  a.per_split = (int)div_up(a.kt, splits);
+  const dim3 grid((unsigned)(a.tm * a.tn), (unsigned)splits);
+  if (t.big) hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
+}
+
+template <bool F32>
+void pack(const void* src, int64_t R, const Plan& p, uint16_t* dst, hipStream_t st) {
+  const int64_t n = R * (p.Kp / 8);
+  hipLaunchKernelGGL((k_xent_pack<F32, F32 ? 3 : 1>), dim3((unsigned)std::min(div_up(n, 256), kMostBlocks)),
+                     dim3(256), 0, st, src, R,
+                     (int)p.H, (int)p.Kp, dst);
+}
+
+template <bool F32, bool LEFT>
+void pack_t(const void* src, int64_t R, int64_t Rp, const Plan& p, Rows rows, uint16_t* dst, hipStream_t st) {
+  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)(Rp / 64 * div_up(p.H, 64))), dim3(256),
+                     0, st, src, R, (int)p.H, Rp, rows, dst);
+}
+
+bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+struct Call {
+  const void *x, *W, *b;
+  Rows rows;
+  char* ws;
+  hipStream_t st;
+};
+
+template <bool F32>
+struct Operand {
+  const uint16_t* p;
+  int64_t ld, plane;
+  int K;
+};
+
+// x or a piece of W as the product's operand: as it lies where its rows start on 16 bytes, else packed.
+template <bool F32>
+Operand<F32> operand(const void* src, int64_t R, const Plan& p, int64_t at, const Call& c) {
+  if (p.direct_ok && aligned(src, 16)) return {static_cast<const uint16_t*>(src), p.H, 0, (int)p.H};
+  uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + at);
+  pack<F32>(src, R, p, dst, c.st);
+  return {dst, p.Kp, R * p.Kp, (int)p.Kp};
+}
+
+template <bool F32>
+GemmArgs logits_args(const Operand<F32>& w, const Operand<F32>& x, const Plan& p, const Call& c, int64_t v0,
+                     int64_t vc) {
+  GemmArgs a = {};
+  a.A = w.p, a.lda = w.ld, a.sa = w.plane, a.M = vc;
+  a.B = x.p, a.ldb = x.ld, a.sb = x.plane, a.N = p.N;
+  // one of the two may be packed (zeros behind H) and the other not
+  a.K = std::min(w.K, x.K);
+  a.rows = c.rows;
+  a.bias = c.b ? static_cast<const char*>(c.b) + v0 * (F32 ? 4 : 2) : nullptr;
+  a.v0 = v0, a.V = p.V;
+  return a;
+}
+
+template <bool F32>
+void forward(const Plan& p, const Call& c, float* loss, float* stats) {
+  const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
+  for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
+    const int64_t vc = std::min(p.piece, p.V - v0);
+    const Operand<F32> w =
+        operand<F32>(static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, p, p.o_w, c);
+    GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
+    a.part = reinterpret_cast<float2*>(c.ws + p.o_part);
+    a.part_y = reinterpret_cast<float2*>(c.ws + p.o_party);
+    a.hit = reinterpret_cast<float*>(c.ws + p.o_hit);
+    mm<E_LSE, F32>(a, 1, c.st);
+    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, c.st, p.N,
+                       div_up(vc, tile_of(vc, p.N).bm), a.part,
+                       c.rows.kind == GNCDE_TARGET_ROWS ? a.part_y : nullptr, a.hit, c.rows, p.V,
+                       reinterpret_cast<float4*>(c.ws + p.o_run), v0 == 0, v0 + p.piece >= p.V, loss, stats);
+  }
+}
+
+template <bool F32>
+void sum_out(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t ldacc, int64_t stride, void* out,
+             int64_t ldo, hipStream_t st) {
+  hipLaunchKernelGGL((k_xent_sum<F32>), dim3((unsigned)std::min(div_up(N * M, 256), kMostBlocks)), dim3(256), 0, st, N,
+                     M, (int)splits, acc, ldacc, stride, out, ldo);
+}
+
+template <bool F32>
+void backward(const Plan& p, const Call& c, const float* stats, const float* g, void* gx, void* gW, void* gb) {
+  constexpr int64_t SZ = F32 ? 4 : 2;
+  const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
+  uint16_t* xt = reinterpret_cast<uint16_t*>(c.ws + p.o_xt);
+  uint16_t* wt = reinterpret_cast<uint16_t*>(c.ws + p.o_wt);
+  uint16_t* P = reinterpret_cast<uint16_t*>(c.ws + p.o_p);
+  uint16_t* Pt = reinterpret_cast<uint16_t*>(c.ws + p.o_pt);
+  float* acc_x = reinterpret_cast<float*>(c.ws + p.o_gx);
+  float* acc_w = reinterpret_cast<float*>(c.ws + p.o_gw);
+  float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
+  if (gW) pack_t<F32, true>(c.x, p.N, p.Np, p, c.rows, xt, c.st);
+  const bool one = p.piece >= p.V;
+  for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
+    const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, 64);
+    const char* wsrc = static_cast<const char*>(c.W) + v0 * p.H * SZ;
+    const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
+    GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
+    a.stats = stats, a.g = g;
+    a.P = P, a.ldp = vp, a.sp = p.N * vp;
+    a.Pt = Pt, a.ldpt = p.Np, a.spt = vc * p.Np;
+    a.part_b = gb ? part_b : nullptr;
+    mm<E_DL, F32>(a, 1, c.st);
+    if (gb) {
+      const Tile t = tile_of(vc, p.N);
+      sum_out<F32>(1, vc, div_up(p.N, t.bn) * t.wn, part_b, vc, vc, static_cast<char*>(gb) + v0 * SZ, vc, c.st);
+    }
+    if (gx) {
+      pack_t<F32, false>(wsrc, vc, vp, p, c.rows, wt, c.st);
+      GemmArgs q = {};
+      q.A = wt, q.lda = vp, q.sa = p.H * vp, q.M = p.H;
+      q.B = P, q.ldb = vp, q.sb = p.N * vp, q.N = p.N;
+      q.K = (int)vp;
+      q.out = gx, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(gx, 4 * SZ);
+      const int64_t sp = split_of(p.H, p.N, vp / kBK, p.np);
+      // every piece's splits fill the same sums; the last piece may have fewer steps, and leaves the others as they are
+      const bool sums = !one || sp > 1;
+      if (sums) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
+      const int64_t use = std::min(sp, p.gx_split);
+      mm<E_OUT, F32>(q, use, c.st);
+      if (sums && v0 + p.piece >= p.V)
+        sum_out<F32>(p.N, p.H, one ? use : p.gx_split, acc_x, p.ldacc, p.N * p.ldacc, gx, p.H, c.st);
+    }
+    if (gW) {
+      GemmArgs q = {};
+      q.A = xt, q.lda = p.Np, q.sa = p.H * p.Np, q.M = p.H;
+      q.B = Pt, q.ldb = p.Np, q.sb = vc * p.Np, q.N = vc;
+      q.K = (int)p.Np;
+      char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
+      q.out = out, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(out, 4 * SZ);
+      const int64_t sp = std::min(split_of(p.H, vc, p.Np / kBK, p.np), p.gw_split);
+      if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
+      mm<E_OUT, F32>(q, sp, c.st);
+      if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, out, p.H, c.st);
+    }
+  }
+}
+
+int check(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype, const void* x, const void* W, const void* b,
+          int32_t kind, const void* target, bool grad, const void* ws, size_t ws_bytes, Plan& p) {
+  if (rows < 0 || hidden <= 0 || classes <= 0) return GNCDE_ERR_SHAPE;
+  if (kind < GNCDE_TARGET_INDEX32 || kind > GNCDE_TARGET_ROWS) return GNCDE_ERR_ARG;
+  if (!make_plan(rows, hidden, classes, dtype, grad, p)) return GNCDE_ERR_UNSUPPORTED;
+  const int64_t sz = p.f32 ? 4 : 2, tsz = kind == GNCDE_TARGET_INDEX64 ? 8 : 4;
+  if (!W || !aligned(W, sz) || !aligned(b, sz)) return GNCDE_ERR_ARG;
+  if (rows > 0 && (!x || !target || !aligned(x, sz) || !aligned(target, tsz))) return GNCDE_ERR_ARG;
+  if (rows > 0 && (!ws || !aligned(ws, 256) || ws_bytes < (size_t)p.bytes)) return GNCDE_ERR_WORKSPACE;
+  return GNCDE_OK;
+}
+
+}  // namespace
+}  // namespace gncde
+
+extern "C" {
+
+size_t gncde_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype,
+                                                  int32_t grad) {
+  gncde::Plan p;
+  return gncde::make_plan(rows, hidden, classes, dtype, grad != 0, p) ? (size_t)p.bytes : 0;
+}
+
+int gncde_linear_cross_entropy(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype, const void* x,
+                               const void* W, const void* b, int32_t target_kind, const void* target,
+                               const uint8_t* mask, float* loss, float* stats, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  gncde::Plan p;
+  const int rc = gncde::check(rows, hidden, classes, dtype, x, W, b, target_kind, target, false, workspace,
+                              workspace_bytes, p);
+  if (rc != GNCDE_OK) return rc;
+  if (rows == 0) return GNCDE_OK;
+  if (!loss || !stats) return GNCDE_ERR_ARG;
+  const gncde::Call c{x, W, b, {target, mask, target_kind}, static_cast<char*>(workspace),
+                      static_cast<hipStream_t>(stream)};
+  if (p.f32) gncde::forward<true>(p, c, loss, stats);
+  else gncde::forward<false>(p, c, loss, stats);
+  return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
+}
+
+int gncde_linear_cross_entropy_grad(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype, const void* x,
+                                    const void* W, const void* b, int32_t target_kind, const void* target,
+                                    const uint8_t* mask, const float* stats, const float* g, void* gx, void* gW,
+                                    void* gb, void* workspace, size_t workspace_bytes, void* stream) {
+  gncde::Plan p;
+  const int rc = gncde::check(rows, hidden, classes, dtype, x, W, b, target_kind, target, true, workspace,
+                              workspace_bytes, p);
+  if (rc != GNCDE_OK) return rc;
+  const int64_t sz = p.f32 ? 4 : 2;
+  if (!gncde::aligned(gx, sz) || !gncde::aligned(gW, sz) || !gncde::aligned(gb, sz)) return GNCDE_ERR_ARG;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows == 0) {  // no row: gradients of nothing
+    if (p.f32) {
+      if (gW) gncde::sum_out<true>(classes, hidden, 0, nullptr, 0, 0, gW, hidden, st);
+      if (gb) gncde::sum_out<true>(1, classes, 0, nullptr, 0, 0, gb, classes, st);
+    } else {
+      if (gW) gncde::sum_out<false>(classes, hidden, 0, nullptr, 0, 0, gW, hidden, st);
+      if (gb) gncde::sum_out<false>(1, classes, 0, nullptr, 0, 0, gb, classes, st);
+    }
+    return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
+  }
+  if (!stats || !g) return GNCDE_ERR_ARG;
+  if (!gx && !gW && !gb) return GNCDE_OK;
+  const gncde::Call c{x, W, b, {target, mask, target_kind}, static_cast<char*>(workspace), st};
+  if (p.f32) gncde::backward<true>(p, c, stats, g, gx, gW, gb);
+  else gncde::backward<false>(p, c, stats, g, gx, gW, gb);
+  return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
+}
+
+}  // extern "C"

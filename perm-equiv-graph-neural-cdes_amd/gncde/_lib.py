@@ -49,6 +49,12 @@ EXPORTED_SYMBOLS = (
     "gncde_node_affine_grad",
     "gncde_adamw_workspace_bytes",
     "gncde_clip_adamw",
+    "gncde_global_norm_workspace_bytes",
+    "gncde_global_norm",
+    "gncde_clip_by_global_norm",
+    "gncde_linear_cross_entropy_workspace_bytes",
+    "gncde_linear_cross_entropy",
+    "gncde_linear_cross_entropy_grad",
     "gncde_interval_index",
     "gncde_graph_operator",
     "gncde_hermite_coefficients",
@@ -100,6 +106,20 @@ class GncdeSolver(ctypes.Structure):
         ("act_rec_len", ctypes.c_int64),
         ("pid_ckpt", c_void_p),
         ("rec_steps", c_int32),
+    ]
+
+
+TARGET_INDEX32, TARGET_INDEX64, TARGET_ROWS = 0, 1, 2  # GNCDE_TARGET_*
+DTYPE_FP32, DTYPE_BF16, DTYPE_FP16 = 0, 1, 2  # GNCDE_DTYPE_*
+
+
+class GncdeTensor(ctypes.Structure):
+    _fields_ = [
+        ("inp", c_void_p),
+        ("out", c_void_p),
+        ("numel", ctypes.c_int64),
+        ("dtype", c_int32),
+        ("reserved", c_int32),
     ]
 
 
@@ -208,6 +228,22 @@ def load(path: str | None = None):
     lib.gncde_clip_adamw.restype = c_int32
     lib.gncde_clip_adamw.argtypes = [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_float, c_float,
                                      c_float, c_float, c_float, c_float, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.gncde_global_norm_workspace_bytes.restype = c_size_t
+    lib.gncde_global_norm_workspace_bytes.argtypes = [c_int32]
+    lib.gncde_global_norm.restype = c_int32
+    lib.gncde_global_norm.argtypes = [c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.gncde_clip_by_global_norm.restype = c_int32
+    lib.gncde_clip_by_global_norm.argtypes = [c_int32, c_void_p, c_float, c_void_p, c_void_p, c_size_t, c_void_p]
+    i64 = ctypes.c_int64
+    lib.gncde_linear_cross_entropy_workspace_bytes.restype = c_size_t
+    lib.gncde_linear_cross_entropy_workspace_bytes.argtypes = [i64, i64, i64, c_int32, c_int32]
+    lib.gncde_linear_cross_entropy.restype = c_int32
+    lib.gncde_linear_cross_entropy.argtypes = [i64, i64, i64, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
+                                               c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.gncde_linear_cross_entropy_grad.restype = c_int32
+    lib.gncde_linear_cross_entropy_grad.argtypes = [i64, i64, i64, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
+                                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                    c_void_p, c_void_p, c_size_t, c_void_p]
     lib.gncde_interval_index.restype = c_int32
     lib.gncde_interval_index.argtypes = [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
                                          c_void_p]

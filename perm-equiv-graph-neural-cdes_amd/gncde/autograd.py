@@ -322,3 +322,28 @@ def node_affine(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | None) -> tor
     """Differentiable per-node affine map (eqx.nn.Linear under vmap) on gncde_node_affine(_grad)."""
     return _NodeAffine.apply(x.to(torch.float32), W.to(device=x.device, dtype=torch.float32),
                              None if b is None else b.to(device=x.device, dtype=torch.float32))
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, b, target, mask):
+        loss, stats = engine.linear_cross_entropy(x, W, b, target, mask)
+        ctx.save_for_backward(x, W, b, target, mask, stats)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, W, b, target, mask, stats = ctx.saved_tensors
+        gx, gW, gb = engine.linear_cross_entropy_grad(x, W, b, target, stats, g, mask, *ctx.needs_input_grad[:3])
+        return gx, gW, gb, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | None, target: torch.Tensor,
+                         mask: torch.Tensor | None = None) -> torch.Tensor:
+    """Differentiable (w.r.t. x, W, b) cross-entropy of the read-out ``x @ W.T + b`` per row, fp32 [...]: the logits are
+    never stored (engine.linear_cross_entropy, whose arguments these are).  Labels are data: label rows that require a
+    gradient are refused."""
+    if target.requires_grad:
+        raise _lib.GncdeError("linear_cross_entropy: no gradient with respect to the labels")
+    return _LinearCrossEntropy.apply(x, W, b, target, mask)

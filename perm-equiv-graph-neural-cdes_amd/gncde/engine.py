@@ -7,10 +7,12 @@ torch's current stream.  Errors from the library raise ``GncdeError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 from dataclasses import dataclass, field
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -24,6 +26,11 @@ def _require_gpu():
 
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+def _on(dev: torch.device):
+    """The tensors' device made current (entered only where it is not: their stream is that device's)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _stream():
@@ -379,6 +386,183 @@ def clip_adamw(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: to
     _lib.check(lib.gncde_clip_adamw(P, _ptr(params), _ptr(grads), _ptr(m), _ptr(v), int(step), lr, b1, b2, eps,
                                     weight_decay, max_norm, _ptr(stats), _ptr(ws), nbytes, _stream()))
     return stats
+
+
+_READOUT_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _readout_args(name: str, x, W, b, target, mask):
+    """Checked (rows, hidden, classes, dtype, x, W, b, target kind, target, mask) of the read-out's cross-entropy."""
+    kind = _READOUT_DTYPES.get(x.dtype)
+    if kind is None or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
+        raise _lib.GncdeError(f"{name}: x, W and b must all be fp32 or all be bf16 (got {x.dtype}, {W.dtype}"
+                              f"{'' if b is None else f', {b.dtype}'})")
+    if x.dim() < 1 or W.dim() != 2 or x.shape[-1] != W.shape[1] or W.numel() == 0:
+        raise _lib.GncdeError(f"{name}: x {tuple(x.shape)} [..., hidden] does not fit W {tuple(W.shape)} "
+                              "[classes, hidden]")
+    hidden, classes = int(W.shape[1]), int(W.shape[0])
+    rows = x.numel() // hidden
+    lead = tuple(x.shape[:-1])
+    if b is not None and tuple(b.shape) != (classes,):
+        raise _lib.GncdeError(f"{name}: b {tuple(b.shape)} must be [{classes}]")
+    if target.dtype in (torch.int32, torch.int64):
+        tkind = _lib.TARGET_INDEX32 if target.dtype == torch.int32 else _lib.TARGET_INDEX64
+        if tuple(target.shape) != lead:
+            raise _lib.GncdeError(f"{name}: class indices {tuple(target.shape)} must be {lead}")
+    elif target.dtype == torch.float32:
+        tkind = _lib.TARGET_ROWS
+        if tuple(target.shape) != lead + (classes,):
+            raise _lib.GncdeError(f"{name}: label rows {tuple(target.shape)} must be {lead + (classes,)}")
+    else:
+        raise _lib.GncdeError(f"{name}: target must be int32 / int64 class indices or fp32 label rows, got "
+                              f"{target.dtype}")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != lead):
+        raise _lib.GncdeError(f"{name}: mask must be bool {lead}, got {mask.dtype} {tuple(mask.shape)}")
+    for t in (x, W, b, target, mask):
+        if t is not None and (t.device.type != "cuda" or t.device != x.device):
+            raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
+    return (rows, hidden, classes, kind, x.contiguous(), W.contiguous(), None if b is None else b.contiguous(), tkind,
+            target.contiguous(), None if mask is None else mask.contiguous())
+
+
+def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | None, target: torch.Tensor,
+                         mask: torch.Tensor | None = None):
+    """Softmax cross-entropy of the read-out ``x @ W.T + b`` without its logits in memory: (loss [...], stats [..., 2])
+    in fp32 (trainer_tgb.cross_entropy_loss per row, trainer_tgb.py:42-60).
+
+    x [..., hidden], W [classes, hidden], b [classes] or None: fp32 or bf16, all the same.  target: class indices [...]
+    (int32 / int64; a negative one leaves its row out, one past the last class makes the row NaN) or label rows
+    [..., classes] fp32, of any mass.  mask [...] bool: False leaves the row out; its loss is 0 and its values change
+    nothing.  ``stats`` holds each row's (log of the summed exponentials, label mass) for
+    ``linear_cross_entropy_grad``."""
+    args = _readout_args("linear_cross_entropy", x, W, b, target, mask)
+    _require_gpu()
+    lib = _lib.load()
+    rows, hidden, classes, kind, x, W, b, tkind, target, mask = args
+    with _on(x.device):
+        loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=x.device)
+        nbytes = lib.gncde_linear_cross_entropy_workspace_bytes(rows, hidden, classes, kind, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.gncde_linear_cross_entropy(rows, hidden, classes, kind, _ptr(x), _ptr(W), _ptr(b), tkind,
+                                                  _ptr(target), _ptr(mask), _ptr(loss), _ptr(stats), _ptr(ws), nbytes,
+                                                  _stream()))
+    return loss, stats
+
+
+def linear_cross_entropy_grad(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | None, target: torch.Tensor,
+                              stats: torch.Tensor, g: torch.Tensor, mask: torch.Tensor | None = None, need_x=True,
+                              need_w=True, need_b=True):
+    """Reverse mode of ``linear_cross_entropy`` for the rows' cotangents g [...] fp32: (gx, gW, gb) in x's type (None
+    where not needed; gb None without b)."""
+    args = _readout_args("linear_cross_entropy_grad", x, W, b, target, mask)
+    rows, hidden, classes, kind, x, W, b, tkind, target, mask = args
+    lead = tuple(x.shape[:-1])
+    if stats.dtype != torch.float32 or tuple(stats.shape) != lead + (2,) or stats.device != x.device:
+        raise _lib.GncdeError(f"linear_cross_entropy_grad: stats must be the loss's fp32 {lead + (2,)}")
+    if g.dtype != torch.float32 or tuple(g.shape) != lead or g.device != x.device:
+        raise _lib.GncdeError(f"linear_cross_entropy_grad: g must be fp32 {lead}, got {g.dtype} {tuple(g.shape)}")
+    _require_gpu()
+    lib = _lib.load()
+    with _on(x.device):
+        stats, g = stats.contiguous(), g.contiguous()
+        gx = torch.empty_like(x) if need_x else None
+        gW = torch.empty_like(W) if need_w else None
+        gb = torch.empty_like(b) if need_b and b is not None else None
+        nbytes = lib.gncde_linear_cross_entropy_workspace_bytes(rows, hidden, classes, kind, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.gncde_linear_cross_entropy_grad(rows, hidden, classes, kind, _ptr(x), _ptr(W), _ptr(b), tkind,
+                                                       _ptr(target), _ptr(mask), _ptr(stats), _ptr(g), _ptr(gx),
+                                                       _ptr(gW), _ptr(gb), _ptr(ws), nbytes, _stream()))
+    return gx, gW, gb
+
+
+_LIST_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+
+
+def _tensor_table(name: str, tensors, out=None):
+    """(host array of GncdeTensor, kept tensors, device) of a tensor list, checked."""
+    if torch.is_tensor(tensors):
+        raise _lib.GncdeError(f"{name}: a list of tensors is wanted, not one tensor")
+    tensors = list(tensors)
+    if not tensors:
+        raise _lib.GncdeError(f"{name}: an empty list of tensors")
+    dev = tensors[0].device
+    kinds = [_LIST_DTYPES.get(t.dtype) for t in tensors]
+    if None in kinds:
+        raise _lib.GncdeError(f"{name}: tensors must be fp32, bf16 or fp16, got {tensors[kinds.index(None)].dtype}")
+    if dev.type != "cuda" or any(t.device != dev for t in tensors):
+        raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
+    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    rows = np.zeros((len(tensors), 4), dtype=np.int64)  # GncdeTensor: in, out, numel, dtype (+ reserved 0)
+    rows[:, 0] = [t.data_ptr() for t in tensors]
+    rows[:, 2] = [t.numel() for t in tensors]
+    rows[:, 3] = kinds
+    if out is not None:
+        if len(out) != len(tensors):
+            raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
+        for t, o in zip(tensors, out):
+            if o.dtype != t.dtype or o.shape != t.shape or o.device != dev or not o.is_contiguous():
+                raise _lib.GncdeError(f"{name}: an output must be contiguous, of its tensor's type, shape and device")
+        rows[:, 1] = [o.data_ptr() for o in out]
+        _refuse_overlap(name, rows, [t.element_size() for t in tensors])
+    return rows, tensors, dev
+
+
+def _refuse_overlap(name: str, rows, sizes):
+    """Outputs that meet each other, or a tensor that is not their own, would be written while they are read."""
+    bytes_ = rows[:, 2] * np.asarray(sizes, dtype=np.int64)
+    live = bytes_ > 0
+    out, end = rows[live, 1], rows[live, 1] + bytes_[live]
+    order = np.argsort(out, kind="stable")
+    lo, hi = out[order], end[order]
+    if np.any(lo[1:] < hi[:-1]):
+        raise _lib.GncdeError(f"{name}: two outputs share memory (the same tensor twice?)")
+    src, stop = rows[live, 0], rows[live, 0] + bytes_[live]
+    # outputs are disjoint, so those that meet [src, stop) are a run of the sorted order
+    first = np.searchsorted(hi, src, side="right")
+    last = np.searchsorted(lo, stop, side="left")
+    met = last - first
+    own = (src == out)
+    if np.any(met > own):
+        raise _lib.GncdeError(f"{name}: an output shares memory with a tensor that is not its own")
+
+
+def global_norm(tensors) -> torch.Tensor:
+    """Device stats [2] = (global L2 norm, largest magnitude) over a list of fp32 / bf16 / fp16 CUDA tensors of any
+    sizes, on the tensors' device and torch's current stream there (squares and sums in 64 bits; NaN anywhere makes
+    both NaN)."""
+    _require_gpu()
+    lib = _lib.load()
+    rows, kept, dev = _tensor_table("global_norm", tensors)
+    with _on(dev):
+        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        nbytes = lib.gncde_global_norm_workspace_bytes(len(kept))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.check(lib.gncde_global_norm(len(kept), rows.ctypes.data, _ptr(stats), _ptr(ws), nbytes, _stream()))
+    return stats
+
+
+def clip_by_global_norm(tensors, max_norm: float, out=None):
+    """``optax.clip_by_global_norm(max_norm)`` (optimiser_configs.py:76-84) over a list of tensors: (clipped list,
+    device stats [2] of the list before clipping, as ``global_norm``).  ``out``: the list the clipped tensors are written
+    to (``out=tensors`` clips in place); new tensors without it."""
+    _require_gpu()
+    lib = _lib.load()
+    max_norm = float(max_norm)
+    if not 0.0 < max_norm < float("inf"):
+        raise _lib.GncdeError(f"clip_by_global_norm: max_norm {max_norm} must be positive and finite")
+    tensors = list(tensors) if not torch.is_tensor(tensors) else tensors
+    if out is None and not torch.is_tensor(tensors):
+        out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors]
+    rows, kept, dev = _tensor_table("clip_by_global_norm", tensors, out)
+    with _on(dev):
+        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        nbytes = lib.gncde_global_norm_workspace_bytes(len(kept))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.check(lib.gncde_clip_by_global_norm(len(kept), rows.ctypes.data, max_norm, _ptr(stats), _ptr(ws),
+                                                 nbytes, _stream()))
+    return out, stats
 
 
 _OPERATORS = {"norm_lap": _lib.OP_NORM_LAP, "norm_adj": _lib.OP_NORM_ADJ, "kipf": _lib.OP_KIPF,

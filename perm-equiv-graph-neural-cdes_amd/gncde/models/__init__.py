@@ -260,10 +260,13 @@ class TGBGraphNeuralCDE(nn.Module):
     GNCDE_COMPUTE_*).  "bf16_storage" is config 5's bf16 path: bfloat16 operator coefficients (half the form's
     coefficient stream) read by the persistent adaptive solve with fp32 products, so the PID controller sees no
     rounding noise.  The single-plane "bf16_mfma" mode is not offered here: it deviates 8-24 % from
-    fp32 at no speed-up (round-4 measurements) and the PID controller refuses it."""
+    fp32 at no speed-up (round-4 measurements) and the PID controller refuses it.
+
+    ``readout_loss`` (build extension): "logits" | "fused".  "fused" computes ``loss_terms`` with
+    ``autograd.linear_cross_entropy``: the decoder's [B, n, n] logits and their gradient are never stored."""
 
     def __init__(self, cfg, vector_field, interpolation="cubic", model_key=None, dt0=0.01, solver=None,
-                 compute="fp32", **kwargs):
+                 compute="fp32", readout_loss="logits", **kwargs):
         super().__init__()
         self.cfg = _cfg(cfg, hidden_dim=32, method="Tsit5", return_sequence=False, use_mlps=False)
         if getattr(self.cfg, "use_mlps", False):
@@ -285,9 +288,16 @@ class TGBGraphNeuralCDE(nn.Module):
             raise ValueError(f"compute {compute!r}: 'fp32', 'bf16' or 'bf16_storage' (the single-plane 'bf16_mfma' "
                              "mode is retired from the TGB model: 8-24 % from fp32 at no speed-up, DESIGN.md §3.5)")
         self.compute = compute
+        if readout_loss not in ("logits", "fused"):
+            raise ValueError(f"readout_loss {readout_loss!r}: 'logits' or 'fused'")
+        self.readout_loss = readout_loss
         self.last_steps = None
 
     def batched(self, ts, coeffs_adj, x_data, x0, start_time=None, evolving_out=False):
+        return _affine(self.decoder, self._states(ts, coeffs_adj, x_data, x0, evolving_out))
+
+    def _states(self, ts, coeffs_adj, x_data, x0, evolving_out=False):
+        """The node states [B, n, h] at t1, before the decoder."""
         if evolving_out:
             raise NotImplementedError("SaveAt(ts) with ConstantStepSize (dense output) is not implemented")
         control_adj = _control(ts, coeffs_adj)
@@ -323,11 +333,17 @@ class TGBGraphNeuralCDE(nn.Module):
             ys = engine.integrate(prob, spec, y0)
         if self.adaptive:
             self.last_steps = spec.stats_out[:, _lib.STAT_STEPS]
-        return _affine(self.decoder, ys)
+        return ys
 
     def loss_terms(self, ts, coeffs_adj, x_data, x0, labels, source_mask):
         """(sum of masked cross-entropies, number of unmasked rows) of trainer_tgb.cross_entropy_loss
         (trainer_tgb.py:42-60): -sum(label * log_softmax(pred)) per node, rows where source_mask is True."""
+        if self.readout_loss == "fused":
+            ys = self._states(ts, coeffs_adj, x_data, x0)
+            W, b = self.decoder.weight, self.decoder.bias
+            labels = torch.as_tensor(labels, dtype=torch.float32, device=ys.device).reshape(*ys.shape[:-1], W.shape[0])
+            mask = torch.as_tensor(source_mask, device=ys.device).reshape(ys.shape[:-1]).to(torch.bool)
+            return autograd.linear_cross_entropy(ys, W, b, labels, mask).sum(), mask.sum().to(ys.dtype)
         pred = self.batched(ts, coeffs_adj, x_data, x0)
         labels = torch.as_tensor(labels, dtype=torch.float32, device=pred.device).reshape(pred.shape)
         mask = torch.as_tensor(source_mask, device=pred.device).reshape(pred.shape[:-1]).to(pred.dtype)

@@ -270,9 +270,11 @@ class WindowTrainer:
             # build-only model key `solver: pid` (BASELINE config 5's adaptive Tsit5); absent: the reference's
             # ConstantStepSize(0.01)
             # build-only key `compute` ("fp32" | "bf16" | "bf16_storage"): the solve's arithmetic
-            model = TGBGraphNeuralCDE({k: v for k, v in m.items() if k not in ("solver", "compute")}, vf,
-                                      m.get("interpolation", "cubic"), self.seed, solver=m.get("solver"),
-                                      compute=m.get("compute", "fp32"))
+            # build-only key `readout_loss` ("logits" | "fused"): how the cross-entropy is computed
+            model = TGBGraphNeuralCDE({k: v for k, v in m.items() if k not in ("solver", "compute", "readout_loss")},
+                                      vf, m.get("interpolation", "cubic"), self.seed, solver=m.get("solver"),
+                                      compute=m.get("compute", "fp32"),
+                                      readout_loss=m.get("readout_loss", "logits"))
         else:
             model = PGTGraphNeuralCDE(m, vf, m.get("interpolation", "cubic"), self.seed)
         return ds, model.to("cuda")

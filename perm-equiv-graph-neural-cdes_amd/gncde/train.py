@@ -136,7 +136,57 @@ class ClipAdamW:
                                  self.eps, self.wd, self.max_norm)
 
 
-def make_step(opt: ClipAdamW, loss_terms, *args, **kwargs):
+class ClippedOptimiser:
+    """``optax.chain(optax.clip_by_global_norm(max_norm), <optimiser>)`` for any ``torch.optim.Optimizer`` (the
+    reference's OptimiserCfg.build wraps adam, adamw and sgd alike, optimiser_configs.py:70-88), with ``ClipAdamW``'s
+    interface for ``make_step``.  The parameters stay where they are, in their own types; the norm and the clipping run
+    on gncde_clip_by_global_norm over the parameters' gradients as they lie (``max_norm`` None: the norm alone)."""
+
+    def __init__(self, optimiser: torch.optim.Optimizer, max_norm: float | None = 1.0):
+        self.optimiser = optimiser
+        self.params = [p for grp in optimiser.param_groups for p in grp["params"] if p.requires_grad]
+        if not self.params:
+            raise ValueError("no trainable parameters")
+        dev = self.params[0].device
+        if dev.type != "cuda" or any(p.device != dev for p in self.params):
+            raise ValueError("ClippedOptimiser: move the model to one GPU first (model.to('cuda'))")
+        if max_norm is not None and not 0.0 < max_norm < float("inf"):
+            raise ValueError(f"max_norm {max_norm}: positive and finite, or None")
+        self.max_norm = max_norm
+
+    def zero_grad(self):
+        self.optimiser.zero_grad(set_to_none=True)
+
+    def flat_grad(self) -> torch.Tensor:
+        return torch.cat([p.grad.reshape(-1).to(torch.float32) if p.grad is not None
+                          else torch.zeros(p.numel(), dtype=torch.float32, device=p.device) for p in self.params])
+
+    def clip(self) -> torch.Tensor:
+        """Clip the parameters' gradients in place; device stats (global norm, max|grad|) of what they were."""
+        grads = [p.grad for p in self.params if p.grad is not None]
+        if not grads:
+            return torch.zeros(2, dtype=torch.float32, device=self.params[0].device)
+        if self.max_norm is None:
+            return engine.global_norm(grads)
+        return engine.clip_by_global_norm(grads, self.max_norm, out=grads)[1]
+
+    def step(self, flat_grad: torch.Tensor) -> torch.Tensor:
+        """Apply one update from the (reduced) flat gradient; returns device stats (global grad norm, max|grad|,
+        max|update|)."""
+        off = 0
+        for p in self.params:
+            k = p.numel()
+            p.grad = flat_grad[off:off + k].view_as(p).to(p.dtype)
+            off += k
+        stats = self.clip()
+        before = [p.detach().clone() for p in self.params]
+        self.optimiser.step()
+        update = torch.stack([(p.detach() - q).abs().amax().to(torch.float32) if p.numel() else stats.new_zeros(())
+                              for p, q in zip(self.params, before)]).amax()
+        return torch.cat([stats, update.reshape(1)])
+
+
+def make_step(opt: ClipAdamW | ClippedOptimiser, loss_terms, *args, **kwargs):
     """One data-parallel training step.  ``loss_terms(*args, **kwargs)`` returns (sum of squared errors on
     this rank's shard, element count) — e.g. ``GraphNeuralCDE.loss_terms``.  Returns (loss, max|grad|,
     max|update|) like trainer.py:327 (device scalars)."""
