@@ -30,10 +30,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kBK = 64;  // contraction per step: 128 bytes, eight 16-byte chunks a row
+constexpr int kPad = 64;  // packed contractions are padded to a multiple of this
 constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 __device__ __forceinline__ float from_bf16(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
@@ -77,7 +75,14 @@ __device__ __forceinline__ float value(const void* p, int64_t i) {
   return F32 ? static_cast<const float*>(p)[i] : from_bf16(static_cast<const uint16_t*>(p)[i]);
 }
 
-// src [R, H] -> planes [NP][R][Kp], zeros behind H.
+// Packed operands: rows of Kp values (zeros behind the contraction), or for three parts rows of 3 Kp with 32 values of
+// each part side by side: value k of part q at (k / 32) * 96 + q * 32 + k % 32.
+template <int NP>
+__device__ __forceinline__ int64_t packed(int64_t k, int q) {
+  return NP == 1 ? k : (k >> 5) * 96 + q * 32 + (k & 31);
+}
+
+// src [R, H] -> packed [R][Kp].
 template <bool F32, int NP>
 __global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int Kp, uint16_t* __restrict__ dst) {
   const int cpr = Kp / 8;
@@ -93,11 +98,11 @@ __global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int 
       for (int q = 0; q < NP; ++q) o[q][i] = p[q];
     }
 #pragma unroll
-    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + ((int64_t)q * R + r) * Kp + h0) = o[q];
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + r * NP * Kp + packed<NP>(h0, q)) = o[q];
   }
 }
 
-// src [R, H] -> transposed planes [NP][H][Rp], zeros behind R and (LEFT) in rows left out, whatever they hold.
+// src [R, H] -> transposed, packed [H][Rp], zeros behind R and (LEFT) in rows left out, whatever they hold.
 template <bool F32, int NP, bool LEFT>
 __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
                                                      Rows rows, uint16_t* __restrict__ dst) {
@@ -126,7 +131,7 @@ __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ sr
       for (int q = 0; q < NP; ++q) o[q][j] = p[q];
     }
 #pragma unroll
-    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + ((int64_t)q * H + h) * Rp + r0 + rc) = o[q];
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + (int64_t)h * NP * Rp + packed<NP>(r0 + rc, q)) = o[q];
   }
 }
 
@@ -136,10 +141,10 @@ enum { E_LSE = 0, E_DL = 1, E_OUT = 2 };
 struct GemmArgs {
   const uint16_t* A;
   const uint16_t* B;
-  int64_t lda, ldb, sa, sb;  // row and plane strides in values
+  int64_t lda, ldb;          // row strides in values (of packed rows: of all parts)
   int64_t M, N;              // rows of A and of B
   int K;                     // contraction, a multiple of 8
-  int kt;                    // steps of kBK over K
+  int kt;                    // steps over K
   int per_split;             // steps a workgroup of one split takes
   int64_t tm, tn;            // tiles
   // logits
@@ -151,9 +156,9 @@ struct GemmArgs {
   float* hit;                // E_LSE, indices: [N] the target's logit
   const float* stats;        // E_DL
   const float* g;
-  uint16_t* P;               // E_DL: planes [N][ldp]
-  uint16_t* Pt;              // planes [M][ldpt]
-  int64_t ldp, ldpt, sp, spt;
+  uint16_t* P;               // E_DL: packed [N][ldp]
+  uint16_t* Pt;              // packed [M][ldpt]
+  int64_t ldp, ldpt;         // classes and rows with their padding
   float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
   // products
   void* out;                 // E_OUT: [N][ldo]
@@ -163,77 +168,116 @@ struct GemmArgs {
   int32_t vec;               // out rows can be written four values at a time
 };
 
+// One tile of C^T.  A step brings kStep values of every row of A and B into LDS: for one part 64 values, for three parts
+// 32 of each part, which lie side by side in the packed operands.  Two LDS buffers; a wave's fragments are read one
+// half-step (one part: a third of the products) before they are multiplied, and the barrier that hands a buffer over
+// lies between two runs of products whose fragments are in registers already, so neither LDS latency nor the barrier
+// leaves the matrix units idle while both waves of a SIMD keep up.
+template <int NP>
+struct Step {
+  static constexpr int K = NP == 1 ? 64 : 32;     // contraction a step
+  static constexpr int ROW = K * NP;              // values a row in LDS
+  static constexpr int CH = ROW / 8;              // 16-byte chunks a row
+  // A row's chunk c lies at place(c, row): rows that one LDS cycle reads together then differ in bank.
+  static __device__ __forceinline__ int place(int c, int row) {
+    return NP == 1 ? c ^ (row & 7) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
+  }
+};
+
+// The order within a half-step of MMS products: an LDS read behind every product or two, then LOADS loads of the step
+// after next, which the compiler keeps behind the reads.
+template <int MMS, int READS, int LOADS>
+__device__ __forceinline__ void interleave() {
+  constexpr int PER = LOADS > 0 || MMS < 2 * READS ? 1 : 2;
+  constexpr int LATER = MMS >= READS + 2 * LOADS ? 2 : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, LATER, 0);
+    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, MMS, 0);
+}
+
 template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32>
-__global__ void __launch_bounds__(WM* WN * 64, 1) k_xent_mm(GemmArgs a) {
+__global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1) k_xent_mm(GemmArgs a) {
+  typedef Step<NP> S;
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
-  constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;  // 1 KB (eight rows) loads a wave
-  static_assert(IA * 8 * NW == BM && IB * 8 * NW == BN, "tile rows divide over the waves");
-  constexpr int TILE = (BM + BN) * kBK;
-  constexpr int NSEG = NP == 1 ? 1 : 6;
+  constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
+  static_assert(IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
+  constexpr int TILE = (BM + BN) * S::ROW;
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
   // Tile of this workgroup: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the tile order,
   // and the order walks blocks of eight tiles of A by all of B: what an XCD reads at a time stays in its own cache.
-  int64_t tile_m, tile_n;
+  int tile_m, tile_n;
   {
-    const int64_t nt = a.tm * a.tn, bid = blockIdx.x;
-    const int64_t q = nt >> 3, r = nt & 7, xcd = bid & 7, idx = bid >> 3;
-    const int64_t lin = xcd * q + (xcd < r ? xcd : r) + idx;
-    const int64_t grp = lin / (8 * a.tn), in = lin - grp * 8 * a.tn;
-    const int64_t gm = a.tm - grp * 8 < 8 ? a.tm - grp * 8 : 8;
-    tile_m = grp * 8 + in % gm;
-    tile_n = in / gm;
+    const uint32_t nt = (uint32_t)(a.tm * a.tn), tn = (uint32_t)a.tn, bid = blockIdx.x;
+    const uint32_t q = nt >> 3, r = nt & 7, xcd = bid & 7;
+    const uint32_t lin = xcd * q + (xcd < r ? xcd : r) + (bid >> 3);
+    const uint32_t grp = lin / (8 * tn), in = lin - grp * 8 * tn;
+    const uint32_t left = (uint32_t)a.tm - grp * 8, gm = left < 8 ? left : 8;
+    tile_m = __builtin_amdgcn_readfirstlane((int)(grp * 8 + in % gm));
+    tile_n = __builtin_amdgcn_readfirstlane((int)(in / gm));
   }
-  const int64_t m0 = tile_m * BM, n0 = tile_n * BN;
+  const int64_t m0 = (int64_t)tile_m * BM, n0 = (int64_t)tile_n * BN;
 
-  // Each lane's source chunk: row lane / 8 of the eight, chunk (lane % 8) ^ row, so that the chunk a lane of the matrix
-  // operand reads later lies in another bank for every row.
-  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) * 8;
-  const uint16_t* pa[IA];
-  const uint16_t* pb[IB];
+  // This lane's chunks of a step, as byte offsets from the tile's first row of A or B (rows behind the last read the
+  // last one's values: their results are never written).
+  uint32_t off[IT];
+  const int col = ((lane & 7) ^ (lane >> 3)) * 8;  // one part: first value of all of them within the step
+  auto place_of = [&](int i) {  // this lane's chunk of the buffer
+    return i < IA ? (wave * IA + i) * 64 + lane : BM * S::CH + (wave * (IT - IA) + i - IA) * 64 + lane;
+  };
 #pragma unroll
-  for (int i = 0; i < IA; ++i) {
-    int64_t row = m0 + (wave * IA + i) * 8 + lr;
-    row = row < a.M ? row : a.M - 1;
-    pa[i] = a.A + row * a.lda + lc;
-  }
-#pragma unroll
-  for (int i = 0; i < IB; ++i) {
-    int64_t row = n0 + (wave * IB + i) * 8 + lr;
-    row = row < a.N ? row : a.N - 1;
-    pb[i] = a.B + row * a.ldb + lc;
+  for (int i = 0; i < IT; ++i) {
+    const int slot = place_of(i), row = slot / S::CH;
+    const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
+    const int64_t r = i < IA ? row : row - BM;
+    const int64_t most = i < IA ? a.M - 1 - m0 : a.N - 1 - n0;
+    off[i] = (uint32_t)((r < most ? r : most) * (i < IA ? a.lda : a.ldb) + c * 8) * 2u;
   }
   const int k_from = blockIdx.y * a.per_split;
   const int k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
-  const int steps = (k_to - k_from) * NSEG;
-  const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zero16);
+  // Buffer descriptors of the tile's rows; a load behind the last step goes through one of no bytes and reads nothing.
+  const uint16_t* base_a = a.A + m0 * a.lda;
+  const uint16_t* base_b = a.B + n0 * a.ldb;
 
-  auto load = [&](int s, int buf) {
-    int64_t oa = 0, ob = 0;
-    int k = s + k_from;
-    if (NSEG > 1) {
-      const int seg = s / (k_to - k_from);
-      k = s - seg * (k_to - k_from) + k_from;
-      const int ia = seg == 1 ? 2 : (seg == 2 || seg == 4) ? 1 : 0;  // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-      const int ib = seg == 0 ? 2 : (seg == 2 || seg == 3) ? 1 : 0;
-      oa = ia * a.sa;
-      ob = ib * a.sb;
+  auto load = [&](int k, int buf) {
+    const int bytes = __builtin_amdgcn_readfirstlane((k - k_to) >> 31);  // all of 2^32, or none
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
+    const uint32_t at = (uint32_t)k * (S::ROW * 2);
+    // of a ragged last step's chunks behind the end, one that is there: zeroed below
+    const uint32_t behind = k * S::K + col >= a.K ? (uint32_t)col * 2u : 0u;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      uint32_t o = off[i];
+      if (NP == 1) o -= behind;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          i < IA ? ra : rb, (__attribute__((address_space(3))) void*)(lds + buf * TILE + (place_of(i) - lane) * 8), 16, o,
+          at, 0, 0);
     }
-    const int kk = k * kBK;
-    const bool in = kk + lc < a.K;
+  };
+  // The buffer of step k is complete for every wave, and everybody has read the other one.
+  auto hand_over = [&](int k, int buf) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    if (NP == 1 && (k + 1) * S::K > a.K) {  // chunks behind the contraction's end
+      if (k * S::K + col >= a.K)
 #pragma unroll
-    for (int i = 0; i < IA; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(in ? pa[i] + oa + kk : zero),
-          (__attribute__((address_space(3))) void*)(lds + buf * TILE + (wave * IA + i) * 8 * kBK), 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < IB; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(in ? pb[i] + ob + kk : zero),
-          (__attribute__((address_space(3))) void*)(lds + buf * TILE + BM * kBK + (wave * IB + i) * 8 * kBK), 16, 0,
-          0);
+        for (int i = 0; i < IT; ++i)
+          *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i) * 8) = u16x8{};
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
 
   floatx4 acc[RT][CT];
@@ -243,31 +287,65 @@ __global__ void __launch_bounds__(WM* WN * 64, 1) k_xent_mm(GemmArgs a) {
     for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int fr = lane & 15, fk = lane >> 4;
-  const uint16_t* la = lds + (wm * (BM / WM) + fr) * kBK;
-  const uint16_t* lb = lds + BM * kBK + (wn * (BN / WN) + fr) * kBK;
-  const int c0 = ((fk) ^ (fr & 7)) * 8, c1 = ((4 + fk) ^ (fr & 7)) * 8;
+  const uint16_t* la = lds + (wm * (BM / WM) + fr) * S::ROW;
+  const uint16_t* lb = lds + (BM + wn * (BN / WN) + fr) * S::ROW;
+  // Fragment set q: of one part the half-step q, of three parts the part q.
+  auto read = [&](int q, int buf, bf16x8(&fa)[RT], bf16x8(&fb)[CT]) {
+    const int c = S::place(q * 4 + fk, fr) * 8 + buf * TILE;  // tile rows are multiples of 16: place() sees fr
+#pragma unroll
+    for (int j = 0; j < CT; ++j) fb[j] = *reinterpret_cast<const bf16x8*>(lb + j * 16 * S::ROW + c);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) fa[i] = *reinterpret_cast<const bf16x8*>(la + i * 16 * S::ROW + c);
+  };
+  auto multiply = [&](const bf16x8(&fa)[RT], const bf16x8(&fb)[CT]) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+  };
 
-  if (steps > 0) load(0, 0);
-  for (int s = 0; s < steps; ++s) {
-    const int buf = s & 1;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads are in LDS
-    __syncthreads();                     // everybody's are, and the other buffer has been read
-    if (s + 1 < steps) load(s + 1, buf ^ 1);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int c = kk ? c1 : c0;
-      bf16x8 fa[RT], fb[CT];
-#pragma unroll
-      for (int j = 0; j < CT; ++j) fb[j] = *reinterpret_cast<const bf16x8*>(lb + buf * TILE + j * 16 * kBK + c);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) fa[i] = *reinterpret_cast<const bf16x8*>(la + buf * TILE + i * 16 * kBK + c);
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < CT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+  if (k_from < k_to) {
+    load(k_from, 0);
+    hand_over(k_from, 0);
+    load(k_from + 1, 1);
+    if constexpr (NP == 1) {
+      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
+      read(0, 0, fa0, fb0);
+      for (int k = k_from; k < k_to; ++k) {
+        const int buf = (k - k_from) & 1;
+        read(1, buf, fa1, fb1);
+        multiply(fa0, fb0);
+        interleave<RT * CT, RT + CT, 0>();
+        hand_over(k + 1, buf ^ 1);
+        read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
+        load(k + 2, buf);
+        multiply(fa1, fb1);
+        interleave<RT * CT, RT + CT, IT>();
+      }
+    } else {
+      bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
+      read(1, 0, ma, mb);
+      for (int k = k_from; k < k_to; ++k) {
+        const int buf = (k - k_from) & 1;
+        read(0, buf, ha, hb);
+        multiply(ma, mb);
+        interleave<RT * CT, RT + CT, 0>();
+        read(2, buf, sa, sb);
+        multiply(ma, hb);
+        multiply(ha, mb);
+        interleave<2 * RT * CT, RT + CT, 0>();
+        hand_over(k + 1, buf ^ 1);
+        read(1, buf ^ 1, ma, mb);
+        load(k + 2, buf);
+        multiply(sa, hb);
+        multiply(ha, sb);
+        multiply(ha, hb);
+        interleave<3 * RT * CT, RT + CT, IT>();
+      }
     }
   }
+  __builtin_amdgcn_s_waitcnt(0x0070);
   __syncthreads();
 
   const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
@@ -425,14 +503,14 @@ __global__ void __launch_bounds__(WM* WN * 64, 1) k_xent_mm(GemmArgs a) {
         if (n < a.N && m < a.ldp) {
 #pragma unroll
           for (int s = 0; s < NP; ++s)
-            *reinterpret_cast<u16x4*>(a.P + s * a.sp + n * a.ldp + m) = u16x4{p[0][s], p[1][s], p[2][s], p[3][s]};
+            *reinterpret_cast<u16x4*>(a.P + n * NP * a.ldp + packed<NP>(m, s)) = u16x4{p[0][s], p[1][s], p[2][s], p[3][s]};
         }
         if (n < a.ldpt) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (m + q < a.M) {
 #pragma unroll
-              for (int s = 0; s < NP; ++s) a.Pt[s * a.spt + (m + q) * a.ldpt + n] = p[q][s];
+              for (int s = 0; s < NP; ++s) a.Pt[(m + q) * NP * a.ldpt + packed<NP>(n, s)] = p[q][s];
             }
         }
       }
@@ -450,7 +528,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 1) k_xent_mm(GemmArgs a) {
           s += __shfl_xor(s, 4);
           s += __shfl_xor(s, 8);
           const int64_t m = mb + i * 16 + q;
-          if (fr == 0 && m < a.M) a.part_b[(tile_n * WN + wn) * a.M + m] = s;
+          if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = s;
         }
     }
   }
@@ -555,25 +633,29 @@ struct Tile {
   int64_t bm, bn, wn;
 };
 
-// 256 x 256 tiles read the least per product; below one for every CU, 128 x 128 tiles keep more CUs at work.
-Tile tile_of(int64_t M, int64_t N) {
-  const bool big = div_up(M, 256) * div_up(N, 256) >= 200;
-  return big ? Tile{true, 256, 256, 4} : Tile{false, 128, 128, 2};
+// 256 x 256 tiles (three parts: 256 x 128, what LDS holds twice) read the least per product; below one for every CU,
+// 128 x 128 tiles keep more CUs at work.
+Tile tile_of(int64_t M, int64_t N, int np) {
+  const int64_t bn = np == 1 ? 256 : 128;
+  const bool big = div_up(M, 256) * div_up(N, bn) >= 200;
+  return big ? Tile{true, 256, bn, np == 1 ? 4 : 2} : Tile{false, 128, 128, 2};
 }
+
+int64_t steps_of(int64_t K, int np) { return np == 1 ? div_up(K, 64) : up(K, kPad) / 32; }
 
 // Splits of the contraction so that a product of few tiles fills the chip; at least four steps each.
 int64_t split_of(int64_t M, int64_t N, int64_t kt, int np) {
-  const Tile t = tile_of(M, N);
+  const Tile t = tile_of(M, N, np);
   const int64_t tiles = div_up(M, t.bm) * div_up(N, t.bn);
   const int64_t want = std::max<int64_t>(1, kCus / std::max<int64_t>(tiles, 1));
-  const int64_t most = std::max<int64_t>(1, kt * (np == 1 ? 1 : 6) / 4);
+  const int64_t most = std::max<int64_t>(1, kt / 4);
   int64_t s = std::min({want, most, kt, int64_t(64)});
   return div_up(kt, div_up(kt, s));  // no split without a step
 }
 
 bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& p) {
-  // launches stay below 2^32 threads
-  if (N < 0 || H <= 0 || V <= 0 || N > (int64_t(1) << 24) || H > (int64_t(1) << 16) || V > (int64_t(1) << 26) ||
+  // launches stay below 2^32 threads, and 256 rows of every operand below 2^32 bytes
+  if (N < 0 || H <= 0 || V <= 0 || N > (int64_t(1) << 21) || H > (int64_t(1) << 16) || V > (int64_t(1) << 26) ||
       N * H > (int64_t(1) << 35) || V * H > (int64_t(1) << 35))
     return false;
   if (dtype != GNCDE_DTYPE_FP32 && dtype != GNCDE_DTYPE_BF16) return false;
@@ -602,11 +684,11 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
     p.o_pt = p.take(plane * p.piece * p.Np);
     p.ldacc = up(H, 4);
     const int64_t vc = std::min(p.piece, V);
-    p.gx_split = split_of(H, N, div_up(vc, kBK), p.np);
-    p.gw_split = split_of(H, vc, p.Np / kBK, p.np);
+    p.gx_split = split_of(H, N, steps_of(vc, p.np), p.np);
+    p.gw_split = split_of(H, vc, steps_of(p.Np, p.np), p.np);
     p.o_gx = p.take(4 * p.gx_split * N * p.ldacc);
     p.o_gw = p.take(p.gw_split > 1 ? 4 * p.gw_split * vc * p.ldacc : 0);
-    p.o_b = p.take(4 * 4 * div_up(N, 256) * vc);  // tile columns times waves across, of either tile size
+    p.o_b = p.take(4 * 4 * div_up(N, 128) * vc);  // tile columns times waves across, of either tile size
   }
   return true;
 }
@@ -615,12 +697,15 @@ template <int EPI, bool F32>
 void mm(const GemmArgs& in, int64_t splits, hipStream_t st) {
   constexpr int NP = F32 ? 3 : 1;
   GemmArgs a = in;
-  const Tile t = tile_of(a.M, a.N);
+  const Tile t = tile_of(a.M, a.N, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
-  a.kt = (int)div_up(a.K, kBK);
+  a.kt = (int)steps_of(a.K, NP);
   a.per_split = (int)div_up(a.kt, splits);
   const dim3 grid((unsigned)(a.tm * a.tn), (unsigned)splits);
-  if (t.big) hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
+  if (t.big) {
+    if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
+  }
   else hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
 }
 
@@ -650,25 +735,25 @@ struct Call {
 template <bool F32>
 struct Operand {
   const uint16_t* p;
-  int64_t ld, plane;
+  int64_t ld;
   int K;
 };
 
 // x or a piece of W as the product's operand: as it lies where its rows start on 16 bytes, else packed.
 template <bool F32>
 Operand<F32> operand(const void* src, int64_t R, const Plan& p, int64_t at, const Call& c) {
-  if (p.direct_ok && aligned(src, 16)) return {static_cast<const uint16_t*>(src), p.H, 0, (int)p.H};
+  if (p.direct_ok && aligned(src, 16)) return {static_cast<const uint16_t*>(src), p.H, (int)p.H};
   uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + at);
   pack<F32>(src, R, p, dst, c.st);
-  return {dst, p.Kp, R * p.Kp, (int)p.Kp};
+  return {dst, p.np * p.Kp, (int)p.Kp};
 }
 
 template <bool F32>
 GemmArgs logits_args(const Operand<F32>& w, const Operand<F32>& x, const Plan& p, const Call& c, int64_t v0,
                      int64_t vc) {
   GemmArgs a = {};
-  a.A = w.p, a.lda = w.ld, a.sa = w.plane, a.M = vc;
-  a.B = x.p, a.ldb = x.ld, a.sb = x.plane, a.N = p.N;
+  a.A = w.p, a.lda = w.ld, a.M = vc;
+  a.B = x.p, a.ldb = x.ld, a.N = p.N;
   // one of the two may be packed (zeros behind H) and the other not
   a.K = std::min(w.K, x.K);
   a.rows = c.rows;
@@ -690,7 +775,7 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
     a.hit = reinterpret_cast<float*>(c.ws + p.o_hit);
     mm<E_LSE, F32>(a, 1, c.st);
     hipLaunchKernelGGL(k_xent_join, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, c.st, p.N,
-                       div_up(vc, tile_of(vc, p.N).bm), a.part,
+                       div_up(vc, tile_of(vc, p.N, p.np).bm), a.part,
                        c.rows.kind == GNCDE_TARGET_ROWS ? a.part_y : nullptr, a.hit, c.rows, p.V,
                        reinterpret_cast<float4*>(c.ws + p.o_run), v0 == 0, v0 + p.piece >= p.V, loss, stats);
   }
@@ -722,22 +807,22 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
     const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
     GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
     a.stats = stats, a.g = g;
-    a.P = P, a.ldp = vp, a.sp = p.N * vp;
-    a.Pt = Pt, a.ldpt = p.Np, a.spt = vc * p.Np;
+    a.P = P, a.ldp = vp;
+    a.Pt = Pt, a.ldpt = p.Np;
     a.part_b = gb ? part_b : nullptr;
     mm<E_DL, F32>(a, 1, c.st);
     if (gb) {
-      const Tile t = tile_of(vc, p.N);
+      const Tile t = tile_of(vc, p.N, p.np);
       sum_out<F32>(1, vc, div_up(p.N, t.bn) * t.wn, part_b, vc, vc, static_cast<char*>(gb) + v0 * SZ, vc, c.st);
     }
     if (gx) {
       pack_t<F32, false>(wsrc, vc, vp, p, c.rows, wt, c.st);
       GemmArgs q = {};
-      q.A = wt, q.lda = vp, q.sa = p.H * vp, q.M = p.H;
-      q.B = P, q.ldb = vp, q.sb = p.N * vp, q.N = p.N;
+      q.A = wt, q.lda = p.np * vp, q.M = p.H;
+      q.B = P, q.ldb = p.np * vp, q.N = p.N;
       q.K = (int)vp;
       q.out = gx, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(gx, 4 * SZ);
-      const int64_t sp = split_of(p.H, p.N, vp / kBK, p.np);
+      const int64_t sp = split_of(p.H, p.N, steps_of(vp, p.np), p.np);
       // every piece's splits fill the same sums; the last piece may have fewer steps, and leaves the others as they are
       const bool sums = !one || sp > 1;
       if (sums) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
@@ -748,12 +833,12 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
     }
     if (gW) {
       GemmArgs q = {};
-      q.A = xt, q.lda = p.Np, q.sa = p.H * p.Np, q.M = p.H;
-      q.B = Pt, q.ldb = p.Np, q.sb = vc * p.Np, q.N = vc;
+      q.A = xt, q.lda = p.np * p.Np, q.M = p.H;
+      q.B = Pt, q.ldb = p.np * p.Np, q.N = vc;
       q.K = (int)p.Np;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(out, 4 * SZ);
-      const int64_t sp = std::min(split_of(p.H, vc, p.Np / kBK, p.np), p.gw_split);
+      const int64_t sp = std::min(split_of(p.H, vc, steps_of(p.Np, p.np), p.np), p.gw_split);
       if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
       mm<E_OUT, F32>(q, sp, c.st);
       if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, out, p.H, c.st);
