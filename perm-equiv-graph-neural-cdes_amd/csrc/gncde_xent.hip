@@ -534,6 +534,14 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   }
 }
 
+// A pair (largest, sum of exponentials relative to it) joined with another.
+__device__ __forceinline__ void join_pair(float& top, float& sum, float top2, float sum2) {
+  const float nt = fmaxf(top, top2), ref = nt == -INFINITY ? 0.f : nt;
+  sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
+        sum2 * (top2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top2 - ref) * kLog2e));
+  top = nt;
+}
+
 // ---- joins ------------------------------------------------------------------------------------------------------
 // One wave a row: the tiles' (largest, sum) pairs into the row's running pair; at the last piece, lse and the loss.
 __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, const float2* __restrict__ part,
@@ -550,10 +558,7 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
   }
   for (int64_t i = lane; i < tiles; i += 64) {
     const float2 p = part[n * tiles + i];
-    const float nt = fmaxf(top, p.x), ref = nt == -INFINITY ? 0.f : nt;
-    sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
-          p.y * (p.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p.x - ref) * kLog2e));
-    top = nt;
+    join_pair(top, sum, p.x, p.y);
     if (part_y) {
       const float2 q = part_y[n * tiles + i];
       dot += q.x;
@@ -562,11 +567,7 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d);
-    const float nt = fmaxf(top, ot), ref = nt == -INFINITY ? 0.f : nt;
-    sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
-          os * (ot == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ot - ref) * kLog2e));
-    top = nt;
+    join_pair(top, sum, __shfl_xor(top, d), __shfl_xor(sum, d));
     dot += __shfl_xor(dot, d);
     mass += __shfl_xor(mass, d);
   }
@@ -601,6 +602,570 @@ __global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __rest
   }
 }
 
+// ---- few classes and a narrow hidden row: everything in LDS -----------------------------------------------------
+// W (as fp32), 16 rows of x and their dl stay in LDS and all four products run on v_mfma_f32_16x16x4f32 (either type:
+// the products of bf16 values are exact there), so nothing but the results goes to memory: the loss is one launch, the
+// gradient two (the second adds the workgroups' gW and gb).  TGB's read-out (classes = nodes, hidden 32) is this size,
+// where the tiled kernels above are eleven launches of a few microseconds.
+//
+// Sixteen waves a workgroup; a row tile's classes go round the waves by 16, two rounds at most.
+constexpr int kSmallLds = 20480;     // floats: W [Vp][Hs], x [16][Hs], dl [16][Vs], joins
+constexpr int kSmallJoin = 5120;     // [16][16][4] of the loss, [16 / (Hp / 16)][16][Hs] of gx
+constexpr int kSmallTiles = 4;       // 16 x 16 tiles of gW a wave holds
+constexpr int kSmallThreads = 1024, kSmallWaves = 16;
+
+struct SmallSize {
+  int Vp, Hp, Hs, Vs;  // padded to 16; row strides of W / x and of dl, 4 floats off a multiple of 16 (banks)
+};
+
+__host__ __device__ __forceinline__ SmallSize small_size(int H, int V) {
+  SmallSize z;
+  z.Vp = (V + 15) / 16 * 16, z.Hp = (H + 15) / 16 * 16;
+  z.Hs = z.Hp + 4, z.Vs = z.Vp + 4;
+  return z;
+}
+
+bool small_fits(int64_t H, int64_t V) {
+  if (H > 128 || V > 2 * 16 * kSmallWaves) return false;
+  const SmallSize z = small_size((int)H, (int)V);
+  return z.Vp * z.Hs + 16 * z.Hs + 16 * z.Vs + kSmallJoin <= kSmallLds &&
+         (z.Vp / 16) * (z.Hp / 16) <= kSmallWaves * kSmallTiles;
+}
+
+struct SmallArgs {
+  const void *x, *W, *b;
+  Rows rows;
+  int64_t N;
+  int H, V;
+  float *loss, *stats;         // the loss writes both
+  const float *row_stats, *g;  // the gradient reads both
+  void* gx;                    // may be NULL
+  float* part;                 // [workgroups][V H + V]; NULL without gW and gb
+};
+
+// Values at p[i..i+3], zeros from `to` on.
+template <bool F32>
+__device__ __forceinline__ floatx4 four(const void* p, int64_t i, int64_t to) {
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+  if (i + 4 <= to) {
+    if (F32) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+      return floatx4{v[0], v[1], v[2], v[3]};
+    }
+    const u16x4u v = *reinterpret_cast<const u16x4u*>(static_cast<const uint16_t*>(p) + i);
+    return floatx4{from_bf16(v[0]), from_bf16(v[1]), from_bf16(v[2]), from_bf16(v[3])};
+  }
+  floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (i + q < to) v[q] = value<F32>(p, i + q);
+  return v;
+}
+
+template <bool F32, bool GRAD>
+__global__ void __launch_bounds__(kSmallThreads) k_xent_small(SmallArgs a) {
+  __shared__ __attribute__((aligned(16))) float sm[kSmallLds];
+  const SmallSize z = small_size(a.H, a.V);
+  float* w = sm;
+  float* x = w + z.Vp * z.Hs;
+  float* d = x + 16 * z.Hs;
+  float* join = d + 16 * z.Vs;
+  const int lane = threadIdx.x & 63, fr = lane & 15, fk = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int vt = z.Vp / 16, ht = z.Hp / 16, hq = z.Hp / 4;
+  const int lr = threadIdx.x / hq, lh = (threadIdx.x - lr * hq) * 4;  // this thread's row and values of W and x
+  for (int v = lr; v < z.Vp; v += kSmallThreads / hq) {
+    if (lr >= kSmallThreads / hq) break;
+    *reinterpret_cast<floatx4*>(w + v * z.Hs + lh) =
+        v < a.V && lh < a.H ? four<F32>(a.W, (int64_t)v * a.H + lh, (int64_t)v * a.H + a.H) : floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  floatx4 bias[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int v = (wave + kSmallWaves * i) * 16 + fk * 4;
+    bias[i] = a.b && v < a.V ? four<F32>(a.b, v, a.V) : floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
+  floatx4 gw[kSmallTiles];
+  float gb = 0.f;  // of class threadIdx.x
+#pragma unroll
+  for (int i = 0; i < kSmallTiles; ++i) gw[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int64_t tiles = (a.N + 15) / 16;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t r0 = t * 16, n = r0 + fr;  // n: this lane's row
+    const bool in = n < a.N && row_counts(a.rows, n);
+    const int64_t hit = in && !soft ? row_index(a.rows, n) : -1;
+    floatx4 y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int v = (wave + kSmallWaves * i) * 16 + fk * 4;
+      y[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (soft && in && v < a.V) y[i] = four<true>(a.rows.target, n * a.V + v, n * a.V + a.V);
+    }
+    float lse = 0.f, gv = 0.f, gs = 0.f;
+    if (GRAD && in) {
+      lse = a.row_stats[2 * n];
+      gv = a.g[n];
+      gs = gv * a.row_stats[2 * n + 1];
+    }
+    floatx4 xv = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (lr < 16 && r0 + lr < a.N && lh < a.H && (!GRAD || row_counts(a.rows, r0 + lr)))
+      xv = four<F32>(a.x, (r0 + lr) * a.H + lh, (r0 + lr) * a.H + a.H);
+    __syncthreads();  // the last tile's x, dl and joins have been read
+    if (lr < 16) *reinterpret_cast<floatx4*>(x + lr * z.Hs + lh) = xv;
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f, dot = 0.f, mass = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tile = wave + kSmallWaves * i;
+      if (tile >= vt) break;
+      floatx4 l = floatx4{0.f, 0.f, 0.f, 0.f}, l1 = l;
+      const float* wa = w + (tile * 16 + fr) * z.Hs + fk;
+      const float* xb = x + fr * z.Hs + fk;
+      for (int h = 0; h < z.Hp; h += 16) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          l = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[h + 8 * k], xb[h + 8 * k], l, 0, 0, 0);
+          l1 = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[h + 8 * k + 4], xb[h + 8 * k + 4], l1, 0, 0, 0);
+        }
+      }
+      const int v = tile * 16 + fk * 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) l[q] = v + q < a.V ? l[q] + l1[q] + bias[i][q] : -INFINITY;
+      if (GRAD) {
+        floatx4 dv;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          dv[q] = gs * __builtin_amdgcn_exp2f((l[q] - lse) * kLog2e);
+          if (soft) dv[q] -= gv * y[i][q];
+          else dv[q] -= hit == v + q ? gv : 0.f;
+          dv[q] = in && v + q < a.V ? dv[q] : 0.f;
+        }
+        *reinterpret_cast<floatx4*>(d + fr * z.Vs + v) = dv;
+      } else {
+        const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = tt == -INFINITY ? 0.f : tt;
+        float ts = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          ts += __builtin_amdgcn_exp2f((l[q] - ref) * kLog2e);
+          if (soft) {
+            mass += y[i][q];
+            dot += y[i][q] == 0.f ? 0.f : y[i][q] * l[q];  // a class at -inf without mass adds nothing
+          } else if (hit == v + q) {
+            dot = l[q];
+          }
+        }
+        join_pair(top, sum, tt, ts);
+      }
+    }
+    if (!GRAD) {
+#pragma unroll
+      for (int s = 16; s < 64; s <<= 1) {
+        join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
+        dot += __shfl_xor(dot, s);
+        mass += __shfl_xor(mass, s);
+      }
+      if (fk == 0) *reinterpret_cast<floatx4*>(join + (wave * 16 + fr) * 4) = floatx4{top, sum, dot, mass};
+      __syncthreads();
+      if (wave == 0) {  // four of the waves' joins a lane, then the four lanes of a row
+        top = -INFINITY, sum = dot = mass = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSmallWaves / 4; ++i) {
+          const floatx4 q = *reinterpret_cast<const floatx4*>(join + ((fk * 4 + i) * 16 + fr) * 4);
+          join_pair(top, sum, q[0], q[1]);
+          dot += q[2];
+          mass += q[3];
+        }
+#pragma unroll
+        for (int s = 16; s < 64; s <<= 1) {
+          join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
+          dot += __shfl_xor(dot, s);
+          mass += __shfl_xor(mass, s);
+        }
+        if (fk == 0 && n < a.N) {
+          lse = top + logf(sum);
+          if (!soft) {
+            mass = 1.f;
+            if (in && hit >= a.V) lse = dot = NAN;
+          }
+          a.loss[n] = in ? mass * lse - dot : 0.f;
+          a.stats[2 * n] = in ? lse : 0.f;
+          a.stats[2 * n + 1] = in ? mass : 0.f;
+        }
+      }
+    } else {
+      __syncthreads();
+      const int parts = kSmallWaves / ht;  // waves that share a hidden tile of gx, each with its share of the classes
+      if (a.gx && wave < parts * ht) {     // gx^T [hidden][16 rows]
+        const int i = wave % ht, part = wave / ht;
+        floatx4 o0 = floatx4{0.f, 0.f, 0.f, 0.f}, o1 = o0;
+        const float* wa = w + fk * z.Hs + i * 16 + fr;
+        const float* db = d + fr * z.Vs + fk;
+        for (int v = part * 16; v < z.Vp; v += parts * 16) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            o0 = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[(v + 8 * k) * z.Hs], db[v + 8 * k], o0, 0, 0, 0);
+            o1 = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[(v + 8 * k + 4) * z.Hs], db[v + 8 * k + 4], o1, 0, 0, 0);
+          }
+        }
+        *reinterpret_cast<floatx4*>(join + (part * 16 + fr) * z.Hs + i * 16 + fk * 4) = o0 + o1;
+      }
+      if (a.part) {
+#pragma unroll
+        for (int i = 0; i < kSmallTiles; ++i) {  // gW [classes][hidden]: tiles round the waves
+          const int tile = wave + kSmallWaves * i;
+          if (tile >= vt * ht) break;
+          const int v = tile / ht * 16, h = tile % ht * 16;
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            gw[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[(k + fk) * z.Vs + v + fr], x[(k + fk) * z.Hs + h + fr],
+                                                         gw[i], 0, 0, 0);
+        }
+        if (threadIdx.x < a.V) {
+          float s = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s += d[r * z.Vs + threadIdx.x];
+          gb += s;
+        }
+      }
+      __syncthreads();
+      if (a.gx && lr < 16 && r0 + lr < a.N) {
+        floatx4 o = *reinterpret_cast<const floatx4*>(join + lr * z.Hs + lh);
+        for (int q = 1; q < parts; ++q) o += *reinterpret_cast<const floatx4*>(join + (q * 16 + lr) * z.Hs + lh);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (lh + q < a.H) {
+            if (F32) static_cast<float*>(a.gx)[(r0 + lr) * a.H + lh + q] = o[q];
+            else static_cast<uint16_t*>(a.gx)[(r0 + lr) * a.H + lh + q] = to_bf16(o[q]);
+          }
+      }
+    }
+  }
+  if (GRAD && a.part) {
+    float* out = a.part + (int64_t)blockIdx.x * ((int64_t)a.V * a.H + a.V);
+#pragma unroll
+    for (int i = 0; i < kSmallTiles; ++i) {
+      const int tile = wave + kSmallWaves * i;
+      if (tile >= vt * ht) break;
+      const int v = tile / ht * 16 + fk * 4, h = tile % ht * 16 + fr;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (v + q < a.V && h < a.H) out[(v + q) * a.H + h] = gw[i][q];
+    }
+    if (threadIdx.x < a.V) out[a.V * a.H + threadIdx.x] = gb;
+  }
+}
+
+// VH values of gW and V of gb (or gx's, with V 0) from the workgroups' parts: 64 values a workgroup, sixteen runs of
+// parts side by side, added in order.
+template <bool F32>
+__global__ void __launch_bounds__(1024) k_xent_parts_sum(int parts, int VH, int V, const float* __restrict__ part,
+                                                         void* __restrict__ gW, void* __restrict__ gb) {
+  __shared__ float run[16][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int e = blockIdx.x * 64 + c, len = VH + V;
+  const int per = (parts + 15) / 16, to = per * (q + 1) < parts ? per * (q + 1) : parts;
+  float s = 0.f;
+  if (e < len)
+    for (int i = per * q; i < to; ++i) s += part[(int64_t)i * len + e];
+  run[q][c] = s;
+  __syncthreads();
+  if (q != 0 || e >= len) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += run[i][c];
+  void* out = e < VH ? gW : gb;
+  const int at = e < VH ? e : e - VH;
+  if (!out) return;
+  if (F32) static_cast<float*>(out)[at] = s;
+  else static_cast<uint16_t*>(out)[at] = to_bf16(s);
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
+// Up to 16 rows: one matrix tile's columns, and the weight's bytes are all there is.  Every wave streams its own W rows
+// from memory into matrix operands (16 classes, 16 bytes a lane; LDS holds x alone), eight loads ahead of the products;
+// where the classes are too few for all waves, ks of them share a tile's contraction.  The gradient reads W once for dl
+// and once more, row by row, for gx, writing gW in the same loop: a VALU product, which for so few rows hides behind
+// the bytes, and needs no transposed copy of W.
+constexpr int kFewRows = 16;
+constexpr int kFewWaves = 16;
+constexpr int kFewLds = 147456;   // bytes of x
+constexpr int kFewAhead = 8;      // loads in flight a lane
+
+template <bool F32>
+struct Few {
+  static constexpr int K = F32 ? 16 : 32;  // contraction a load of all lanes
+  static constexpr int C = F32 ? 4 : 8;    // values a lane
+  static constexpr int SZ = F32 ? 4 : 2;
+};
+
+struct FewArgs {
+  const void *x, *W, *b;
+  Rows rows;
+  int N, H, ks, xs;            // ks: waves that share a tile; xs: values a row of x in LDS
+  int64_t V, tiles;
+  float2 *part, *part_y;       // the loss: [N][workgroups]
+  float* hit;
+  const float *stats, *g;      // the gradient
+  float* d;                    // [N][V]
+  void* gb;
+};
+
+template <bool F32, bool GRAD>
+__global__ void __launch_bounds__(kFewWaves * 64) k_xent_few(FewArgs a) {
+  typedef Few<F32> S;
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef __bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
+  extern __shared__ __attribute__((aligned(16))) char few_lds[];
+  char* xl = few_lds;
+  __shared__ __attribute__((aligned(16))) float join[kFewWaves * 64 * 4];
+  const int lane = threadIdx.x & 63, fr = lane & 15, fk = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int xs = a.xs;
+  for (int e = threadIdx.x; e < a.N * xs; e += kFewWaves * 64) {
+    const int n = e / xs, h = e - n * xs;
+    const bool in = h < a.H;
+    if (F32) reinterpret_cast<float*>(xl)[e] = in ? static_cast<const float*>(a.x)[n * a.H + h] : 0.f;
+    else reinterpret_cast<uint16_t*>(xl)[e] = in ? static_cast<const uint16_t*>(a.x)[n * a.H + h] : (uint16_t)0;
+  }
+  __syncthreads();
+  const int64_t n = fr;
+  const bool in = n < a.N && row_counts(a.rows, n);
+  const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
+  const int64_t hit = in && !soft ? row_index(a.rows, n) : -1;
+  const float* y = in && soft ? static_cast<const float*>(a.rows.target) + n * a.V : nullptr;
+  float lse = 0.f, gv = 0.f, gs = 0.f;
+  if (GRAD && in) {
+    lse = a.stats[2 * n];
+    gv = a.g[n];
+    gs = gv * a.stats[2 * n + 1];
+  }
+  float top = -INFINITY, sum = 0.f, dot = 0.f, mass = 0.f;
+  const int group = wave / a.ks, share = wave % a.ks, groups = kFewWaves / a.ks;
+  const int ksteps = (a.H + S::K - 1) / S::K, per = (ksteps + a.ks - 1) / a.ks;
+  const int s_from = share * per, s_to = s_from + per < ksteps ? s_from + per : ksteps;
+  const char* xrow = xl + (fr < a.N ? fr : a.N - 1) * xs * S::SZ + fk * 16;
+  for (int64_t t0 = (int64_t)blockIdx.x * groups; t0 < a.tiles; t0 += (int64_t)gridDim.x * groups) {
+    const int64_t tile = t0 + group, v0 = tile * 16;
+    floatx4 acc0 = floatx4{0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
+    if (tile < a.tiles) {
+      const int64_t row = v0 + fr < a.V ? v0 + fr : a.V - 1;
+      const char* wrow = static_cast<const char*>(a.W) + (row * a.H + fk * S::C) * S::SZ;
+      auto get = [&](int s, u16x8& o) {  // 16 bytes of this lane's W row, zeros behind its end
+        const int h = s * S::K + fk * S::C;
+        const char* p = wrow + (int64_t)s * S::K * S::SZ;
+        if (h + S::C <= a.H) {
+          if (F32) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+            o = __builtin_bit_cast(u16x8, floatx4{v[0], v[1], v[2], v[3]});
+          } else {
+            const bf16x8u v = *reinterpret_cast<const bf16x8u*>(p);
+            o = __builtin_bit_cast(u16x8, v);
+          }
+        } else {
+          o = u16x8{};
+          if (F32) {
+            floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (h + q < a.H) v[q] = reinterpret_cast<const float*>(p)[q];
+            o = __builtin_bit_cast(u16x8, v);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (h + q < a.H) o[q] = reinterpret_cast<const uint16_t*>(p)[q];
+          }
+        }
+      };
+      auto use = [&](int s, const u16x8& o, floatx4& acc) {
+        const u16x8 xv = *reinterpret_cast<const u16x8*>(xrow + s * S::K * S::SZ);
+        if (F32) {
+          const floatx4 wf = __builtin_bit_cast(floatx4, o), xf = __builtin_bit_cast(floatx4, xv);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], acc, 0, 0, 0);
+        } else {
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o), __builtin_bit_cast(bf16x8, xv),
+                                                        acc, 0, 0, 0);
+        }
+      };
+      u16x8 now[kFewAhead], next[kFewAhead];
+      int s = s_from;
+      const int whole = s_from + (s_to - s_from) / kFewAhead * kFewAhead;
+      if (s < whole) {
+#pragma unroll
+        for (int u = 0; u < kFewAhead; ++u) get(s + u, now[u]);
+      }
+      for (; s < whole; s += kFewAhead) {
+        if (s + kFewAhead < whole) {
+#pragma unroll
+          for (int u = 0; u < kFewAhead; ++u) get(s + kFewAhead + u, next[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kFewAhead; ++u) use(s + u, now[u], u & 1 ? acc1 : acc0);
+#pragma unroll
+        for (int u = 0; u < kFewAhead; ++u) now[u] = next[u];
+      }
+      for (; s < s_to; ++s) {
+        u16x8 o;
+        get(s, o);
+        use(s, o, acc0);
+      }
+    }
+    floatx4 l = acc0 + acc1;
+    if (a.ks > 1) {  // the shares of a tile, added in order by its first wave
+      __syncthreads();
+      *reinterpret_cast<floatx4*>(join + (wave * 64 + lane) * 4) = l;
+      __syncthreads();
+      if (share != 0) continue;
+      for (int q = 1; q < a.ks; ++q) l += *reinterpret_cast<const floatx4*>(join + ((wave + q) * 64 + lane) * 4);
+    }
+    if (tile >= a.tiles) continue;
+    const int64_t v = v0 + fk * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      l[q] = v + q < a.V ? l[q] + (a.b ? value<F32>(a.b, v + q) : 0.f) : -INFINITY;
+    if (GRAD) {
+      float dv[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        dv[q] = gs * __builtin_amdgcn_exp2f((l[q] - lse) * kLog2e);
+        if (soft) dv[q] -= in && v + q < a.V ? gv * y[v + q] : 0.f;
+        else dv[q] -= hit == v + q ? gv : 0.f;
+        dv[q] = in && v + q < a.V ? dv[q] : 0.f;
+        if (n < a.N && v + q < a.V) a.d[n * a.V + v + q] = dv[q];
+      }
+      if (a.gb) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float r = dv[q];
+#pragma unroll
+          for (int i = 1; i < 16; i <<= 1) r += __shfl_xor(r, i);
+          if (fr == 0 && v + q < a.V) {
+            if (F32) static_cast<float*>(a.gb)[v + q] = r;
+            else static_cast<uint16_t*>(a.gb)[v + q] = to_bf16(r);
+          }
+        }
+      }
+    } else {
+      const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = tt == -INFINITY ? 0.f : tt;
+      float ts = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        ts += __builtin_amdgcn_exp2f((l[q] - ref) * kLog2e);
+        if (soft) {
+          const float yv = in && v + q < a.V ? y[v + q] : 0.f;
+          mass += yv;
+          dot += yv == 0.f ? 0.f : yv * l[q];  // a class at -inf without mass adds nothing
+        } else if (hit == v + q) {
+          a.hit[n] = l[q];
+        }
+      }
+      join_pair(top, sum, tt, ts);
+    }
+  }
+  if (GRAD) return;
+#pragma unroll
+  for (int s = 16; s < 64; s <<= 1) {
+    join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
+    dot += __shfl_xor(dot, s);
+    mass += __shfl_xor(mass, s);
+  }
+  __syncthreads();
+  if (fk == 0) *reinterpret_cast<floatx4*>(join + (wave * 16 + fr) * 4) = floatx4{top, sum, dot, mass};
+  __syncthreads();
+  if (threadIdx.x < a.N) {
+    top = -INFINITY, sum = dot = mass = 0.f;
+    for (int w = 0; w < kFewWaves; ++w) {
+      const floatx4 q = *reinterpret_cast<const floatx4*>(join + (w * 16 + threadIdx.x) * 4);
+      join_pair(top, sum, q[0], q[1]);
+      dot += q[2];
+      mass += q[3];
+    }
+    a.part[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(top, sum);
+    if (soft) a.part_y[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(dot, mass);
+  }
+}
+
+// gx and gW from dl, W streamed once: a workgroup takes a run of classes (blockIdx.x) and 256 C columns (blockIdx.y).
+template <bool F32, int NR, int C>
+__global__ void __launch_bounds__(256) k_xent_few_out(int N, int H, int64_t V, int64_t per, const float* __restrict__ d,
+                                                      const void* __restrict__ x, const void* __restrict__ W,
+                                                      Rows rows, float* __restrict__ part, void* __restrict__ gW) {
+  const int h = (blockIdx.y * 256 + threadIdx.x) * C;
+  if (h >= H) return;
+  const int64_t v_from = blockIdx.x * per, v_to = v_from + per < V ? v_from + per : V;
+  float xv[NR][C], gx[NR][C];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const bool in = n < N && row_counts(rows, n);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      xv[n][c] = in && h + c < H ? value<F32>(x, (int64_t)n * H + h + c) : 0.f;
+      gx[n][c] = 0.f;
+    }
+  }
+  auto get = [&](int64_t v, float (&w)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; c += 4) {
+      const floatx4 q = four<F32>(W, v * H + h + c, v * H + H);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[c + i] = q[i];
+    }
+  };
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+  auto out = [&](int64_t v, const float (&w)[C]) {
+    float o[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const float dv = n < N ? d[n * V + v] : 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        gx[n][c] = fmaf(dv, w[c], gx[n][c]);
+        o[c] = fmaf(dv, xv[n][c], o[c]);
+      }
+    }
+    if (!gW) return;
+#pragma unroll
+    for (int c = 0; c < C; c += 4) {
+      if (h + c + 4 <= H) {
+        if (F32) *reinterpret_cast<f32x4*>(static_cast<float*>(gW) + v * H + h + c) = f32x4{o[c], o[c + 1], o[c + 2], o[c + 3]};
+        else *reinterpret_cast<u16x4u*>(static_cast<uint16_t*>(gW) + v * H + h + c) =
+            u16x4u{to_bf16(o[c]), to_bf16(o[c + 1]), to_bf16(o[c + 2]), to_bf16(o[c + 3])};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (h + c + i < H) {
+            if (F32) static_cast<float*>(gW)[v * H + h + c + i] = o[c + i];
+            else static_cast<uint16_t*>(gW)[v * H + h + c + i] = to_bf16(o[c + i]);
+          }
+      }
+    }
+  };
+  int64_t v = v_from;
+  for (; v + 4 <= v_to; v += 4) {
+    float w[4][C];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) get(v + u, w[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) out(v + u, w[u]);
+  }
+  for (; v < v_to; ++v) {
+    float w[C];
+    get(v, w);
+    out(v, w);
+  }
+  if (!part) return;
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (n < N && h + c < H) part[((int64_t)blockIdx.x * N + n) * H + h + c] = gx[n][c];
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
@@ -611,6 +1176,10 @@ constexpr int64_t kPieceBytes = int64_t(512) << 20;
 
 struct Plan {
   int64_t N, H, V;
+  bool small = false;   // k_xent_small
+  bool few = false;     // k_xent_few
+  int64_t few_groups = 0, few_out = 0;  // workgroups of the loss / dl, runs of classes of gx and gW
+  int ks = 1, xs = 0;
   bool f32, direct_ok;  // direct_ok: sizes allow x and W as operands as they lie (the pointers decide too)
   int np;
   int64_t Kp, Np;
@@ -653,6 +1222,12 @@ int64_t split_of(int64_t M, int64_t N, int64_t kt, int np) {
   return div_up(kt, div_up(kt, s));  // no split without a step
 }
 
+// Workgroups of the small gradient: one for each CU, each with its share of the row tiles and one part of gW.
+int64_t small_groups(int64_t N) { return std::min(div_up(std::max<int64_t>(N, 1), 16), kCus); }
+
+// Columns a thread of k_xent_few_out takes: what its rows of x and gx leave registers for.
+int64_t few_cols(int64_t N) { return N > 4 ? 4 : 8; }
+
 bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& p) {
   // launches stay below 2^32 threads, and 256 rows of every operand below 2^32 bytes
   if (N < 0 || H <= 0 || V <= 0 || N > (int64_t(1) << 21) || H > (int64_t(1) << 16) || V > (int64_t(1) << 26) ||
@@ -665,6 +1240,33 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   p.np = p.f32 ? 3 : 1;
   p.direct_ok = !p.f32 && H % 8 == 0;
   p.Kp = up(H, 64), p.Np = up(std::max<int64_t>(N, 1), 64);
+  p.small = small_fits(H, V);
+  if (p.small) {
+    p.o_b = p.take(grad ? 4 * small_groups(N) * (V * H + V) : 0);
+    return true;
+  }
+  if (N > 0 && N <= kFewRows) {
+    const int64_t sz = p.f32 ? 4 : 2, step = p.f32 ? 16 : 32;
+    const int64_t xs = up(H, step) + 16 / sz;  // rows of x start in different banks
+    if (N * xs * sz <= kFewLds) {
+      p.few = true;
+      p.xs = (int)xs;
+      const int64_t tiles = div_up(V, 16);
+      while (p.ks < kFewWaves && tiles * p.ks < kCus * kFewWaves && div_up(H, step) >= 2 * kFewAhead * p.ks) p.ks *= 2;
+      p.few_groups = std::min(div_up(tiles * p.ks, kFewWaves), kCus);
+      const int64_t cols = div_up(H, 256 * few_cols(N));
+      p.few_out = std::min(div_up(V, 4), std::max<int64_t>(1, 4 * kCus / cols));
+      if (!grad) {
+        p.o_part = p.take(8 * N * p.few_groups);
+        p.o_party = p.take(8 * N * p.few_groups);
+        p.o_hit = p.take(4 * N);
+      } else {
+        p.o_p = p.take(4 * N * V);
+        p.o_gx = p.take(4 * p.few_out * N * H);
+      }
+      return true;
+    }
+  }
   const int64_t plane = 2 * p.np;
   // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
   const int64_t per_class = grad ? plane * (2 * p.Np + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
@@ -762,8 +1364,42 @@ GemmArgs logits_args(const Operand<F32>& w, const Operand<F32>& x, const Plan& p
   return a;
 }
 
+SmallArgs small_args(const Plan& p, const Call& c) {
+  SmallArgs a = {};
+  a.x = c.x, a.W = c.W, a.b = c.b, a.rows = c.rows;
+  a.N = p.N, a.H = (int)p.H, a.V = (int)p.V;
+  return a;
+}
+
+FewArgs few_args(const Plan& p, const Call& c) {
+  FewArgs a = {};
+  a.x = c.x, a.W = c.W, a.b = c.b, a.rows = c.rows;
+  a.N = (int)p.N, a.H = (int)p.H, a.ks = p.ks, a.xs = p.xs;
+  a.V = p.V, a.tiles = div_up(p.V, 16);
+  return a;
+}
+
 template <bool F32>
 void forward(const Plan& p, const Call& c, float* loss, float* stats) {
+  if (p.few) {
+    FewArgs a = few_args(p, c);
+    a.part = reinterpret_cast<float2*>(c.ws + p.o_part);
+    a.part_y = reinterpret_cast<float2*>(c.ws + p.o_party);
+    a.hit = reinterpret_cast<float*>(c.ws + p.o_hit);
+    hipLaunchKernelGGL((k_xent_few<F32, false>), dim3((unsigned)p.few_groups), dim3(kFewWaves * 64),
+                       (unsigned)(p.N * p.xs * (F32 ? 4 : 2)), c.st, a);
+    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, c.st, p.N, p.few_groups, a.part,
+                       c.rows.kind == GNCDE_TARGET_ROWS ? a.part_y : nullptr, a.hit, c.rows, p.V, nullptr, 1, 1, loss,
+                       stats);
+    return;
+  }
+  if (p.small) {
+    SmallArgs a = small_args(p, c);
+    a.loss = loss, a.stats = stats;
+    hipLaunchKernelGGL((k_xent_small<F32, false>), dim3((unsigned)std::min(div_up(p.N, 16), 8 * kCus)),
+                       dim3(kSmallThreads), 0, c.st, a);
+    return;
+  }
   const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, p.V - v0);
@@ -791,6 +1427,42 @@ void sum_out(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t lda
 template <bool F32>
 void backward(const Plan& p, const Call& c, const float* stats, const float* g, void* gx, void* gW, void* gb) {
   constexpr int64_t SZ = F32 ? 4 : 2;
+  if (p.small) {
+    SmallArgs a = small_args(p, c);
+    a.row_stats = stats, a.g = g, a.gx = gx;
+    a.part = gW || gb ? reinterpret_cast<float*>(c.ws + p.o_b) : nullptr;
+    const int groups = (int)small_groups(p.N);
+    hipLaunchKernelGGL((k_xent_small<F32, true>), dim3(groups), dim3(kSmallThreads), 0, c.st, a);
+    const int VH = a.V * a.H;
+    if (a.part)
+      hipLaunchKernelGGL((k_xent_parts_sum<F32>), dim3((unsigned)div_up(VH + a.V, 64)), dim3(1024), 0, c.st, groups, VH,
+                         a.V, a.part, gW, gb);
+    return;
+  }
+  if (p.few) {
+    FewArgs a = few_args(p, c);
+    a.stats = stats, a.g = g, a.gb = gb;
+    a.d = reinterpret_cast<float*>(c.ws + p.o_p);
+    hipLaunchKernelGGL((k_xent_few<F32, true>), dim3((unsigned)p.few_groups), dim3(kFewWaves * 64),
+                       (unsigned)(p.N * p.xs * SZ), c.st, a);
+    if (!gx && !gW) return;
+    float* part = gx ? reinterpret_cast<float*>(c.ws + p.o_gx) : nullptr;
+    const int64_t per = div_up(p.V, p.few_out), runs = div_up(p.V, per);
+    const dim3 grid((unsigned)runs, (unsigned)div_up(p.H, 256 * few_cols(p.N)));
+    if (p.N == 1)
+      hipLaunchKernelGGL((k_xent_few_out<F32, 1, 8>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W, c.rows,
+                         part, gW);
+    else if (p.N <= 4)
+      hipLaunchKernelGGL((k_xent_few_out<F32, 4, 8>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W, c.rows,
+                         part, gW);
+    else
+      hipLaunchKernelGGL((k_xent_few_out<F32, 16, 4>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W,
+                         c.rows, part, gW);
+    if (gx)
+      hipLaunchKernelGGL((k_xent_parts_sum<F32>), dim3((unsigned)div_up(p.N * p.H, 64)), dim3(1024), 0, c.st, (int)runs,
+                         (int)(p.N * p.H), 0, part, gx, nullptr);
+    return;
+  }
   const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
   uint16_t* xt = reinterpret_cast<uint16_t*>(c.ws + p.o_xt);
   uint16_t* wt = reinterpret_cast<uint16_t*>(c.ws + p.o_wt);

@@ -33,6 +33,14 @@ def _on(dev: torch.device):
     return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream_of(dev: torch.device):
+    return torch._C._cuda_getCurrentRawStream(dev.index)  # torch.cuda.current_stream(dev).cuda_stream, in a tenth the time
+
+
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
@@ -418,9 +426,7 @@ def _readout_args(name: str, x, W, b, target, mask):
                               f"{target.dtype}")
     if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != lead):
         raise _lib.GncdeError(f"{name}: mask must be bool {lead}, got {mask.dtype} {tuple(mask.shape)}")
-    for t in (x, W, b, target, mask):
-        if t is not None and (t.device.type != "cuda" or t.device != x.device):
-            raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
+    _one_device(name, [t for t in (x, W, b, target, mask) if t is not None])
     return (rows, hidden, classes, kind, x.contiguous(), W.contiguous(), None if b is None else b.contiguous(), tkind,
             target.contiguous(), None if mask is None else mask.contiguous())
 
@@ -435,18 +441,19 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | Non
     [..., classes] fp32, of any mass.  mask [...] bool: False leaves the row out; its loss is 0 and its values change
     nothing.  ``stats`` holds each row's (log of the summed exponentials, label mass) for
     ``linear_cross_entropy_grad``."""
-    args = _readout_args("linear_cross_entropy", x, W, b, target, mask)
-    _require_gpu()
+    rows, hidden, classes, kind, x, W, b, tkind, target, mask = _readout_args("linear_cross_entropy", x, W, b, target,
+                                                                              mask)
     lib = _lib.load()
-    rows, hidden, classes, kind, x, W, b, tkind, target, mask = args
-    with _on(x.device):
-        loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=x.device)
+    dev, lead = x.device, x.shape[:-1]
+    with _on(dev):
+        loss = torch.empty(lead, dtype=torch.float32, device=dev)
+        stats = torch.empty((*lead, 2), dtype=torch.float32, device=dev)
         nbytes = lib.gncde_linear_cross_entropy_workspace_bytes(rows, hidden, classes, kind, 0)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.gncde_linear_cross_entropy(rows, hidden, classes, kind, _ptr(x), _ptr(W), _ptr(b), tkind,
-                                                  _ptr(target), _ptr(mask), _ptr(loss), _ptr(stats), _ptr(ws), nbytes,
-                                                  _stream()))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.gncde_linear_cross_entropy(rows, hidden, classes, kind, x.data_ptr(), W.data_ptr(), _addr(b), tkind,
+                                            target.data_ptr(), _addr(mask), loss.data_ptr(), stats.data_ptr(),
+                                            ws.data_ptr(), nbytes, _stream_of(dev))
+    _lib.check(rc)
     return loss, stats
 
 
@@ -462,69 +469,81 @@ def linear_cross_entropy_grad(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor 
         raise _lib.GncdeError(f"linear_cross_entropy_grad: stats must be the loss's fp32 {lead + (2,)}")
     if g.dtype != torch.float32 or tuple(g.shape) != lead or g.device != x.device:
         raise _lib.GncdeError(f"linear_cross_entropy_grad: g must be fp32 {lead}, got {g.dtype} {tuple(g.shape)}")
-    _require_gpu()
     lib = _lib.load()
-    with _on(x.device):
+    dev = x.device
+    with _on(dev):
         stats, g = stats.contiguous(), g.contiguous()
         gx = torch.empty_like(x) if need_x else None
         gW = torch.empty_like(W) if need_w else None
         gb = torch.empty_like(b) if need_b and b is not None else None
         nbytes = lib.gncde_linear_cross_entropy_workspace_bytes(rows, hidden, classes, kind, 1)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.gncde_linear_cross_entropy_grad(rows, hidden, classes, kind, _ptr(x), _ptr(W), _ptr(b), tkind,
-                                                       _ptr(target), _ptr(mask), _ptr(stats), _ptr(g), _ptr(gx),
-                                                       _ptr(gW), _ptr(gb), _ptr(ws), nbytes, _stream()))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.gncde_linear_cross_entropy_grad(rows, hidden, classes, kind, x.data_ptr(), W.data_ptr(), _addr(b),
+                                                 tkind, target.data_ptr(), _addr(mask), stats.data_ptr(), g.data_ptr(),
+                                                 _addr(gx), _addr(gW), _addr(gb), ws.data_ptr(), nbytes,
+                                                 _stream_of(dev))
+    _lib.check(rc)
     return gx, gW, gb
 
 
 _LIST_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
+_LIST_SIZES = np.array([4, 2, 2], dtype=np.int64)  # bytes a value, by GNCDE_DTYPE_*
+
+
 def _tensor_table(name: str, tensors, out=None):
-    """(host array of GncdeTensor, kept tensors, device) of a tensor list, checked."""
+    """(host array of GncdeTensor, kept tensors, device) of a tensor list, checked.  ``out`` may be the list itself."""
     if torch.is_tensor(tensors):
         raise _lib.GncdeError(f"{name}: a list of tensors is wanted, not one tensor")
-    tensors = list(tensors)
-    if not tensors:
+    if len(tensors) == 0:
         raise _lib.GncdeError(f"{name}: an empty list of tensors")
-    dev = tensors[0].device
     kinds = [_LIST_DTYPES.get(t.dtype) for t in tensors]
     if None in kinds:
         raise _lib.GncdeError(f"{name}: tensors must be fp32, bf16 or fp16, got {tensors[kinds.index(None)].dtype}")
-    if dev.type != "cuda" or any(t.device != dev for t in tensors):
-        raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
-    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    index = _one_device(name, tensors)
+    if not all([t.is_contiguous() for t in tensors]):
+        if out is tensors:
+            raise _lib.GncdeError(f"{name}: tensors clipped in place must be contiguous")
+        tensors = [t.contiguous() for t in tensors]
     rows = np.zeros((len(tensors), 4), dtype=np.int64)  # GncdeTensor: in, out, numel, dtype (+ reserved 0)
     rows[:, 0] = [t.data_ptr() for t in tensors]
     rows[:, 2] = [t.numel() for t in tensors]
     rows[:, 3] = kinds
     if out is not None:
-        if len(out) != len(tensors):
-            raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
-        for t, o in zip(tensors, out):
-            if o.dtype != t.dtype or o.shape != t.shape or o.device != dev or not o.is_contiguous():
+        if out is not tensors:
+            if len(out) != len(tensors):
+                raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
+            if ([o.dtype for o in out] != [t.dtype for t in tensors] or [o.shape for o in out] != [t.shape for t in tensors]
+                    or _one_device(name, out) != index or not all([o.is_contiguous() for o in out])):
                 raise _lib.GncdeError(f"{name}: an output must be contiguous, of its tensor's type, shape and device")
-        rows[:, 1] = [o.data_ptr() for o in out]
-        _refuse_overlap(name, rows, [t.element_size() for t in tensors])
-    return rows, tensors, dev
+        rows[:, 1] = rows[:, 0] if out is tensors else [o.data_ptr() for o in out]
+        _refuse_overlap(name, rows, _LIST_SIZES[rows[:, 3]])
+    return rows, tensors, torch.device("cuda", index)
+
+
+def _one_device(name: str, tensors) -> int:
+    index = {t.get_device() for t in tensors}
+    if len(index) != 1 or -1 in index:
+        raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
+    return index.pop()
 
 
 def _refuse_overlap(name: str, rows, sizes):
     """Outputs that meet each other, or a tensor that is not their own, would be written while they are read."""
-    bytes_ = rows[:, 2] * np.asarray(sizes, dtype=np.int64)
-    live = bytes_ > 0
-    out, end = rows[live, 1], rows[live, 1] + bytes_[live]
-    order = np.argsort(out, kind="stable")
-    lo, hi = out[order], end[order]
-    if np.any(lo[1:] < hi[:-1]):
+    nbytes = rows[:, 2] * np.asarray(sizes, dtype=np.int64)
+    if not nbytes.all():
+        live = nbytes > 0
+        rows, nbytes = rows[live], nbytes[live]
+    src, out = rows[:, 0], rows[:, 1]
+    order = out.argsort(kind="stable")
+    lo = out[order]
+    hi = lo + nbytes[order]
+    if (lo[1:] < hi[:-1]).any():
         raise _lib.GncdeError(f"{name}: two outputs share memory (the same tensor twice?)")
-    src, stop = rows[live, 0], rows[live, 0] + bytes_[live]
-    # outputs are disjoint, so those that meet [src, stop) are a run of the sorted order
-    first = np.searchsorted(hi, src, side="right")
-    last = np.searchsorted(lo, stop, side="left")
-    met = last - first
-    own = (src == out)
-    if np.any(met > own):
+    # outputs are disjoint, so those that meet [src, src + nbytes) are a run of the sorted order
+    met = lo.searchsorted(src + nbytes, side="left") - hi.searchsorted(src, side="right")
+    if (met > (src == out)).any():
         raise _lib.GncdeError(f"{name}: an output shares memory with a tensor that is not its own")
 
 
@@ -532,14 +551,15 @@ def global_norm(tensors) -> torch.Tensor:
     """Device stats [2] = (global L2 norm, largest magnitude) over a list of fp32 / bf16 / fp16 CUDA tensors of any
     sizes, on the tensors' device and torch's current stream there (squares and sums in 64 bits; NaN anywhere makes
     both NaN)."""
-    _require_gpu()
+    rows, kept, dev = _tensor_table("global_norm", tensors if torch.is_tensor(tensors) else list(tensors))
     lib = _lib.load()
-    rows, kept, dev = _tensor_table("global_norm", tensors)
     with _on(dev):
         stats = torch.empty(2, dtype=torch.float32, device=dev)
         nbytes = lib.gncde_global_norm_workspace_bytes(len(kept))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.check(lib.gncde_global_norm(len(kept), rows.ctypes.data, _ptr(stats), _ptr(ws), nbytes, _stream()))
+        rc = lib.gncde_global_norm(len(kept), rows.ctypes.data, stats.data_ptr(), ws.data_ptr(), nbytes,
+                                   _stream_of(dev))
+    _lib.check(rc)
     return stats
 
 
@@ -547,21 +567,23 @@ def clip_by_global_norm(tensors, max_norm: float, out=None):
     """``optax.clip_by_global_norm(max_norm)`` (optimiser_configs.py:76-84) over a list of tensors: (clipped list,
     device stats [2] of the list before clipping, as ``global_norm``).  ``out``: the list the clipped tensors are written
     to (``out=tensors`` clips in place); new tensors without it."""
-    _require_gpu()
-    lib = _lib.load()
     max_norm = float(max_norm)
     if not 0.0 < max_norm < float("inf"):
         raise _lib.GncdeError(f"clip_by_global_norm: max_norm {max_norm} must be positive and finite")
-    tensors = list(tensors) if not torch.is_tensor(tensors) else tensors
-    if out is None and not torch.is_tensor(tensors):
-        out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors]
+    if out is tensors:
+        out = tensors = tensors if torch.is_tensor(tensors) else list(tensors)
+    elif not torch.is_tensor(tensors):
+        tensors = list(tensors)
+        out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors] if out is None else list(out)
     rows, kept, dev = _tensor_table("clip_by_global_norm", tensors, out)
+    lib = _lib.load()
     with _on(dev):
         stats = torch.empty(2, dtype=torch.float32, device=dev)
         nbytes = lib.gncde_global_norm_workspace_bytes(len(kept))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.check(lib.gncde_clip_by_global_norm(len(kept), rows.ctypes.data, max_norm, _ptr(stats), _ptr(ws),
-                                                 nbytes, _stream()))
+        rc = lib.gncde_clip_by_global_norm(len(kept), rows.ctypes.data, max_norm, stats.data_ptr(), ws.data_ptr(),
+                                           nbytes, _stream_of(dev))
+    _lib.check(rc)
     return out, stats
 
 

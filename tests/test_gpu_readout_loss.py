@@ -124,7 +124,12 @@ def check(c):
 
 
 SIZES = [(1, 1, 1), (1, 16, 2), (3, 5, 7), (2, 64, 64), (17, 32, 255), (130, 64, 129), (255, 32, 255), (64, 200, 5000),
-         (257, 96, 513), (300, 333, 1001), (1030, 72, 4099)]
+         (257, 96, 513), (300, 333, 1001), (1030, 72, 4099),
+         # everything in LDS, at its widths and past one workgroup a CU
+         (40, 48, 100), (33, 128, 60), (100, 16, 440), (5000, 20, 70), (21, 80, 130), (50, 3, 500),
+         # few rows
+         (1, 512, 4096), (16, 100, 700), (13, 333, 1234), (5, 1000, 77), (2, 40, 9001), (4, 2050, 300),
+         (16, 4000, 90)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
