@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
+import operator
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -489,6 +490,9 @@ def linear_cross_entropy_grad(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor 
 _LIST_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
+# a list of hundreds of tensors is looked over faster than the GPU reads it only without a Python frame a tensor
+_DTYPE, _NUMEL, _DATA_PTR = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.data_ptr
+_DEVICE, _CONTIGUOUS = torch.Tensor.get_device, torch.Tensor.is_contiguous
 _LIST_SIZES = np.array([4, 2, 2], dtype=np.int64)  # bytes a value, by GNCDE_DTYPE_*
 
 
@@ -498,32 +502,36 @@ def _tensor_table(name: str, tensors, out=None):
         raise _lib.GncdeError(f"{name}: a list of tensors is wanted, not one tensor")
     if len(tensors) == 0:
         raise _lib.GncdeError(f"{name}: an empty list of tensors")
-    kinds = [_LIST_DTYPES.get(t.dtype) for t in tensors]
+    dtypes = list(map(_DTYPE, tensors))
+    kinds = list(map(_LIST_DTYPES.get, dtypes))
     if None in kinds:
         raise _lib.GncdeError(f"{name}: tensors must be fp32, bf16 or fp16, got {tensors[kinds.index(None)].dtype}")
     index = _one_device(name, tensors)
-    if not all([t.is_contiguous() for t in tensors]):
+    if not all(map(_CONTIGUOUS, tensors)):
         if out is tensors:
             raise _lib.GncdeError(f"{name}: tensors clipped in place must be contiguous")
         tensors = [t.contiguous() for t in tensors]
     rows = np.zeros((len(tensors), 4), dtype=np.int64)  # GncdeTensor: in, out, numel, dtype (+ reserved 0)
-    rows[:, 0] = [t.data_ptr() for t in tensors]
-    rows[:, 2] = [t.numel() for t in tensors]
+    numels = list(map(_NUMEL, tensors))
+    rows[:, 0] = list(map(_DATA_PTR, tensors))
+    rows[:, 2] = numels
     rows[:, 3] = kinds
+    if out is tensors:
+        rows[:, 1] = rows[:, 0]
+    elif out is not None:
+        if len(out) != len(tensors):
+            raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
+        if (list(map(_DTYPE, out)) != dtypes or list(map(_NUMEL, out)) != numels or _one_device(name, out) != index
+                or not all(map(_CONTIGUOUS, out))):
+            raise _lib.GncdeError(f"{name}: an output must be contiguous, of its tensor's type, size and device")
+        rows[:, 1] = list(map(_DATA_PTR, out))
     if out is not None:
-        if out is not tensors:
-            if len(out) != len(tensors):
-                raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
-            if ([o.dtype for o in out] != [t.dtype for t in tensors] or [o.shape for o in out] != [t.shape for t in tensors]
-                    or _one_device(name, out) != index or not all([o.is_contiguous() for o in out])):
-                raise _lib.GncdeError(f"{name}: an output must be contiguous, of its tensor's type, shape and device")
-        rows[:, 1] = rows[:, 0] if out is tensors else [o.data_ptr() for o in out]
         _refuse_overlap(name, rows, _LIST_SIZES[rows[:, 3]])
     return rows, tensors, torch.device("cuda", index)
 
 
 def _one_device(name: str, tensors) -> int:
-    index = {t.get_device() for t in tensors}
+    index = set(map(_DEVICE, tensors))
     if len(index) != 1 or -1 in index:
         raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
     return index.pop()
