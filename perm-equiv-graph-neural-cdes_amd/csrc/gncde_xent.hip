@@ -75,6 +75,26 @@ __device__ __forceinline__ float value(const void* p, int64_t i) {
   return F32 ? static_cast<const float*>(p)[i] : from_bf16(static_cast<const uint16_t*>(p)[i]);
 }
 
+// Values at p[i..i+3], zeros from `to` on.
+template <bool F32>
+__device__ __forceinline__ floatx4 four(const void* p, int64_t i, int64_t to) {
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+  if (i + 4 <= to) {
+    if (F32) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+      return floatx4{v[0], v[1], v[2], v[3]};
+    }
+    const u16x4u v = *reinterpret_cast<const u16x4u*>(static_cast<const uint16_t*>(p) + i);
+    return floatx4{from_bf16(v[0]), from_bf16(v[1]), from_bf16(v[2]), from_bf16(v[3])};
+  }
+  floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (i + q < to) v[q] = value<F32>(p, i + q);
+  return v;
+}
+
 // Packed operands: rows of Kp values (zeros behind the contraction), or for three parts rows of 3 Kp with 32 values of
 // each part side by side: value k of part q at (k / 32) * 96 + q * 32 + k % 32.
 template <int NP>
@@ -102,7 +122,8 @@ __global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int 
   }
 }
 
-// src [R, H] -> transposed, packed [H][Rp], zeros behind R and (LEFT) in rows left out, whatever they hold.
+// src [R, H] -> transposed, packed rows of stride Rp, zeros behind R up to kPad and (LEFT) in rows left out, whatever
+// they hold.
 template <bool F32, int NP, bool LEFT>
 __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
                                                      Rows rows, uint16_t* __restrict__ dst) {
@@ -156,9 +177,10 @@ struct GemmArgs {
   float* hit;                // E_LSE, indices: [N] the target's logit
   const float* stats;        // E_DL
   const float* g;
-  uint16_t* P;               // E_DL: packed [N][ldp]
-  uint16_t* Pt;              // packed [M][ldpt]
-  int64_t ldp, ldpt;         // classes and rows with their padding
+  const float* scale;        // E_DL: dl is stored over it; E_OUT: the result is multiplied by it (may be NULL: 1)
+  uint16_t* P;               // E_DL: packed [N][ldp], classes zero-padded to mp
+  uint16_t* Pt;              // packed [M][ldpt], rows zero-padded to np
+  int64_t ldp, ldpt, mp, np;
   float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
   // products
   void* out;                 // E_OUT: [N][ldo]
@@ -210,21 +232,26 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
   static_assert(IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
   constexpr int TILE = (BM + BN) * S::ROW;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE];
+  constexpr int PAD = 16;  // values a staged row of dl is longer
+  constexpr int STAGE = EPI != E_DL ? 0 : BN * (BM + PAD) > BM * (BN + PAD) ? BN * (BM + PAD) : BM * (BN + PAD);
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE > STAGE ? 2 * TILE : STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // Tile of this workgroup: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the tile order,
-  // and the order walks blocks of eight tiles of A by all of B: what an XCD reads at a time stays in its own cache.
-  int tile_m, tile_n;
+  // Tile of this workgroup: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the order: split
+  // by split, and within one in blocks of eight tiles of A by all of B.  What an XCD reads at a time stays in its cache.
+  int tile_m, tile_n, split_k;
   {
-    const uint32_t nt = (uint32_t)(a.tm * a.tn), tn = (uint32_t)a.tn, bid = blockIdx.x;
-    const uint32_t q = nt >> 3, r = nt & 7, xcd = bid & 7;
-    const uint32_t lin = xcd * q + (xcd < r ? xcd : r) + (bid >> 3);
+    const uint32_t nt = (uint32_t)(a.tm * a.tn), tn = (uint32_t)a.tn, all = gridDim.x, bid = blockIdx.x;
+    const uint32_t q = all >> 3, r = all & 7, xcd = bid & 7;
+    uint32_t lin = xcd * q + (xcd < r ? xcd : r) + (bid >> 3);
+    const uint32_t sp = lin / nt;
+    lin -= sp * nt;
     const uint32_t grp = lin / (8 * tn), in = lin - grp * 8 * tn;
     const uint32_t left = (uint32_t)a.tm - grp * 8, gm = left < 8 ? left : 8;
     tile_m = __builtin_amdgcn_readfirstlane((int)(grp * 8 + in % gm));
     tile_n = __builtin_amdgcn_readfirstlane((int)(in / gm));
+    split_k = __builtin_amdgcn_readfirstlane((int)sp);
   }
   const int64_t m0 = (int64_t)tile_m * BM, n0 = (int64_t)tile_n * BN;
 
@@ -243,7 +270,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
     const int64_t most = i < IA ? a.M - 1 - m0 : a.N - 1 - n0;
     off[i] = (uint32_t)((r < most ? r : most) * (i < IA ? a.lda : a.ldb) + c * 8) * 2u;
   }
-  const int k_from = blockIdx.y * a.per_split;
+  const int k_from = split_k * a.per_split;
   const int k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
   // Buffer descriptors of the tile's rows; a load behind the last step goes through one of no bytes and reads nothing.
   const uint16_t* base_a = a.A + m0 * a.lda;
@@ -352,6 +379,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   const int64_t nb = n0 + wn * (BN / WN) + fr;
 
   if constexpr (EPI == E_OUT) {
+    const float scale = a.scale ? *a.scale : 1.f;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
       const int64_t n = nb + j * 16;
@@ -360,9 +388,9 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
       for (int i = 0; i < RT; ++i) {
         const int64_t m = mb + i * 16;
         if (m >= a.M) continue;
-        floatx4 v = acc[i][j];
+        floatx4 v = acc[i][j] * scale;
         if (a.acc) {
-          floatx4* p = reinterpret_cast<floatx4*>(a.acc + ((int64_t)blockIdx.y * a.N + n) * a.ldacc + m);
+          floatx4* p = reinterpret_cast<floatx4*>(a.acc + ((int64_t)split_k * a.N + n) * a.ldacc + m);
           if (a.add) v += *p;
           *p = v;
         } else if (F32) {
@@ -390,16 +418,27 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
     return;
   }
 
-  // logits: bias, classes behind the last at -inf
+  // logits: the bias, and classes behind the last at -inf
+  if (a.bias) {
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i) {
+      const int64_t m = mb + i * 16;
+      const floatx4 bv = m < a.M ? four<F32>(a.bias, m, a.M) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t m = mb + i * 16 + q;
-      const float bv = m < a.M ? (a.bias ? value<F32>(a.bias, m) : 0.f) : 0.f;
-#pragma unroll
-      for (int j = 0; j < CT; ++j) acc[i][j][q] = m < a.M ? acc[i][j][q] + bv : -INFINITY;
+      for (int j = 0; j < CT; ++j) acc[i][j] += bv;
     }
+  }
+  if (m0 + BM > a.M) {
+    const int left = (int)(a.M - mb);  // of this lane's rows of A
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = i * 16 + q < left;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) acc[i][j][q] = in ? acc[i][j][q] : -INFINITY;
+      }
+  }
 
   if constexpr (EPI == E_LSE) {
     float* sm = reinterpret_cast<float*>(lds);  // [4][WM][BN]
@@ -415,35 +454,39 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float ref = top == -INFINITY ? 0.f : top;
+      const float off2 = -ref * kLog2e;
       float sum = 0.f, dot = 0.f, mass = 0.f;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * kLog2e);
+        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
       if (a.rows.kind == GNCDE_TARGET_ROWS) {
         if (in) {
           const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
+          for (int i = 0; i < RT; ++i) {
+            const int64_t m = mb + i * 16;
+            const floatx4 yv = m < a.M ? four<true>(y, m, a.M) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const int64_t m = mb + i * 16 + q;
-              const float yv = m < a.M ? y[m] : 0.f;
-              mass += yv;
-              dot += yv == 0.f ? 0.f : yv * acc[i][j][q];  // a class at -inf without mass adds nothing
+              mass += yv[q];
+              dot += yv[q] == 0.f ? 0.f : yv[q] * acc[i][j][q];  // a class at -inf without mass adds nothing
             }
+          }
         }
         dot += __shfl_xor(dot, 16);
         dot += __shfl_xor(dot, 32);
         mass += __shfl_xor(mass, 16);
         mass += __shfl_xor(mass, 32);
-      } else if (in) {
-        const int64_t t = row_index(a.rows, n) - a.v0 - mb;
+      } else {
+        const int64_t t = in ? row_index(a.rows, n) - a.v0 - mb : -1;
+        if (__any(t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+          for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (t == i * 16 + q && mb + t < a.M) a.hit[n] = acc[i][j][q];
+            for (int q = 0; q < 4; ++q)
+              if (t == i * 16 + q && mb + t < a.M) a.hit[n] = acc[i][j][q];
+        }
       }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
@@ -478,60 +521,132 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
 
   if constexpr (EPI == E_DL) {
     const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
+    const float inv = a.scale ? *a.scale : 1.f;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
       const int64_t n = nb + j * 16;
       const bool in = n < a.N && row_counts(a.rows, n);
-      const float lse = in ? a.stats[2 * n] : 0.f, gv = in ? a.g[n] : 0.f;
-      const float gs = in ? gv * a.stats[2 * n + 1] : 0.f;
-      const int64_t t = (in && !soft) ? row_index(a.rows, n) - a.v0 - mb : -1;
-      const float* y = (in && soft) ? static_cast<const float*>(a.rows.target) + n * a.V + a.v0 : nullptr;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        uint16_t p[4][NP];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int64_t m = mb + i * 16 + q;
-          float d = gs * __builtin_amdgcn_exp2f((acc[i][j][q] - lse) * kLog2e);
-          if (soft) d -= (in && m < a.M) ? gv * y[m] : 0.f;
-          else d -= t == i * 16 + q ? gv : 0.f;
-          d = (in && m < a.M) ? d : 0.f;
-          acc[i][j][q] = d;
-          split<NP>(d, p[q]);
-        }
-        const int64_t m = mb + i * 16;
-        if (n < a.N && m < a.ldp) {
-#pragma unroll
-          for (int s = 0; s < NP; ++s)
-            *reinterpret_cast<u16x4*>(a.P + n * NP * a.ldp + packed<NP>(m, s)) = u16x4{p[0][s], p[1][s], p[2][s], p[3][s]};
-        }
-        if (n < a.ldpt) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (m + q < a.M) {
-#pragma unroll
-              for (int s = 0; s < NP; ++s) a.Pt[(m + q) * NP * a.ldpt + packed<NP>(n, s)] = p[q][s];
-            }
-        }
-      }
-    }
-    if (a.part_b) {
+      const float gv = in ? a.g[n] / inv : 0.f, gs = in ? gv * a.stats[2 * n + 1] : 0.f;
+      const float off2 = in ? -a.stats[2 * n] * kLog2e : 0.f;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float s = 0.f;
+        for (int q = 0; q < 4; ++q)
+          acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+      if (soft) {
+        if (in) {
+          const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
 #pragma unroll
-          for (int j = 0; j < CT; ++j) s += acc[i][j][q];
-          s += __shfl_xor(s, 1);
-          s += __shfl_xor(s, 2);
-          s += __shfl_xor(s, 4);
-          s += __shfl_xor(s, 8);
-          const int64_t m = mb + i * 16 + q;
-          if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = s;
+          for (int i = 0; i < RT; ++i) {
+            const int64_t m = mb + i * 16;
+            if (m < a.M) acc[i][j] -= gv * four<true>(y, m, a.M);
+          }
         }
+      } else {
+        const int64_t t = in ? row_index(a.rows, n) - a.v0 - mb : -1;
+        if (__any(t >= 0 && t < RT * 16)) {  // few tiles hold a target
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] -= t == i * 16 + q ? gv : 0.f;
+        }
+      }
+      if (!__all(in)) {  // rows left out, whatever their logits
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][q] = in ? acc[i][j][q] : 0.f;
+      }
+    }
+    if (m0 + BM > a.M) {  // classes behind the last: an lse of NaN must not reach them
+      const int left = (int)(a.M - mb);
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < CT; ++j) acc[i][j][q] = i * 16 + q < left ? acc[i][j][q] : 0.f;
+    }
+    if (a.part_b) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        floatx4 s = acc[i][0];
+#pragma unroll
+        for (int j = 1; j < CT; ++j) s += acc[i][j];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float r = s[q];
+          r += __shfl_xor(r, 1);
+          r += __shfl_xor(r, 2);
+          r += __shfl_xor(r, 4);
+          r += __shfl_xor(r, 8);
+          const int64_t m = mb + i * 16 + q;
+          if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = r;
+        }
+      }
+    }
+    // dl goes out through LDS, once as rows of classes and once as classes of rows, in whole 16-byte chunks: written
+    // from the registers, its 8 and 2 byte pieces cost 31 us a 256 x 256 tile where the staged ones cost 12.
+    constexpr int THREADS = NW * 64;
+    const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
+#pragma unroll
+    for (int s = 0; s < NP; ++s) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const floatx4 v = acc[i][j];
+          *reinterpret_cast<u16x4*>(lds + (ln + j * 16) * (BM + PAD) + lm + i * 16) =
+              u16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+        }
+      __syncthreads();
+#pragma unroll 2
+      for (int e = threadIdx.x; e < BN * (BM / 8); e += THREADS) {
+        const int row = e / (BM / 8), c = e % (BM / 8) * 8;
+        if (n0 + row < a.N && m0 + c < a.mp)
+          *reinterpret_cast<u16x8*>(a.P + (n0 + row) * NP * a.ldp + packed<NP>(m0 + c, s)) =
+              *reinterpret_cast<const u16x8*>(lds + row * (BM + PAD) + c);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint16_t part = to_bf16(acc[i][j][q]);
+            lds[(lm + i * 16 + q) * (BN + PAD) + ln + j * 16] = part;
+            if (NP > 1) acc[i][j][q] -= from_bf16(part);  // what the next part holds
+          }
+      __syncthreads();
+#pragma unroll 2
+      for (int e = threadIdx.x; e < BM * (BN / 8); e += THREADS) {
+        const int row = e / (BN / 8), c = e % (BN / 8) * 8;
+        if (m0 + row < a.M && n0 + c < a.np)
+          *reinterpret_cast<u16x8*>(a.Pt + (m0 + row) * NP * a.ldpt + packed<NP>(n0 + c, s)) =
+              *reinterpret_cast<const u16x8*>(lds + row * (BN + PAD) + c);
+      }
+      if (s + 1 < NP) __syncthreads();
     }
   }
+}
+
+// The scale of dl: the largest |g| of the rows that count (1 where that is no use).  bf16 dl is stored over it, so that
+// the equal cotangents of a mean leave the target's entry, nearly all of dl, near -1 and not at a rounded -g: the
+// gradients' error is then that of their own rounding (2e-3 instead of 3e-3 of the norm at 8192 rows).
+__global__ void __launch_bounds__(1024) k_xent_scale(int64_t N, Rows rows, const float* __restrict__ g,
+                                                     float* __restrict__ scale) {
+  __shared__ float red[16];
+  float m = 0.f;
+  for (int64_t n = threadIdx.x; n < N; n += 1024) m = fmaxf(m, row_counts(rows, n) ? fabsf(g[n]) : 0.f);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
+  *scale = m > 1e-30f && m < 1e30f ? m : 1.f;
 }
 
 // A pair (largest, sum of exponentials relative to it) joined with another.
@@ -592,11 +707,13 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
 // out[i] = sum over splits of acc[s][i], in the split order.
 template <bool F32>
 __global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __restrict__ acc, int64_t ldacc,
-                           int64_t stride, void* __restrict__ out, int64_t ldo) {
+                           int64_t stride, const float* __restrict__ scale, void* __restrict__ out, int64_t ldo) {
+  const float by = scale ? *scale : 1.f;
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * M; e += (int64_t)gridDim.x * blockDim.x) {
     const int64_t n = e / M, m = e - n * M;
     float s = 0.f;
     for (int k = 0; k < splits; ++k) s += acc[k * stride + n * ldacc + m];
+    s *= by;
     if (F32) static_cast<float*>(out)[n * ldo + m] = s;
     else static_cast<uint16_t*>(out)[n * ldo + m] = to_bf16(s);
   }
@@ -642,26 +759,6 @@ struct SmallArgs {
   void* gx;                    // may be NULL
   float* part;                 // [workgroups][V H + V]; NULL without gW and gb
 };
-
-// Values at p[i..i+3], zeros from `to` on.
-template <bool F32>
-__device__ __forceinline__ floatx4 four(const void* p, int64_t i, int64_t to) {
-  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-  typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
-  if (i + 4 <= to) {
-    if (F32) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-      return floatx4{v[0], v[1], v[2], v[3]};
-    }
-    const u16x4u v = *reinterpret_cast<const u16x4u*>(static_cast<const uint16_t*>(p) + i);
-    return floatx4{from_bf16(v[0]), from_bf16(v[1]), from_bf16(v[2]), from_bf16(v[3])};
-  }
-  floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    if (i + q < to) v[q] = value<F32>(p, i + q);
-  return v;
-}
 
 template <bool F32, bool GRAD>
 __global__ void __launch_bounds__(kSmallThreads) k_xent_small(SmallArgs a) {
@@ -1170,6 +1267,10 @@ __global__ void __launch_bounds__(256) k_xent_few_out(int N, int H, int64_t V, i
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
+// Row stride of an operand in the workspace: padded to kPad, and an odd number of 128-byte lines, so that the rows of a
+// tile do not all fall on the same channels (a stride of 8 KB cost the gW product a third of its rate).
+int64_t stride_of(int64_t k) { return up(k, kPad) | kPad; }
+
 constexpr int64_t kCus = 256;
 constexpr int64_t kMostBlocks = int64_t(1) << 20;  // of the element-wise kernels: the rest by their loops
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
@@ -1182,12 +1283,13 @@ struct Plan {
   int ks = 1, xs = 0;
   bool f32, direct_ok;  // direct_ok: sizes allow x and W as operands as they lie (the pointers decide too)
   int np;
-  int64_t Kp, Np;
+  int64_t Kp, Np;       // packed contraction of x and W; rows padded
+  int64_t Ns;           // row stride of x^T and dl^T
   int64_t piece;        // classes a piece
   int64_t bytes = 0;
   // offsets
   int64_t o_x = 0, o_w = 0, o_part = 0, o_party = 0, o_hit = 0, o_run = 0;
-  int64_t o_xt = 0, o_wt = 0, o_p = 0, o_pt = 0, o_gx = 0, o_gw = 0, o_b = 0;
+  int64_t o_scale = 0, o_xt = 0, o_wt = 0, o_p = 0, o_pt = 0, o_gx = 0, o_gw = 0, o_b = 0;
   int64_t gx_split = 1, gw_split = 1, ldacc = 0;
 
   int64_t take(int64_t n) {
@@ -1240,6 +1342,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   p.np = p.f32 ? 3 : 1;
   p.direct_ok = !p.f32 && H % 8 == 0;
   p.Kp = up(H, 64), p.Np = up(std::max<int64_t>(N, 1), 64);
+  p.Ns = stride_of(p.Np);
   p.small = small_fits(H, V);
   if (p.small) {
     p.o_b = p.take(grad ? 4 * small_groups(N) * (V * H + V) : 0);
@@ -1269,7 +1372,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   }
   const int64_t plane = 2 * p.np;
   // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
-  const int64_t per_class = grad ? plane * (2 * p.Np + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
+  const int64_t per_class = grad ? plane * (p.Ns + N + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
   p.piece = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256));
   // W as it lies may still be unusable (its address): the packed piece has its place in any case.
   p.o_x = p.take(plane * N * p.Kp);
@@ -1280,10 +1383,11 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
     p.o_hit = p.take(4 * N);
     p.o_run = p.take(16 * N);
   } else {
-    p.o_xt = p.take(plane * H * p.Np);
-    p.o_wt = p.take(plane * H * p.piece);
-    p.o_p = p.take(plane * N * p.piece);
-    p.o_pt = p.take(plane * p.piece * p.Np);
+    p.o_scale = p.take(4);
+    p.o_xt = p.take(plane * H * p.Ns);
+    p.o_wt = p.take(plane * H * stride_of(p.piece));
+    p.o_p = p.take(plane * N * stride_of(p.piece));
+    p.o_pt = p.take(plane * p.piece * p.Ns);
     p.ldacc = up(H, 4);
     const int64_t vc = std::min(p.piece, V);
     p.gx_split = split_of(H, N, steps_of(vc, p.np), p.np);
@@ -1303,7 +1407,7 @@ void mm(const GemmArgs& in, int64_t splits, hipStream_t st) {
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
   a.kt = (int)steps_of(a.K, NP);
   a.per_split = (int)div_up(a.kt, splits);
-  const dim3 grid((unsigned)(a.tm * a.tn), (unsigned)splits);
+  const dim3 grid((unsigned)(a.tm * a.tn * splits));
   if (t.big) {
     if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
@@ -1320,9 +1424,9 @@ void pack(const void* src, int64_t R, const Plan& p, uint16_t* dst, hipStream_t 
 }
 
 template <bool F32, bool LEFT>
-void pack_t(const void* src, int64_t R, int64_t Rp, const Plan& p, Rows rows, uint16_t* dst, hipStream_t st) {
-  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)(Rp / 64 * div_up(p.H, 64))), dim3(256),
-                     0, st, src, R, (int)p.H, Rp, rows, dst);
+void pack_t(const void* src, int64_t R, int64_t stride, const Plan& p, Rows rows, uint16_t* dst, hipStream_t st) {
+  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)(div_up(R, 64) * div_up(p.H, 64))),
+                     dim3(256), 0, st, src, R, (int)p.H, stride, rows, dst);
 }
 
 bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -1418,10 +1522,10 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
 }
 
 template <bool F32>
-void sum_out(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t ldacc, int64_t stride, void* out,
-             int64_t ldo, hipStream_t st) {
+void sum_out(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t ldacc, int64_t stride, const float* scale,
+             void* out, int64_t ldo, hipStream_t st) {
   hipLaunchKernelGGL((k_xent_sum<F32>), dim3((unsigned)std::min(div_up(N * M, 256), kMostBlocks)), dim3(256), 0, st, N,
-                     M, (int)splits, acc, ldacc, stride, out, ldo);
+                     M, (int)splits, acc, ldacc, stride, scale, out, ldo);
 }
 
 template <bool F32>
@@ -1471,27 +1575,35 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
   float* acc_x = reinterpret_cast<float*>(c.ws + p.o_gx);
   float* acc_w = reinterpret_cast<float*>(c.ws + p.o_gw);
   float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
-  if (gW) pack_t<F32, true>(c.x, p.N, p.Np, p, c.rows, xt, c.st);
+  if (gW) pack_t<F32, true>(c.x, p.N, p.Ns, p, c.rows, xt, c.st);
+  float* scale = nullptr;
+  if (!F32) {
+    scale = reinterpret_cast<float*>(c.ws + p.o_scale);
+    hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(1024), 0, c.st, p.N, c.rows, g, scale);
+  }
   const bool one = p.piece >= p.V;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
-    const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, 64);
+    const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad), vs = stride_of(vc);
     const char* wsrc = static_cast<const char*>(c.W) + v0 * p.H * SZ;
     const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
     GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
     a.stats = stats, a.g = g;
-    a.P = P, a.ldp = vp;
-    a.Pt = Pt, a.ldpt = p.Np;
+    a.scale = scale;
+    a.P = P, a.ldp = vs, a.mp = vp;
+    a.Pt = Pt, a.ldpt = p.Ns, a.np = p.Np;
     a.part_b = gb ? part_b : nullptr;
     mm<E_DL, F32>(a, 1, c.st);
     if (gb) {
       const Tile t = tile_of(vc, p.N, p.np);
-      sum_out<F32>(1, vc, div_up(p.N, t.bn) * t.wn, part_b, vc, vc, static_cast<char*>(gb) + v0 * SZ, vc, c.st);
+      sum_out<F32>(1, vc, div_up(p.N, t.bn) * t.wn, part_b, vc, vc, scale,
+                   static_cast<char*>(gb) + v0 * SZ, vc, c.st);
     }
     if (gx) {
-      pack_t<F32, false>(wsrc, vc, vp, p, c.rows, wt, c.st);
+      pack_t<F32, false>(wsrc, vc, vs, p, c.rows, wt, c.st);
       GemmArgs q = {};
-      q.A = wt, q.lda = p.np * vp, q.M = p.H;
-      q.B = P, q.ldb = p.np * vp, q.N = p.N;
+      q.scale = scale;
+      q.A = wt, q.lda = p.np * vs, q.M = p.H;
+      q.B = P, q.ldb = p.np * vs, q.N = p.N;
       q.K = (int)vp;
       q.out = gx, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(gx, 4 * SZ);
       const int64_t sp = split_of(p.H, p.N, steps_of(vp, p.np), p.np);
@@ -1501,19 +1613,21 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       const int64_t use = std::min(sp, p.gx_split);
       mm<E_OUT, F32>(q, use, c.st);
       if (sums && v0 + p.piece >= p.V)
-        sum_out<F32>(p.N, p.H, one ? use : p.gx_split, acc_x, p.ldacc, p.N * p.ldacc, gx, p.H, c.st);
+        sum_out<F32>(p.N, p.H, one ? use : p.gx_split, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H,
+                     c.st);
     }
     if (gW) {
       GemmArgs q = {};
-      q.A = xt, q.lda = p.np * p.Np, q.M = p.H;
-      q.B = Pt, q.ldb = p.np * p.Np, q.N = vc;
+      q.scale = scale;
+      q.A = xt, q.lda = p.np * p.Ns, q.M = p.H;
+      q.B = Pt, q.ldb = p.np * p.Ns, q.N = vc;
       q.K = (int)p.Np;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(out, 4 * SZ);
       const int64_t sp = std::min(split_of(p.H, vc, steps_of(p.Np, p.np), p.np), p.gw_split);
       if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
       mm<E_OUT, F32>(q, sp, c.st);
-      if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, out, p.H, c.st);
+      if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H, c.st);
     }
   }
 }
@@ -1571,11 +1685,11 @@ int gncde_linear_cross_entropy_grad(int64_t rows, int64_t hidden, int64_t classe
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows == 0) {  // no row: gradients of nothing
     if (p.f32) {
-      if (gW) gncde::sum_out<true>(classes, hidden, 0, nullptr, 0, 0, gW, hidden, st);
-      if (gb) gncde::sum_out<true>(1, classes, 0, nullptr, 0, 0, gb, classes, st);
+      if (gW) gncde::sum_out<true>(classes, hidden, 0, nullptr, 0, 0, nullptr, gW, hidden, st);
+      if (gb) gncde::sum_out<true>(1, classes, 0, nullptr, 0, 0, nullptr, gb, classes, st);
     } else {
-      if (gW) gncde::sum_out<false>(classes, hidden, 0, nullptr, 0, 0, gW, hidden, st);
-      if (gb) gncde::sum_out<false>(1, classes, 0, nullptr, 0, 0, gb, classes, st);
+      if (gW) gncde::sum_out<false>(classes, hidden, 0, nullptr, 0, 0, nullptr, gW, hidden, st);
+      if (gb) gncde::sum_out<false>(1, classes, 0, nullptr, 0, 0, nullptr, gb, classes, st);
     }
     return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
   }
