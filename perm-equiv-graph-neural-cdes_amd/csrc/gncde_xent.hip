@@ -128,16 +128,21 @@ template <bool F32, int NP, bool LEFT>
 __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
                                                      Rows rows, uint16_t* __restrict__ dst) {
   __shared__ float t[64][65];
+  __shared__ bool keep[64];
   const int64_t ht = (H + 63) / 64;
   const int64_t r0 = (blockIdx.x / ht) * 64;
   const int h0 = (int)(blockIdx.x % ht) * 64;
   const int c = threadIdx.x & 63, q4 = threadIdx.x >> 6;
-  for (int i = q4; i < 64; i += 4) {
-    const int64_t r = r0 + i;
-    const int h = h0 + c;
-    const bool in = r < R && h < H && (!LEFT || row_counts(rows, r));
-    t[i][c] = in ? value<F32>(src, r * H + h) : 0.f;
+  if (LEFT && threadIdx.x < 64) keep[c] = r0 + c < R && row_counts(rows, r0 + c);
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t r = r0 + q4 + 4 * i;
+    v[i] = r < R && h0 + c < H ? value<F32>(src, r * H + h0 + c) : 0.f;
   }
+  if (LEFT) __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[q4 + 4 * i][c] = !LEFT || keep[q4 + 4 * i] ? v[i] : 0.f;
   __syncthreads();
   const int rc = (threadIdx.x & 7) * 8, hh = threadIdx.x >> 3;
   for (int i = hh; i < 64; i += 32) {
@@ -158,6 +163,7 @@ __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ sr
 
 // ---- the product ------------------------------------------------------------------------------------------------
 enum { E_LSE = 0, E_DL = 1, E_OUT = 2 };
+constexpr int kLeftOut = -2;
 
 struct GemmArgs {
   const uint16_t* A;
@@ -172,8 +178,9 @@ struct GemmArgs {
   Rows rows;
   const void* bias;          // this piece's
   int64_t v0, V;             // first class of the piece, classes in all
-  float2* part;              // E_LSE: [N][tm] (largest, sum of exponentials)
-  float2* part_y;            // E_LSE, label rows: [N][tm] (sum y l, sum y)
+  float2* part;              // E_LSE: [N][part_ld] (largest, sum of exponentials), this launch's tiles from part_at
+  float2* part_y;            // E_LSE, label rows: likewise (sum y l, sum y)
+  int64_t part_ld, part_at;
   float* hit;                // E_LSE, indices: [N] the target's logit
   const float* stats;        // E_DL
   const float* g;
@@ -235,6 +242,9 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   constexpr int PAD = 16;  // values a staged row of dl is longer
   constexpr int STAGE = EPI != E_DL ? 0 : BN * (BM + PAD) > BM * (BN + PAD) ? BN * (BM + PAD) : BM * (BN + PAD);
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE > STAGE ? 2 * TILE : STAGE];
+  // What the logits' epilogues need of a row of x, fetched while the first step's operands are on their way:
+  // -lse log2 e, g over the scale, the same times S, and the target's class within the piece (-1: none there; kLeftOut).
+  __shared__ __attribute__((aligned(16))) floatx4 info[EPI == E_OUT ? 1 : BN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
@@ -332,8 +342,27 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
   };
 
+  if (EPI != E_OUT && k_from < k_to) load(k_from, 0);
+  if constexpr (EPI != E_OUT) {
+    for (int r = threadIdx.x; r < BN; r += NW * 64) {
+      const int64_t n = n0 + r;
+      const bool in = n < a.N && row_counts(a.rows, n);
+      floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+      int t = in ? -1 : kLeftOut;
+      if (in && a.rows.kind != GNCDE_TARGET_ROWS) {
+        const int64_t c = row_index(a.rows, n) - a.v0;
+        if (c >= 0 && c < a.M) t = (int)c;
+      }
+      if (EPI == E_DL && in) {
+        const float gv = a.g[n] / (a.scale ? *a.scale : 1.f);
+        v = floatx4{-a.stats[2 * n] * kLog2e, gv, gv * a.stats[2 * n + 1], 0.f};
+      }
+      v[3] = __int_as_float(t);
+      info[r] = v;
+    }
+  }
   if (k_from < k_to) {
-    load(k_from, 0);
+    if (EPI == E_OUT) load(k_from, 0);
     hand_over(k_from, 0);
     load(k_from + 1, 1);
     if constexpr (NP == 1) {
@@ -445,7 +474,8 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
       const int64_t n = nb + j * 16;
-      const bool in = n < a.N && row_counts(a.rows, n);
+      const int target = __float_as_int(info[wn * (BN / WN) + j * 16 + fr][3]);
+      const bool in = target != kLeftOut;
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -479,13 +509,13 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
         mass += __shfl_xor(mass, 16);
         mass += __shfl_xor(mass, 32);
       } else {
-        const int64_t t = in ? row_index(a.rows, n) - a.v0 - mb : -1;
-        if (__any(t >= 0 && t < RT * 16)) {  // few tiles hold a target
+        const int t = target - (int)mb;
+        if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              if (t == i * 16 + q && mb + t < a.M) a.hit[n] = acc[i][j][q];
+              if (target >= 0 && t == i * 16 + q) a.hit[n] = acc[i][j][q];
         }
       }
       sum += __shfl_xor(sum, 16);
@@ -513,21 +543,21 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
         dot += sm[(2 * WM + w) * BN + col];
         mass += sm[(3 * WM + w) * BN + col];
       }
-      a.part[(n0 + col) * a.tm + tile_m] = make_float2(top, sum);
-      if (a.rows.kind == GNCDE_TARGET_ROWS) a.part_y[(n0 + col) * a.tm + tile_m] = make_float2(dot, mass);
+      a.part[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(top, sum);
+      if (a.rows.kind == GNCDE_TARGET_ROWS) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
     }
     return;
   }
 
   if constexpr (EPI == E_DL) {
     const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
-    const float inv = a.scale ? *a.scale : 1.f;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
       const int64_t n = nb + j * 16;
-      const bool in = n < a.N && row_counts(a.rows, n);
-      const float gv = in ? a.g[n] / inv : 0.f, gs = in ? gv * a.stats[2 * n + 1] : 0.f;
-      const float off2 = in ? -a.stats[2 * n] * kLog2e : 0.f;
+      const floatx4 row = info[wn * (BN / WN) + j * 16 + fr];
+      const int target = __float_as_int(row[3]);
+      const bool in = target != kLeftOut;
+      const float off2 = row[0], gv = row[1], gs = row[2];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -543,12 +573,12 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
           }
         }
       } else {
-        const int64_t t = in ? row_index(a.rows, n) - a.v0 - mb : -1;
-        if (__any(t >= 0 && t < RT * 16)) {  // few tiles hold a target
+        const int t = target - (int)mb;
+        if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[i][j][q] -= t == i * 16 + q ? gv : 0.f;
+            for (int q = 0; q < 4; ++q) acc[i][j][q] -= target >= 0 && t == i * 16 + q ? gv : 0.f;
         }
       }
       if (!__all(in)) {  // rows left out, whatever their logits
@@ -638,7 +668,19 @@ __global__ void __launch_bounds__(1024) k_xent_scale(int64_t N, Rows rows, const
                                                      float* __restrict__ scale) {
   __shared__ float red[16];
   float m = 0.f;
-  for (int64_t n = threadIdx.x; n < N; n += 1024) m = fmaxf(m, row_counts(rows, n) ? fabsf(g[n]) : 0.f);
+  for (int64_t n0 = threadIdx.x; n0 < N; n0 += 8192) {
+    float v[8];
+    bool in[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // side by side: one wait for all
+      const int64_t n = n0 + 1024 * i < N ? n0 + 1024 * i : n0;
+      v[i] = fabsf(g[n]);
+      in[i] = !rows.mask || rows.mask[n] != 0;
+      if (rows.kind != GNCDE_TARGET_ROWS) in[i] &= row_index(rows, n) >= 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, in[i] ? v[i] : 0.f);
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
@@ -1273,7 +1315,83 @@ int64_t stride_of(int64_t k) { return up(k, kPad) | kPad; }
 
 constexpr int64_t kCus = 256;
 constexpr int64_t kMostBlocks = int64_t(1) << 20;  // of the element-wise kernels: the rest by their loops
-constexpr int64_t kPieceBytes = int64_t(512) << 20;
+constexpr int64_t kPieceBytes = int64_t(1) << 30;  // of a piece's operands: fewer pieces are fewer passes over gx's sums
+
+struct Tile {
+  int64_t bm, bn, wn;
+};
+
+Tile tile_of(bool big, int np) { return big ? Tile{256, np == 1 ? 256 : 128, np == 1 ? 4 : 2} : Tile{128, 128, 2}; }
+
+int64_t steps_of(int64_t K, int np) { return np == 1 ? div_up(K, 64) : up(K, kPad) / 32; }
+
+struct Cfg {
+  bool big = true;  // 256 x 256 tiles (three parts: 256 x 128), else 128 x 128
+  int splits = 1;   // of the contraction
+  double us = 0;    // what the model below says
+};
+
+// The model that chooses tiles, splits and pieces: rounds of workgroups over the CUs, each its steps and a fixed part,
+// and the join of splits.  Measured on one MI355X in us: a step of a 256 x 256 tile 1.45 (1.5 PFLOP/s over 256 CUs), of
+// a 128 x 128 tile 0.83 alone on its CU and 1.05 beside another; of three parts 2.2 (256 x 128) and 1.5.  The large tile
+// is 1.4 to 2.3 times faster a product and loses where it leaves CUs without one: 784 tiles are four rounds of 256.
+Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, bool big, int64_t splits) {
+  const Tile t = tile_of(big, np);
+  const int64_t groups = div_up(M, t.bm) * div_up(N, t.bn) * splits;
+  const bool two = !big && np == 1 && groups > kCus;
+  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) : (big ? 2.2 : 1.5);
+  const double fixed = epi == E_DL ? (big ? 16 : 12) : 7;
+  Cfg c{big, (int)splits, (double)div_up(groups, two ? 2 * kCus : kCus) * ((double)div_up(kt, splits) * step + fixed)};
+  if (splits > 1) c.us += 5 + (double)splits * (double)N * (double)M * 8 / 4.5e6;
+  return c;
+}
+
+Cfg choose(int epi, int64_t M, int64_t N, int64_t kt, int np, int64_t most_splits) {
+  Cfg best = cost(epi, M, N, kt, np, true, 1);
+  const int64_t tiles = div_up(M, 256) * div_up(N, 256);
+  for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+    if (s > most_splits || s * 2 > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
+    for (const bool big : {true, false}) {
+      const Cfg c = cost(epi, M, N, kt, np, big, div_up(kt, div_up(kt, s)));  // no split without a step
+      if (c.us < best.us) best = c;
+    }
+  }
+  return best;
+}
+
+// A piece's classes as whole rounds of large tiles and the rest in small ones, where that is faster than one launch.
+struct Cover {
+  int64_t first = 0;  // classes of the first launch; the others go to the second
+  Cfg a, b;
+  double us = 0;
+};
+
+Cover cover(int epi, int64_t vc, int64_t N, int64_t kt, int np) {
+  Cover c;
+  c.first = vc, c.a = choose(epi, vc, N, kt, np, 1), c.us = c.a.us;
+  const int64_t tn = div_up(N, tile_of(true, np).bn), rounds = div_up(vc, 256) * tn / kCus;
+  const int64_t first = rounds * kCus / tn * 256;
+  if (first > 0 && first < vc) {
+    const Cfg a = cost(epi, first, N, kt, np, true, 1), b = choose(epi, vc - first, N, kt, np, 1);
+    if (a.us + b.us + 3 < c.us) c.first = first, c.a = a, c.b = b, c.us = a.us + b.us + 3;
+  }
+  return c;
+}
+
+struct PieceCfg {
+  Cover dl;
+  Cfg gx, gw;
+  double us = 0;
+};
+
+PieceCfg piece_cfg(int64_t N, int64_t H, int64_t vc, int np, int64_t most_gx) {
+  PieceCfg c;
+  c.dl = cover(E_DL, vc, N, steps_of(H, np), np);
+  c.gx = choose(E_OUT, H, N, steps_of(vc, np), np, most_gx);
+  c.gw = choose(E_OUT, H, vc, steps_of(N, np), np, 64);
+  c.us = c.dl.us + c.gx.us + c.gw.us + 10 + (double)H * (double)(vc * 4 * np + N * 8) / 3e6;
+  return c;
+}
 
 struct Plan {
   int64_t N, H, V;
@@ -1285,12 +1403,13 @@ struct Plan {
   int np;
   int64_t Kp, Np;       // packed contraction of x and W; rows padded
   int64_t Ns;           // row stride of x^T and dl^T
-  int64_t piece;        // classes a piece
+  int64_t piece, whole; // classes a piece; the loss's where W is used as it lies
   int64_t bytes = 0;
   // offsets
   int64_t o_x = 0, o_w = 0, o_part = 0, o_party = 0, o_hit = 0, o_run = 0;
   int64_t o_scale = 0, o_xt = 0, o_wt = 0, o_p = 0, o_pt = 0, o_gx = 0, o_gw = 0, o_b = 0;
-  int64_t gx_split = 1, gw_split = 1, ldacc = 0;
+  int64_t ldacc = 0;
+  PieceCfg full, last;  // the gradient's products for a full piece and the last one
 
   int64_t take(int64_t n) {
     const int64_t at = bytes;
@@ -1299,33 +1418,11 @@ struct Plan {
   }
 };
 
-struct Tile {
-  bool big;
-  int64_t bm, bn, wn;
-};
-
-// 256 x 256 tiles (three parts: 256 x 128, what LDS holds twice) read the least per product; below one for every CU,
-// 128 x 128 tiles keep more CUs at work.
-Tile tile_of(int64_t M, int64_t N, int np) {
-  const int64_t bn = np == 1 ? 256 : 128;
-  const bool big = div_up(M, 256) * div_up(N, bn) >= 200;
-  return big ? Tile{true, 256, bn, np == 1 ? 4 : 2} : Tile{false, 128, 128, 2};
-}
-
-int64_t steps_of(int64_t K, int np) { return np == 1 ? div_up(K, 64) : up(K, kPad) / 32; }
-
-// Splits of the contraction so that a product of few tiles fills the chip; at least four steps each.
-int64_t split_of(int64_t M, int64_t N, int64_t kt, int np) {
-  const Tile t = tile_of(M, N, np);
-  const int64_t tiles = div_up(M, t.bm) * div_up(N, t.bn);
-  const int64_t want = std::max<int64_t>(1, kCus / std::max<int64_t>(tiles, 1));
-  const int64_t most = std::max<int64_t>(1, kt / 4);
-  int64_t s = std::min({want, most, kt, int64_t(64)});
-  return div_up(kt, div_up(kt, s));  // no split without a step
-}
-
 // Workgroups of the small gradient: one for each CU, each with its share of the row tiles and one part of gW.
 int64_t small_groups(int64_t N) { return std::min(div_up(std::max<int64_t>(N, 1), 16), kCus); }
+
+// Rows of the bias's sums: tile columns times waves across, of either tile size.
+int64_t bias_rows(int64_t N) { return 4 * div_up(N, 128); }
 
 // Columns a thread of k_xent_few_out takes: what its rows of x and gx leave registers for.
 int64_t few_cols(int64_t N) { return N > 4 ? 4 : 8; }
@@ -1373,46 +1470,61 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   const int64_t plane = 2 * p.np;
   // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
   const int64_t per_class = grad ? plane * (p.Ns + N + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
-  p.piece = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256));
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256);
+  p.piece = std::min(up(V, 256), most);
+  p.whole = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np / 8 + 16) / 256 * 256));
+  if (grad && p.piece < V) {  // of several pieces: the size whose products fill the CUs best
+    double best = 0;
+    for (int64_t i = 0; i < 16; ++i) {
+      const int64_t grain = i < 8 ? 2048 : 256, at = i < 8 ? 16 - i : 24 - i;
+      const int64_t c = most * at / 16 / grain * grain;
+      if (c < 256) continue;
+      const int64_t n = V / c, rest = V - n * c;
+      const double us = (double)n * piece_cfg(N, H, c, p.np, 64).us + (rest ? piece_cfg(N, H, rest, p.np, 64).us : 0);
+      if (best == 0 || us < best) best = us, p.piece = c;
+    }
+  }
   // W as it lies may still be unusable (its address): the packed piece has its place in any case.
   p.o_x = p.take(plane * N * p.Kp);
   p.o_w = p.take(plane * std::min(p.piece, V) * p.Kp);
   if (!grad) {
-    p.o_part = p.take(8 * N * (p.piece / 128));
-    p.o_party = p.take(8 * N * (p.piece / 128));
+    const int64_t tiles = std::max(p.piece, p.direct_ok ? p.whole : 0) / 128;
+    p.o_part = p.take(8 * N * tiles);
+    p.o_party = p.take(8 * N * tiles);
     p.o_hit = p.take(4 * N);
     p.o_run = p.take(16 * N);
   } else {
+    const int64_t vc = std::min(p.piece, V), rest = V % p.piece ? V % p.piece : vc;
+    p.full = piece_cfg(N, H, vc, p.np, 64);
+    // the last one adds to the sums that the others left
+    p.last = rest == vc ? p.full : piece_cfg(N, H, rest, p.np, p.full.gx.splits);
     p.o_scale = p.take(4);
     p.o_xt = p.take(plane * H * p.Ns);
     p.o_wt = p.take(plane * H * stride_of(p.piece));
     p.o_p = p.take(plane * N * stride_of(p.piece));
     p.o_pt = p.take(plane * p.piece * p.Ns);
     p.ldacc = up(H, 4);
-    const int64_t vc = std::min(p.piece, V);
-    p.gx_split = split_of(H, N, steps_of(vc, p.np), p.np);
-    p.gw_split = split_of(H, vc, steps_of(p.Np, p.np), p.np);
-    p.o_gx = p.take(4 * p.gx_split * N * p.ldacc);
-    p.o_gw = p.take(p.gw_split > 1 ? 4 * p.gw_split * vc * p.ldacc : 0);
-    p.o_b = p.take(4 * 4 * div_up(N, 128) * vc);  // tile columns times waves across, of either tile size
+    p.o_gx = p.take(4 * std::max(p.full.gx.splits, p.last.gx.splits) * N * p.ldacc);
+    const int64_t a = p.full.gw.splits > 1 ? p.full.gw.splits * vc : 0;
+    const int64_t b = p.last.gw.splits > 1 ? p.last.gw.splits * rest : 0;
+    p.o_gw = p.take(4 * std::max(a, b) * p.ldacc);
+    p.o_b = p.take(4 * bias_rows(N) * vc);
   }
   return true;
 }
 
 template <int EPI, bool F32>
-void mm(const GemmArgs& in, int64_t splits, hipStream_t st) {
+void mm(const GemmArgs& in, const Cfg& cfg, hipStream_t st) {
   constexpr int NP = F32 ? 3 : 1;
   GemmArgs a = in;
-  const Tile t = tile_of(a.M, a.N, NP);
+  const Tile t = tile_of(cfg.big, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
   a.kt = (int)steps_of(a.K, NP);
-  a.per_split = (int)div_up(a.kt, splits);
-  const dim3 grid((unsigned)(a.tm * a.tn * splits));
-  if (t.big) {
-    if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
-  }
-  else hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
+  a.per_split = (int)div_up(a.kt, cfg.splits);
+  const dim3 grid((unsigned)(a.tm * a.tn * cfg.splits));
+  if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
+  else if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
 }
 
 template <bool F32>
@@ -1454,17 +1566,18 @@ Operand<F32> operand(const void* src, int64_t R, const Plan& p, int64_t at, cons
   return {dst, p.np * p.Kp, (int)p.Kp};
 }
 
+// The logits of classes v0 + at .. of a piece that starts at v0.
 template <bool F32>
-GemmArgs logits_args(const Operand<F32>& w, const Operand<F32>& x, const Plan& p, const Call& c, int64_t v0,
-                     int64_t vc) {
+GemmArgs logits_args(const Operand<F32>& w, const Operand<F32>& x, const Plan& p, const Call& c, int64_t v0, int64_t at,
+                     int64_t n) {
   GemmArgs a = {};
-  a.A = w.p, a.lda = w.ld, a.M = vc;
+  a.A = w.p + at * w.ld, a.lda = w.ld, a.M = n;
   a.B = x.p, a.ldb = x.ld, a.N = p.N;
   // one of the two may be packed (zeros behind H) and the other not
   a.K = std::min(w.K, x.K);
   a.rows = c.rows;
-  a.bias = c.b ? static_cast<const char*>(c.b) + v0 * (F32 ? 4 : 2) : nullptr;
-  a.v0 = v0, a.V = p.V;
+  a.bias = c.b ? static_cast<const char*>(c.b) + (v0 + at) * (F32 ? 4 : 2) : nullptr;
+  a.v0 = v0 + at, a.V = p.V;
   return a;
 }
 
@@ -1505,19 +1618,28 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
     return;
   }
   const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
-  for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
-    const int64_t vc = std::min(p.piece, p.V - v0);
+  const int64_t piece = p.direct_ok && aligned(c.W, 16) ? p.whole : p.piece;
+  for (int64_t v0 = 0; v0 < p.V; v0 += piece) {
+    const int64_t vc = std::min(piece, p.V - v0);
     const Operand<F32> w =
         operand<F32>(static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, p, p.o_w, c);
-    GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
-    a.part = reinterpret_cast<float2*>(c.ws + p.o_part);
-    a.part_y = reinterpret_cast<float2*>(c.ws + p.o_party);
-    a.hit = reinterpret_cast<float*>(c.ws + p.o_hit);
-    mm<E_LSE, F32>(a, 1, c.st);
-    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, c.st, p.N,
-                       div_up(vc, tile_of(vc, p.N, p.np).bm), a.part,
-                       c.rows.kind == GNCDE_TARGET_ROWS ? a.part_y : nullptr, a.hit, c.rows, p.V,
-                       reinterpret_cast<float4*>(c.ws + p.o_run), v0 == 0, v0 + p.piece >= p.V, loss, stats);
+    const Cover cv = cover(E_LSE, vc, p.N, steps_of(std::min(w.K, x.K), p.np), p.np);
+    const int64_t tiles_a = div_up(cv.first, tile_of(cv.a.big, p.np).bm);
+    const int64_t tiles = tiles_a + (cv.first < vc ? div_up(vc - cv.first, tile_of(cv.b.big, p.np).bm) : 0);
+    for (int64_t at = 0; at < vc; at += cv.first) {
+      GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, at == 0 ? cv.first : vc - cv.first);
+      a.part = reinterpret_cast<float2*>(c.ws + p.o_part);
+      a.part_y = reinterpret_cast<float2*>(c.ws + p.o_party);
+      a.part_ld = tiles, a.part_at = at == 0 ? 0 : tiles_a;
+      a.hit = reinterpret_cast<float*>(c.ws + p.o_hit);
+      mm<E_LSE, F32>(a, at == 0 ? cv.a : cv.b, c.st);
+      if (at != 0) break;
+    }
+    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)div_up(p.N, 4)), dim3(256), 0, c.st, p.N, tiles,
+                       reinterpret_cast<const float2*>(c.ws + p.o_part),
+                       c.rows.kind == GNCDE_TARGET_ROWS ? reinterpret_cast<const float2*>(c.ws + p.o_party) : nullptr,
+                       reinterpret_cast<const float*>(c.ws + p.o_hit), c.rows, p.V,
+                       reinterpret_cast<float4*>(c.ws + p.o_run), v0 == 0, v0 + piece >= p.V, loss, stats);
   }
 }
 
@@ -1585,18 +1707,24 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad), vs = stride_of(vc);
     const char* wsrc = static_cast<const char*>(c.W) + v0 * p.H * SZ;
+    const PieceCfg& cfg = v0 + p.piece >= p.V ? p.last : p.full;
     const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
-    GemmArgs a = logits_args<F32>(w, x, p, c, v0, vc);
-    a.stats = stats, a.g = g;
-    a.scale = scale;
-    a.P = P, a.ldp = vs, a.mp = vp;
-    a.Pt = Pt, a.ldpt = p.Ns, a.np = p.Np;
-    a.part_b = gb ? part_b : nullptr;
-    mm<E_DL, F32>(a, 1, c.st);
-    if (gb) {
-      const Tile t = tile_of(vc, p.N, p.np);
-      sum_out<F32>(1, vc, div_up(p.N, t.bn) * t.wn, part_b, vc, vc, scale,
-                   static_cast<char*>(gb) + v0 * SZ, vc, c.st);
+    for (int64_t at = 0; at < vc; at += cfg.dl.first) {
+      const int64_t len = at == 0 ? cfg.dl.first : vc - cfg.dl.first;
+      GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, len);
+      a.stats = stats, a.g = g;
+      a.scale = scale;
+      a.P = P + p.np * at, a.ldp = vs, a.mp = at + len < vc ? len : vp - at;
+      a.Pt = Pt + p.np * at * p.Ns, a.ldpt = p.Ns, a.np = p.Np;
+      a.part_b = gb ? part_b + bias_rows(p.N) * at : nullptr;
+      const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
+      mm<E_DL, F32>(a, one_cfg, c.st);
+      if (gb) {
+        const Tile t = tile_of(one_cfg.big, p.np);
+        sum_out<F32>(1, len, div_up(p.N, t.bn) * t.wn, a.part_b, len, len, scale,
+                     static_cast<char*>(gb) + (v0 + at) * SZ, len, c.st);
+      }
+      if (at != 0) break;
     }
     if (gx) {
       pack_t<F32, false>(wsrc, vc, vs, p, c.rows, wt, c.st);
@@ -1606,14 +1734,12 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       q.B = P, q.ldb = p.np * vs, q.N = p.N;
       q.K = (int)vp;
       q.out = gx, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(gx, 4 * SZ);
-      const int64_t sp = split_of(p.H, p.N, steps_of(vp, p.np), p.np);
-      // every piece's splits fill the same sums; the last piece may have fewer steps, and leaves the others as they are
-      const bool sums = !one || sp > 1;
+      // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
+      const bool sums = !one || cfg.gx.splits > 1;
       if (sums) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
-      const int64_t use = std::min(sp, p.gx_split);
-      mm<E_OUT, F32>(q, use, c.st);
+      mm<E_OUT, F32>(q, cfg.gx, c.st);
       if (sums && v0 + p.piece >= p.V)
-        sum_out<F32>(p.N, p.H, one ? use : p.gx_split, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H,
+        sum_out<F32>(p.N, p.H, one ? p.last.gx.splits : p.full.gx.splits, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H,
                      c.st);
     }
     if (gW) {
@@ -1624,9 +1750,9 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       q.K = (int)p.Np;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(out, 4 * SZ);
-      const int64_t sp = std::min(split_of(p.H, vc, steps_of(p.Np, p.np), p.np), p.gw_split);
+      const int sp = cfg.gw.splits;
       if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
-      mm<E_OUT, F32>(q, sp, c.st);
+      mm<E_OUT, F32>(q, cfg.gw, c.st);
       if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H, c.st);
     }
   }

@@ -60,9 +60,10 @@ def test_workspace_is_sized_for_what_is_accepted():
     for dtype in (_lib.DTYPE_FP32, _lib.DTYPE_BF16):
         for grad in (0, 1):
             assert f(1, 1, 1, dtype, grad) > 0
-            # a piece of the classes at a time: the workspace of a long batch does not grow with the vocabulary
+            # a piece of the classes at a time: the workspace of a long batch does not grow with the vocabulary (the
+            # size of a piece goes by how its products fill the GPU, the loss keeps a pair for 128 classes of a row)
             a, b = f(8192, 4096, 1 << 17, dtype, grad), f(8192, 4096, 1 << 20, dtype, grad)
-            assert a == b and a < 4 << 30
+            assert a < 4 << 30 and b < 1.5 * a + (8192 << 20) / 8 * (not grad)
     assert f(1, 1, 1, _lib.DTYPE_FP16, 0) == 0
     assert f(-1, 1, 1, 0, 0) == 0 and f(1, 0, 1, 0, 0) == 0 and f(1, 1, 0, 0, 0) == 0
 
