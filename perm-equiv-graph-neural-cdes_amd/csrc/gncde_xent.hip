@@ -110,10 +110,14 @@ __global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int 
     const int64_t r = e / cpr;
     const int h0 = (int)(e - r * cpr) * 8;
     u16x8 o[NP];
+    floatx4 v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] = h0 + 4 * i < H ? four<F32>(src, r * H + h0 + 4 * i, r * H + H) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint16_t p[NP];
-      split<NP>(h0 + i < H ? value<F32>(src, r * H + h0 + i) : 0.f, p);
+      split<NP>(v[i >> 2][i & 3], p);
 #pragma unroll
       for (int q = 0; q < NP; ++q) o[q][i] = p[q];
     }
@@ -132,17 +136,19 @@ __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ sr
   const int64_t ht = (H + 63) / 64;
   const int64_t r0 = (blockIdx.x / ht) * 64;
   const int h0 = (int)(blockIdx.x % ht) * 64;
-  const int c = threadIdx.x & 63, q4 = threadIdx.x >> 6;
-  if (LEFT && threadIdx.x < 64) keep[c] = r0 + c < R && row_counts(rows, r0 + c);
-  float v[16];
+  if (LEFT && threadIdx.x < 64) keep[threadIdx.x] = r0 + threadIdx.x < R && row_counts(rows, r0 + threadIdx.x);
+  floatx4 v[4];
+  const int c = (threadIdx.x & 15) * 4, r16 = threadIdx.x >> 4;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = r0 + q4 + 4 * i;
-    v[i] = r < R && h0 + c < H ? value<F32>(src, r * H + h0 + c) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + r16 + 16 * i;
+    v[i] = r < R && h0 + c < H ? four<F32>(src, r * H + h0 + c, r * H + H) : floatx4{0.f, 0.f, 0.f, 0.f};
   }
   if (LEFT) __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t[q4 + 4 * i][c] = !LEFT || keep[q4 + 4 * i] ? v[i] : 0.f;
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[r16 + 16 * i][c + q] = !LEFT || keep[r16 + 16 * i] ? v[i][q] : 0.f;
   __syncthreads();
   const int rc = (threadIdx.x & 7) * 8, hh = threadIdx.x >> 3;
   for (int i = hh; i < 64; i += 32) {
@@ -172,7 +178,7 @@ struct GemmArgs {
   int64_t M, N;              // rows of A and of B
   int K;                     // contraction, a multiple of 8
   int kt;                    // steps over K
-  int per_split;             // steps a workgroup of one split takes
+  int per_split, splits;     // steps a workgroup of one split takes
   int64_t tm, tn;            // tiles
   // logits
   Rows rows;
@@ -232,27 +238,62 @@ __device__ __forceinline__ void interleave() {
   __builtin_amdgcn_sched_group_barrier(0x008, MMS, 0);
 }
 
+// The sum over each run of 16 lanes, in all of them (lane exchanges within the run: pairs, quads, halves, mirror).
+__device__ __forceinline__ float sum16(float x) {
+  x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xb1, 0xf, 0xf, true));
+  x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4e, 0xf, 0xf, true));
+  x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x141, 0xf, 0xf, true));
+  x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x140, 0xf, 0xf, true));
+  return x;
+}
+
+// A value of the lane's own that the compiler takes for new: what follows from it is worked out again for every tile and
+// does not stay in registers over the products.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32>
-__global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1) k_xent_mm(GemmArgs a) {
+__global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_xent_mm(GemmArgs a) {
   typedef Step<NP> S;
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
   static_assert(IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
   constexpr int TILE = (BM + BN) * S::ROW;
   constexpr int PAD = 16;  // values a staged row of dl is longer
-  constexpr int STAGE = EPI != E_DL ? 0 : BN * (BM + PAD) > BM * (BN + PAD) ? BN * (BM + PAD) : BM * (BN + PAD);
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[2 * TILE > STAGE ? 2 * TILE : STAGE];
-  // What the logits' epilogues need of a row of x, fetched while the first step's operands are on their way:
-  // -lse log2 e, g over the scale, the same times S, and the target's class within the piece (-1: none there; kLeftOut).
-  __shared__ __attribute__((aligned(16))) floatx4 info[EPI == E_OUT ? 1 : BN];
+  // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
+  constexpr int HALVES = BM + BN >= 512 ? 2 : 1;
+  constexpr int STAGE_P = BN / HALVES * (BM + PAD), STAGE_PT = BM / HALVES * (BN + PAD);
+  constexpr int STAGE = EPI != E_DL ? 0 : STAGE_P > STAGE_PT ? STAGE_P : STAGE_PT;
+  // (One LDS object: with two, the compiler waits for every load into LDS before any read of it.)
+  constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8, INFO = EPI == E_OUT ? 0 : BN;
+  constexpr int BIAS = EPI == E_OUT ? 0 : BM;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[BUFS + 2 * INFO * 8 + 2 * BIAS * 2];
+  uint16_t* const stage = lds + TILE;
+  // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
+  // class within the piece (-1: none there; kLeftOut).  Fetched with the tile's first operands, one tile ahead.
+  floatx4* const info = reinterpret_cast<floatx4*>(lds + BUFS);
+  float* const bias = reinterpret_cast<float*>(lds + BUFS + 2 * INFO * 8);  // of the tile's classes, likewise
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
+  const uint32_t all = (uint32_t)(a.tm * a.tn) * (uint32_t)a.splits;
 
-  // Tile of this workgroup: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the order: split
-  // by split, and within one in blocks of eight tiles of A by all of B.  What an XCD reads at a time stays in its cache.
-  int tile_m, tile_n, split_k;
-  {
-    const uint32_t nt = (uint32_t)(a.tm * a.tn), tn = (uint32_t)a.tn, all = gridDim.x, bid = blockIdx.x;
+  // The tile in hand, and what its loads need: this lane's chunks of a step as byte offsets from the tile's first row of
+  // A or B (rows behind the last read the last one's values: their results are never written), and buffer descriptors of
+  // the tile's rows; a load behind the last step goes through one of no bytes and reads nothing.
+  int64_t m0, n0;
+  int tile_m, tile_n, split_k, k_from, k_to;
+  uint32_t off[IT];
+  const int col = ((lane & 7) ^ (lane >> 3)) * 8;  // one part: first value of all of them within the step
+  const uint16_t *base_a, *base_b;
+  auto place_of = [&](int i, int lane) {  // this lane's chunk of the buffer
+    return i < IA ? (wave * IA + i) * 64 + lane : BM * S::CH + (wave * (IT - IA) + i - IA) * 64 + lane;
+  };
+  // Tile `bid`: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the order: split by split, and
+  // within one in blocks of eight tiles of A by all of B.  What an XCD reads at a time stays in its cache.
+  auto take = [&](uint32_t bid) {
+    const uint32_t nt = (uint32_t)(a.tm * a.tn), tn = (uint32_t)a.tn;
     const uint32_t q = all >> 3, r = all & 7, xcd = bid & 7;
     uint32_t lin = xcd * q + (xcd < r ? xcd : r) + (bid >> 3);
     const uint32_t sp = lin / nt;
@@ -262,29 +303,21 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
     tile_m = __builtin_amdgcn_readfirstlane((int)(grp * 8 + in % gm));
     tile_n = __builtin_amdgcn_readfirstlane((int)(in / gm));
     split_k = __builtin_amdgcn_readfirstlane((int)sp);
-  }
-  const int64_t m0 = (int64_t)tile_m * BM, n0 = (int64_t)tile_n * BN;
-
-  // This lane's chunks of a step, as byte offsets from the tile's first row of A or B (rows behind the last read the
-  // last one's values: their results are never written).
-  uint32_t off[IT];
-  const int col = ((lane & 7) ^ (lane >> 3)) * 8;  // one part: first value of all of them within the step
-  auto place_of = [&](int i) {  // this lane's chunk of the buffer
-    return i < IA ? (wave * IA + i) * 64 + lane : BM * S::CH + (wave * (IT - IA) + i - IA) * 64 + lane;
-  };
+    m0 = (int64_t)tile_m * BM, n0 = (int64_t)tile_n * BN;
+    const int lane = fresh(threadIdx.x) & 63;
+    const int most_a = (int)(a.M - m0 < BM ? a.M - m0 : BM) - 1, most_b = (int)(a.N - n0 < BN ? a.N - n0 : BN) - 1;
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int slot = place_of(i), row = slot / S::CH;
-    const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
-    const int64_t r = i < IA ? row : row - BM;
-    const int64_t most = i < IA ? a.M - 1 - m0 : a.N - 1 - n0;
-    off[i] = (uint32_t)((r < most ? r : most) * (i < IA ? a.lda : a.ldb) + c * 8) * 2u;
-  }
-  const int k_from = split_k * a.per_split;
-  const int k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
-  // Buffer descriptors of the tile's rows; a load behind the last step goes through one of no bytes and reads nothing.
-  const uint16_t* base_a = a.A + m0 * a.lda;
-  const uint16_t* base_b = a.B + n0 * a.ldb;
+    for (int i = 0; i < IT; ++i) {
+      const int slot = place_of(i, lane), row = slot / S::CH;
+      const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
+      const int rr = i < IA ? row : row - BM, most = i < IA ? most_a : most_b;
+      off[i] = ((uint32_t)(rr < most ? rr : most) * (uint32_t)(i < IA ? a.lda : a.ldb) + c * 8) * 2u;
+    }
+    k_from = split_k * a.per_split;
+    k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
+    base_a = a.A + m0 * a.lda;
+    base_b = a.B + n0 * a.ldb;
+  };
 
   auto load = [&](int k, int buf) {
     const int bytes = __builtin_amdgcn_readfirstlane((k - k_to) >> 31);  // all of 2^32, or none
@@ -298,8 +331,32 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
       uint32_t o = off[i];
       if (NP == 1) o -= behind;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          i < IA ? ra : rb, (__attribute__((address_space(3))) void*)(lds + buf * TILE + (place_of(i) - lane) * 8), 16, o,
+          i < IA ? ra : rb, (__attribute__((address_space(3))) void*)(lds + buf * TILE + place_of(i, 0) * 8), 16, o,
           at, 0, 0);
+    }
+  };
+  // The rows of x that the tile in hand has, into info[at].
+  auto fetch_rows = [&](int at) {
+    if constexpr (EPI != E_OUT) {
+      if (a.bias)
+        for (int r = fresh(threadIdx.x); r < BM; r += NW * 64)
+          bias[at * BIAS + r] = m0 + r < a.M ? value<F32>(a.bias, m0 + r) : 0.f;
+      for (int r = fresh(threadIdx.x); r < BN; r += NW * 64) {
+        const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1;
+        const bool kept = !a.rows.mask || a.rows.mask[n] != 0;
+        const int64_t c = a.rows.kind == GNCDE_TARGET_ROWS ? 0 : row_index(a.rows, n);
+        floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (EPI == E_DL) {
+          const float lse = a.stats[2 * n], mass = a.stats[2 * n + 1];
+          const float gv = a.g[n] / (a.scale ? *a.scale : 1.f);
+          v = floatx4{-lse * kLog2e, gv, gv * mass, 0.f};
+        }
+        const bool in = n0 + r < a.N && kept && c >= 0;
+        const int64_t t = c - a.v0;
+        if (!in) v = floatx4{0.f, 0.f, 0.f, 0.f};
+        v[3] = __int_as_float(!in ? kLeftOut : a.rows.kind != GNCDE_TARGET_ROWS && t >= 0 && t < a.M ? (int)t : -1);
+        info[at * INFO + r] = v;
+      }
     }
   };
   // The buffer of step k is complete for every wave, and everybody has read the other one.
@@ -309,7 +366,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
       if (k * S::K + col >= a.K)
 #pragma unroll
         for (int i = 0; i < IT; ++i)
-          *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i) * 8) = u16x8{};
+          *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i, lane) * 8) = u16x8{};
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     }
     asm volatile("" ::: "memory");
@@ -318,10 +375,6 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   };
 
   floatx4 acc[RT][CT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int fr = lane & 15, fk = lane >> 4;
   const uint16_t* la = lds + (wm * (BM / WM) + fr) * S::ROW;
@@ -342,68 +395,10 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
   };
 
-  if (EPI != E_OUT && k_from < k_to) load(k_from, 0);
-  if constexpr (EPI != E_OUT) {
-    for (int r = threadIdx.x; r < BN; r += NW * 64) {
-      const int64_t n = n0 + r;
-      const bool in = n < a.N && row_counts(a.rows, n);
-      floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
-      int t = in ? -1 : kLeftOut;
-      if (in && a.rows.kind != GNCDE_TARGET_ROWS) {
-        const int64_t c = row_index(a.rows, n) - a.v0;
-        if (c >= 0 && c < a.M) t = (int)c;
-      }
-      if (EPI == E_DL && in) {
-        const float gv = a.g[n] / (a.scale ? *a.scale : 1.f);
-        v = floatx4{-a.stats[2 * n] * kLog2e, gv, gv * a.stats[2 * n + 1], 0.f};
-      }
-      v[3] = __int_as_float(t);
-      info[r] = v;
-    }
-  }
-  if (k_from < k_to) {
-    if (EPI == E_OUT) load(k_from, 0);
-    hand_over(k_from, 0);
-    load(k_from + 1, 1);
-    if constexpr (NP == 1) {
-      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
-      read(0, 0, fa0, fb0);
-      for (int k = k_from; k < k_to; ++k) {
-        const int buf = (k - k_from) & 1;
-        read(1, buf, fa1, fb1);
-        multiply(fa0, fb0);
-        interleave<RT * CT, RT + CT, 0>();
-        hand_over(k + 1, buf ^ 1);
-        read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
-        load(k + 2, buf);
-        multiply(fa1, fb1);
-        interleave<RT * CT, RT + CT, IT>();
-      }
-    } else {
-      bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
-      read(1, 0, ma, mb);
-      for (int k = k_from; k < k_to; ++k) {
-        const int buf = (k - k_from) & 1;
-        read(0, buf, ha, hb);
-        multiply(ma, mb);
-        interleave<RT * CT, RT + CT, 0>();
-        read(2, buf, sa, sb);
-        multiply(ma, hb);
-        multiply(ha, mb);
-        interleave<2 * RT * CT, RT + CT, 0>();
-        hand_over(k + 1, buf ^ 1);
-        read(1, buf ^ 1, ma, mb);
-        load(k + 2, buf);
-        multiply(sa, hb);
-        multiply(ha, sb);
-        multiply(ha, hb);
-        interleave<3 * RT * CT, RT + CT, IT>();
-      }
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  __syncthreads();
-
+  // Puts out the products of tile (m0, n0); info[at] has its rows.
+  auto put_out = [&](const int64_t m0, const int64_t n0, const int tile_m, const int tile_n, const int split_k,
+                     const int at) {
+  const int tid = fresh(threadIdx.x), lane = tid & 63, fr = lane & 15, fk = lane >> 4;
   const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
   const int64_t nb = n0 + wn * (BN / WN) + fr;
 
@@ -451,8 +446,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   if (a.bias) {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const int64_t m = mb + i * 16;
-      const floatx4 bv = m < a.M ? four<F32>(a.bias, m, a.M) : floatx4{0.f, 0.f, 0.f, 0.f};
+      const floatx4 bv = *reinterpret_cast<const floatx4*>(bias + at * BIAS + wm * (BM / WM) + fk * 4 + i * 16);
 #pragma unroll
       for (int j = 0; j < CT; ++j) acc[i][j] += bv;
     }
@@ -470,28 +464,39 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
   }
 
   if constexpr (EPI == E_LSE) {
-    float* sm = reinterpret_cast<float*>(lds);  // [4][WM][BN]
+    float* sm = reinterpret_cast<float*>(stage);  // [4][WM][BN]
+    float top[CT], sum[CT], dot[CT], mass[CT];
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
-      const int64_t n = nb + j * 16;
-      const int target = __float_as_int(info[wn * (BN / WN) + j * 16 + fr][3]);
-      const bool in = target != kLeftOut;
-      float top = -INFINITY;
+      top[j] = -INFINITY, sum[j] = dot[j] = mass[j] = 0.f;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) top = fmaxf(top, acc[i][j][q]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float off2 = -ref * kLog2e;
-      float sum = 0.f, dot = 0.f, mass = 0.f;
+        for (int q = 0; q < 4; ++q) top[j] = fmaxf(top[j], acc[i][j][q]);
+    }
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+      float other[CT];
+#pragma unroll
+      for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(top[j], d);
+#pragma unroll
+      for (int j = 0; j < CT; ++j) top[j] = fmaxf(top[j], other[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const float off2 = top[j] == -INFINITY ? 0.f : -top[j] * kLog2e;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
-      if (a.rows.kind == GNCDE_TARGET_ROWS) {
-        if (in) {
+        for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+      sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    if (a.rows.kind == GNCDE_TARGET_ROWS) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int64_t n = nb + j * 16;
+        if (__float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut) {
           const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
 #pragma unroll
           for (int i = 0; i < RT; ++i) {
@@ -499,37 +504,52 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
             const floatx4 yv = m < a.M ? four<true>(y, m, a.M) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              mass += yv[q];
-              dot += yv[q] == 0.f ? 0.f : yv[q] * acc[i][j][q];  // a class at -inf without mass adds nothing
+              mass[j] += yv[q];
+              dot[j] += yv[q] == 0.f ? 0.f : yv[q] * acc[i][j][q];  // a class at -inf without mass adds nothing
             }
           }
         }
-        dot += __shfl_xor(dot, 16);
-        dot += __shfl_xor(dot, 32);
-        mass += __shfl_xor(mass, 16);
-        mass += __shfl_xor(mass, 32);
-      } else {
-        const int t = target - (int)mb;
+      }
+#pragma unroll
+      for (int d = 16; d < 64; d <<= 1)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          dot[j] += __shfl_xor(dot[j], d);
+          mass[j] += __shfl_xor(mass[j], d);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int target = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
         if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              if (target >= 0 && t == i * 16 + q) a.hit[n] = acc[i][j][q];
+              if (target >= 0 && t == i * 16 + q) a.hit[nb + j * 16] = acc[i][j][q];
         }
       }
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if (fk == 0) {
-        const int col = wn * (BN / WN) + j * 16 + fr;
-        sm[wm * BN + col] = top;
-        sm[(WM + wm) * BN + col] = sum;
-        sm[(2 * WM + wm) * BN + col] = dot;
-        sm[(3 * WM + wm) * BN + col] = mass;
+    }
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+      float other[CT];
+#pragma unroll
+      for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(sum[j], d);
+#pragma unroll
+      for (int j = 0; j < CT; ++j) sum[j] += other[j];
+    }
+    if (fk == 0) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int c = wn * (BN / WN) + j * 16 + fr;
+        sm[wm * BN + c] = top[j];
+        sm[(WM + wm) * BN + c] = sum[j];
+        sm[(2 * WM + wm) * BN + c] = dot[j];
+        sm[(3 * WM + wm) * BN + c] = mass[j];
       }
     }
     __syncthreads();
-    for (int col = threadIdx.x; col < BN; col += NW * 64) {
+    for (int col = tid; col < BN; col += NW * 64) {
       if (n0 + col >= a.N) break;
       float top = sm[col];
 #pragma unroll
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
       const int64_t n = nb + j * 16;
-      const floatx4 row = info[wn * (BN / WN) + j * 16 + fr];
+      const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
       const int target = __float_as_int(row[3]);
       const bool in = target != kLeftOut;
       const float off2 = row[0], gv = row[1], gs = row[2];
@@ -605,11 +625,7 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
         for (int j = 1; j < CT; ++j) s += acc[i][j];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float r = s[q];
-          r += __shfl_xor(r, 1);
-          r += __shfl_xor(r, 2);
-          r += __shfl_xor(r, 4);
-          r += __shfl_xor(r, 8);
+          const float r = sum16(s[q]);
           const int64_t m = mb + i * 16 + q;
           if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = r;
         }
@@ -617,47 +633,122 @@ __global__ void __launch_bounds__(WM* WN * 64, BM * BN * NP > 256 * 128 ? 2 : 1)
     }
     // dl goes out through LDS, once as rows of classes and once as classes of rows, in whole 16-byte chunks: written
     // from the registers, its 8 and 2 byte pieces cost 31 us a 256 x 256 tile where the staged ones cost 12.
-    constexpr int THREADS = NW * 64;
+    constexpr int THREADS = NW * 64, HN = BN / HALVES, HM = BM / HALVES;
     const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
 #pragma unroll
-      for (int j = 0; j < CT; ++j)
+      for (int half = 0; half < HALVES; ++half) {
+        if (s + half > 0) __syncthreads();
+        if (wn * (BN / WN) / HN == half) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          const floatx4 v = acc[i][j];
-          *reinterpret_cast<u16x4*>(lds + (ln + j * 16) * (BM + PAD) + lm + i * 16) =
-              u16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+          for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              const floatx4 v = acc[i][j];
+              *reinterpret_cast<u16x4*>(stage + (ln - half * HN + j * 16) * (BM + PAD) + lm + i * 16) =
+                  u16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+            }
         }
-      __syncthreads();
+        __syncthreads();
 #pragma unroll 2
-      for (int e = threadIdx.x; e < BN * (BM / 8); e += THREADS) {
-        const int row = e / (BM / 8), c = e % (BM / 8) * 8;
-        if (n0 + row < a.N && m0 + c < a.mp)
-          *reinterpret_cast<u16x8*>(a.P + (n0 + row) * NP * a.ldp + packed<NP>(m0 + c, s)) =
-              *reinterpret_cast<const u16x8*>(lds + row * (BM + PAD) + c);
+        for (int e = tid; e < HN * (BM / 8); e += THREADS) {
+          const int row = e / (BM / 8), c = e % (BM / 8) * 8;
+          const int64_t n = n0 + half * HN + row;
+          if (n < a.N && m0 + c < a.mp)
+            *reinterpret_cast<u16x8*>(a.P + n * NP * a.ldp + packed<NP>(m0 + c, s)) =
+                *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
+        }
       }
-      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < CT; ++j)
+      for (int half = 0; half < HALVES; ++half) {
+        __syncthreads();
+        if (wm * (BM / WM) / HM == half) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+          for (int j = 0; j < CT; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint16_t part = to_bf16(acc[i][j][q]);
-            lds[(lm + i * 16 + q) * (BN + PAD) + ln + j * 16] = part;
-            if (NP > 1) acc[i][j][q] -= from_bf16(part);  // what the next part holds
-          }
-      __syncthreads();
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint16_t part = to_bf16(acc[i][j][q]);
+                stage[(lm - half * HM + i * 16 + q) * (BN + PAD) + ln + j * 16] = part;
+                if (NP > 1) acc[i][j][q] -= from_bf16(part);  // what the next part holds
+              }
+        }
+        __syncthreads();
 #pragma unroll 2
-      for (int e = threadIdx.x; e < BM * (BN / 8); e += THREADS) {
-        const int row = e / (BN / 8), c = e % (BN / 8) * 8;
-        if (m0 + row < a.M && n0 + c < a.np)
-          *reinterpret_cast<u16x8*>(a.Pt + (m0 + row) * NP * a.ldpt + packed<NP>(n0 + c, s)) =
-              *reinterpret_cast<const u16x8*>(lds + row * (BN + PAD) + c);
+        for (int e = tid; e < HM * (BN / 8); e += THREADS) {
+          const int row = e / (BN / 8), c = e % (BN / 8) * 8;
+          const int64_t m = m0 + half * HM + row;
+          if (m < a.M && n0 + c < a.np)
+            *reinterpret_cast<u16x8*>(a.Pt + m * NP * a.ldpt + packed<NP>(n0 + c, s)) =
+                *reinterpret_cast<const u16x8*>(stage + row * (BN + PAD) + c);
+        }
       }
-      if (s + 1 < NP) __syncthreads();
     }
+  }
+  };
+
+  take(blockIdx.x);
+  if (k_from < k_to) load(k_from, 0);
+  fetch_rows(0);
+  int at = 0;
+  for (uint32_t bid = blockIdx.x; bid < all; bid += gridDim.x, at ^= 1) {
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (k_from < k_to) {
+    hand_over(k_from, 0);
+    load(k_from + 1, 1);
+    if constexpr (NP == 1) {
+      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
+      read(0, 0, fa0, fb0);
+      for (int k = k_from; k < k_to; ++k) {
+        const int buf = (k - k_from) & 1;
+        read(1, buf, fa1, fb1);
+        multiply(fa0, fb0);
+        interleave<RT * CT, RT + CT, 0>();
+        hand_over(k + 1, buf ^ 1);
+        read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
+        load(k + 2, buf);
+        multiply(fa1, fb1);
+        interleave<RT * CT, RT + CT, IT>();
+      }
+    } else {
+      bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
+      read(1, 0, ma, mb);
+      for (int k = k_from; k < k_to; ++k) {
+        const int buf = (k - k_from) & 1;
+        read(0, buf, ha, hb);
+        multiply(ma, mb);
+        interleave<RT * CT, RT + CT, 0>();
+        read(2, buf, sa, sb);
+        multiply(ma, hb);
+        multiply(ha, mb);
+        interleave<2 * RT * CT, RT + CT, 0>();
+        hand_over(k + 1, buf ^ 1);
+        read(1, buf ^ 1, ma, mb);
+        load(k + 2, buf);
+        multiply(sa, hb);
+        multiply(ha, sb);
+        multiply(ha, hb);
+        interleave<3 * RT * CT, RT + CT, IT>();
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __syncthreads();
+
+  // The next tile's first operands and rows are on their way while this one's products are put out.
+  const int64_t m0_now = m0, n0_now = n0;
+  const int tm_now = tile_m, tn_now = tile_n, split_now = split_k;
+  if (bid + gridDim.x < all) {
+    take(bid + gridDim.x);
+    if (k_from < k_to) load(k_from, 0);
+    fetch_rows(at ^ 1);
+  }
+  put_out(m0_now, n0_now, tm_now, tn_now, split_now, at);
   }
 }
 
@@ -1520,8 +1611,10 @@ void mm(const GemmArgs& in, const Cfg& cfg, hipStream_t st) {
   const Tile t = tile_of(cfg.big, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
   a.kt = (int)steps_of(a.K, NP);
+  a.splits = cfg.splits;
   a.per_split = (int)div_up(a.kt, cfg.splits);
-  const dim3 grid((unsigned)(a.tm * a.tn * cfg.splits));
+  // a workgroup for every place the chip has (LDS: one large or two small ones a CU), each with its share of the tiles
+  const dim3 grid((unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus));
   if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
   else if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
   else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
