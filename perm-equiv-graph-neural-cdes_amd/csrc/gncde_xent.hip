@@ -126,16 +126,55 @@ __global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int 
   }
 }
 
+// The scale of dl: the largest |g| of the rows that count (1 where that is no use).  bf16 dl is stored over it, so that
+// the equal cotangents of a mean leave the target's entry, nearly all of dl, near -1 and not at a rounded -g: the
+// gradients' error is then that of their own rounding (2e-3 instead of 3e-3 of the norm at 8192 rows).  256 threads.
+__device__ __forceinline__ void largest_cotangent(int64_t N, const Rows& rows, const float* __restrict__ g,
+                                                  float* __restrict__ scale) {
+  __shared__ float red[4];
+  float m = 0.f;
+  for (int64_t n0 = threadIdx.x; n0 < N; n0 += 2048) {
+    float v[8];
+    bool in[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // side by side: one wait for all
+      const int64_t n = n0 + 256 * i < N ? n0 + 256 * i : n0;
+      v[i] = fabsf(g[n]);
+      in[i] = !rows.mask || rows.mask[n] != 0;
+      if (rows.kind != GNCDE_TARGET_ROWS) in[i] &= row_index(rows, n) >= 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, in[i] ? v[i] : 0.f);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (threadIdx.x == 0) *scale = m > 1e-30f && m < 1e30f ? m : 1.f;
+}
+
+__global__ void __launch_bounds__(256) k_xent_scale(int64_t N, Rows rows, const float* __restrict__ g,
+                                                    float* __restrict__ scale) {
+  largest_cotangent(N, rows, g, scale);
+}
+
 // src [R, H] -> transposed, packed rows of stride Rp, zeros behind R up to kPad and (LEFT) in rows left out, whatever
-// they hold.
+// they hold.  With `scale`, the first workgroup finds that instead (a launch less).
 template <bool F32, int NP, bool LEFT>
 __global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
-                                                     Rows rows, uint16_t* __restrict__ dst) {
+                                                     Rows rows, uint16_t* __restrict__ dst,
+                                                     const float* __restrict__ g, float* __restrict__ scale) {
+  if (scale && blockIdx.x == 0) {
+    largest_cotangent(R, rows, g, scale);
+    return;
+  }
+  const int64_t block = (int64_t)blockIdx.x - (scale ? 1 : 0);
   __shared__ float t[64][65];
   __shared__ bool keep[64];
   const int64_t ht = (H + 63) / 64;
-  const int64_t r0 = (blockIdx.x / ht) * 64;
-  const int h0 = (int)(blockIdx.x % ht) * 64;
+  const int64_t r0 = (block / ht) * 64;
+  const int h0 = (int)(block % ht) * 64;
   if (LEFT && threadIdx.x < 64) keep[threadIdx.x] = r0 + threadIdx.x < R && row_counts(rows, r0 + threadIdx.x);
   floatx4 v[4];
   const int c = (threadIdx.x & 15) * 4, r16 = threadIdx.x >> 4;
@@ -752,36 +791,6 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   }
 }
 
-// The scale of dl: the largest |g| of the rows that count (1 where that is no use).  bf16 dl is stored over it, so that
-// the equal cotangents of a mean leave the target's entry, nearly all of dl, near -1 and not at a rounded -g: the
-// gradients' error is then that of their own rounding (2e-3 instead of 3e-3 of the norm at 8192 rows).
-__global__ void __launch_bounds__(1024) k_xent_scale(int64_t N, Rows rows, const float* __restrict__ g,
-                                                     float* __restrict__ scale) {
-  __shared__ float red[16];
-  float m = 0.f;
-  for (int64_t n0 = threadIdx.x; n0 < N; n0 += 8192) {
-    float v[8];
-    bool in[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {  // side by side: one wait for all
-      const int64_t n = n0 + 1024 * i < N ? n0 + 1024 * i : n0;
-      v[i] = fabsf(g[n]);
-      in[i] = !rows.mask || rows.mask[n] != 0;
-      if (rows.kind != GNCDE_TARGET_ROWS) in[i] &= row_index(rows, n) >= 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, in[i] ? v[i] : 0.f);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-#pragma unroll
-  for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
-  *scale = m > 1e-30f && m < 1e30f ? m : 1.f;
-}
-
 // A pair (largest, sum of exponentials relative to it) joined with another.
 __device__ __forceinline__ void join_pair(float& top, float& sum, float top2, float sum2) {
   const float nt = fmaxf(top, top2), ref = nt == -INFINITY ? 0.f : nt;
@@ -1097,8 +1106,15 @@ __global__ void __launch_bounds__(1024) k_xent_parts_sum(int parts, int VH, int 
   const int e = blockIdx.x * 64 + c, len = VH + V;
   const int per = (parts + 15) / 16, to = per * (q + 1) < parts ? per * (q + 1) : parts;
   float s = 0.f;
-  if (e < len)
-    for (int i = per * q; i < to; ++i) s += part[(int64_t)i * len + e];
+  if (e < len) {
+    for (int i = per * q; i < to; i += 8) {  // eight loads side by side
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i + u < to ? part[(int64_t)(i + u) * len + e] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+  }
   run[q][c] = s;
   __syncthreads();
   if (q != 0 || e >= len) return;
@@ -1629,9 +1645,11 @@ void pack(const void* src, int64_t R, const Plan& p, uint16_t* dst, hipStream_t 
 }
 
 template <bool F32, bool LEFT>
-void pack_t(const void* src, int64_t R, int64_t stride, const Plan& p, Rows rows, uint16_t* dst, hipStream_t st) {
-  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)(div_up(R, 64) * div_up(p.H, 64))),
-                     dim3(256), 0, st, src, R, (int)p.H, stride, rows, dst);
+void pack_t(const void* src, int64_t R, int64_t stride, const Plan& p, Rows rows, uint16_t* dst, const float* g,
+            float* scale, hipStream_t st) {
+  const int64_t blocks = div_up(R, 64) * div_up(p.H, 64) + (scale ? 1 : 0);
+  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)blocks), dim3(256), 0, st, src, R, (int)p.H,
+                     stride, rows, dst, g, scale);
 }
 
 bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -1790,12 +1808,9 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
   float* acc_x = reinterpret_cast<float*>(c.ws + p.o_gx);
   float* acc_w = reinterpret_cast<float*>(c.ws + p.o_gw);
   float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
-  if (gW) pack_t<F32, true>(c.x, p.N, p.Ns, p, c.rows, xt, c.st);
-  float* scale = nullptr;
-  if (!F32) {
-    scale = reinterpret_cast<float*>(c.ws + p.o_scale);
-    hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(1024), 0, c.st, p.N, c.rows, g, scale);
-  }
+  float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);  // three parts lose nothing to it
+  if (gW) pack_t<F32, true>(c.x, p.N, p.Ns, p, c.rows, xt, g, scale, c.st);
+  else if (scale) hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(256), 0, c.st, p.N, c.rows, g, scale);
   const bool one = p.piece >= p.V;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad), vs = stride_of(vc);
@@ -1820,7 +1835,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       if (at != 0) break;
     }
     if (gx) {
-      pack_t<F32, false>(wsrc, vc, vs, p, c.rows, wt, c.st);
+      pack_t<F32, false>(wsrc, vc, vs, p, c.rows, wt, nullptr, nullptr, c.st);
       GemmArgs q = {};
       q.scale = scale;
       q.A = wt, q.lda = p.np * vs, q.M = p.H;

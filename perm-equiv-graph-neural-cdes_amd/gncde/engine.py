@@ -10,7 +10,6 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
-import operator
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -397,7 +396,29 @@ def clip_adamw(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: to
     return stats
 
 
+_fast = None
+
+
+def _calls():
+    """The compiled plain-case calls (csrc/gncde_calls.cpp), bound to the loaded library: each returns None for a call
+    that is not plain, which the code behind it here then takes."""
+    global _fast
+    if _fast is None:
+        lib = _lib.load()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise _lib.GncdeError(f"gncde/_calls.so: {e}: build it with `make -C perm-equiv-graph-neural-cdes_amd`") from e
+        module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            lib.gncde_linear_cross_entropy_workspace_bytes, lib.gncde_linear_cross_entropy,
+            lib.gncde_linear_cross_entropy_grad, lib.gncde_global_norm_workspace_bytes, lib.gncde_global_norm,
+            lib.gncde_clip_by_global_norm)), torch._C._cuda_getCurrentRawStream, _lib.check, torch.OutOfMemoryError)
+        _fast = module
+    return _fast
+
+
 _READOUT_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16}
+_TARGET_KINDS = {torch.int32: _lib.TARGET_INDEX32, torch.int64: _lib.TARGET_INDEX64, torch.float32: _lib.TARGET_ROWS}
 
 
 def _readout_args(name: str, x, W, b, target, mask):
@@ -406,28 +427,28 @@ def _readout_args(name: str, x, W, b, target, mask):
     if kind is None or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
         raise _lib.GncdeError(f"{name}: x, W and b must all be fp32 or all be bf16 (got {x.dtype}, {W.dtype}"
                               f"{'' if b is None else f', {b.dtype}'})")
-    if x.dim() < 1 or W.dim() != 2 or x.shape[-1] != W.shape[1] or W.numel() == 0:
-        raise _lib.GncdeError(f"{name}: x {tuple(x.shape)} [..., hidden] does not fit W {tuple(W.shape)} "
-                              "[classes, hidden]")
-    hidden, classes = int(W.shape[1]), int(W.shape[0])
+    xs, ws = x.shape, W.shape
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1] or ws[0] == 0 or ws[1] == 0:
+        raise _lib.GncdeError(f"{name}: x {tuple(xs)} [..., hidden] does not fit W {tuple(ws)} [classes, hidden]")
+    classes, hidden = ws
+    lead = xs[:-1]
     rows = x.numel() // hidden
-    lead = tuple(x.shape[:-1])
-    if b is not None and tuple(b.shape) != (classes,):
+    if b is not None and b.shape != ws[:1]:
         raise _lib.GncdeError(f"{name}: b {tuple(b.shape)} must be [{classes}]")
-    if target.dtype in (torch.int32, torch.int64):
-        tkind = _lib.TARGET_INDEX32 if target.dtype == torch.int32 else _lib.TARGET_INDEX64
-        if tuple(target.shape) != lead:
-            raise _lib.GncdeError(f"{name}: class indices {tuple(target.shape)} must be {lead}")
-    elif target.dtype == torch.float32:
-        tkind = _lib.TARGET_ROWS
-        if tuple(target.shape) != lead + (classes,):
-            raise _lib.GncdeError(f"{name}: label rows {tuple(target.shape)} must be {lead + (classes,)}")
-    else:
+    tkind = _TARGET_KINDS.get(target.dtype)
+    if tkind is None:
         raise _lib.GncdeError(f"{name}: target must be int32 / int64 class indices or fp32 label rows, got "
                               f"{target.dtype}")
-    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != lead):
-        raise _lib.GncdeError(f"{name}: mask must be bool {lead}, got {mask.dtype} {tuple(mask.shape)}")
-    _one_device(name, [t for t in (x, W, b, target, mask) if t is not None])
+    want = lead + ws[:1] if tkind == _lib.TARGET_ROWS else lead
+    if target.shape != want:
+        raise _lib.GncdeError(f"{name}: {'label rows' if tkind == _lib.TARGET_ROWS else 'class indices'} "
+                              f"{tuple(target.shape)} must be {tuple(want)}")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != lead):
+        raise _lib.GncdeError(f"{name}: mask must be bool {tuple(lead)}, got {mask.dtype} {tuple(mask.shape)}")
+    dev = x.get_device()
+    if dev < 0 or W.get_device() != dev or target.get_device() != dev or (b is not None and b.get_device() != dev) or (
+            mask is not None and mask.get_device() != dev):
+        raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
     return (rows, hidden, classes, kind, x.contiguous(), W.contiguous(), None if b is None else b.contiguous(), tkind,
             target.contiguous(), None if mask is None else mask.contiguous())
 
@@ -442,6 +463,9 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | Non
     [..., classes] fp32, of any mass.  mask [...] bool: False leaves the row out; its loss is 0 and its values change
     nothing.  ``stats`` holds each row's (log of the summed exponentials, label mass) for
     ``linear_cross_entropy_grad``."""
+    done = _calls().readout_loss(x, W, b, target, mask)
+    if done is not None:
+        return done
     rows, hidden, classes, kind, x, W, b, tkind, target, mask = _readout_args("linear_cross_entropy", x, W, b, target,
                                                                               mask)
     lib = _lib.load()
@@ -463,6 +487,9 @@ def linear_cross_entropy_grad(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor 
                               need_w=True, need_b=True):
     """Reverse mode of ``linear_cross_entropy`` for the rows' cotangents g [...] fp32: (gx, gW, gb) in x's type (None
     where not needed; gb None without b)."""
+    done = _calls().readout_grad(x, W, b, target, mask, stats, g, need_x, need_w, need_b)
+    if done is not None:
+        return done
     args = _readout_args("linear_cross_entropy_grad", x, W, b, target, mask)
     rows, hidden, classes, kind, x, W, b, tkind, target, mask = args
     lead = tuple(x.shape[:-1])
@@ -490,9 +517,6 @@ def linear_cross_entropy_grad(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor 
 _LIST_DTYPES = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
 
-# a list of hundreds of tensors is looked over faster than the GPU reads it only without a Python frame a tensor
-_DTYPE, _NUMEL, _DATA_PTR = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.data_ptr
-_DEVICE, _CONTIGUOUS = torch.Tensor.get_device, torch.Tensor.is_contiguous
 _LIST_SIZES = np.array([4, 2, 2], dtype=np.int64)  # bytes a value, by GNCDE_DTYPE_*
 
 
@@ -502,36 +526,34 @@ def _tensor_table(name: str, tensors, out=None):
         raise _lib.GncdeError(f"{name}: a list of tensors is wanted, not one tensor")
     if len(tensors) == 0:
         raise _lib.GncdeError(f"{name}: an empty list of tensors")
-    dtypes = list(map(_DTYPE, tensors))
-    kinds = list(map(_LIST_DTYPES.get, dtypes))
+    kinds = [_LIST_DTYPES.get(t.dtype) for t in tensors]
     if None in kinds:
         raise _lib.GncdeError(f"{name}: tensors must be fp32, bf16 or fp16, got {tensors[kinds.index(None)].dtype}")
     index = _one_device(name, tensors)
-    if not all(map(_CONTIGUOUS, tensors)):
+    if not all(t.is_contiguous() for t in tensors):
         if out is tensors:
             raise _lib.GncdeError(f"{name}: tensors clipped in place must be contiguous")
         tensors = [t.contiguous() for t in tensors]
     rows = np.zeros((len(tensors), 4), dtype=np.int64)  # GncdeTensor: in, out, numel, dtype (+ reserved 0)
-    numels = list(map(_NUMEL, tensors))
-    rows[:, 0] = list(map(_DATA_PTR, tensors))
-    rows[:, 2] = numels
+    rows[:, 0] = [t.data_ptr() for t in tensors]
+    rows[:, 2] = [t.numel() for t in tensors]
     rows[:, 3] = kinds
     if out is tensors:
         rows[:, 1] = rows[:, 0]
     elif out is not None:
         if len(out) != len(tensors):
             raise _lib.GncdeError(f"{name}: {len(out)} outputs for {len(tensors)} tensors")
-        if (list(map(_DTYPE, out)) != dtypes or list(map(_NUMEL, out)) != numels or _one_device(name, out) != index
-                or not all(map(_CONTIGUOUS, out))):
+        if _one_device(name, out) != index or any(
+                o.dtype != t.dtype or o.numel() != t.numel() or not o.is_contiguous() for o, t in zip(out, tensors)):
             raise _lib.GncdeError(f"{name}: an output must be contiguous, of its tensor's type, size and device")
-        rows[:, 1] = list(map(_DATA_PTR, out))
+        rows[:, 1] = [o.data_ptr() for o in out]
     if out is not None:
         _refuse_overlap(name, rows, _LIST_SIZES[rows[:, 3]])
     return rows, tensors, torch.device("cuda", index)
 
 
 def _one_device(name: str, tensors) -> int:
-    index = set(map(_DEVICE, tensors))
+    index = {t.get_device() for t in tensors}
     if len(index) != 1 or -1 in index:
         raise _lib.GncdeError(f"{name}: every tensor must be on one CUDA device")
     return index.pop()
@@ -559,7 +581,11 @@ def global_norm(tensors) -> torch.Tensor:
     """Device stats [2] = (global L2 norm, largest magnitude) over a list of fp32 / bf16 / fp16 CUDA tensors of any
     sizes, on the tensors' device and torch's current stream there (squares and sums in 64 bits; NaN anywhere makes
     both NaN)."""
-    rows, kept, dev = _tensor_table("global_norm", tensors if torch.is_tensor(tensors) else list(tensors))
+    tensors = tensors if torch.is_tensor(tensors) else list(tensors)
+    stats = _calls().tensor_list(tensors, None, 0.0)
+    if stats is not None:
+        return stats
+    rows, kept, dev = _tensor_table("global_norm", tensors)
     lib = _lib.load()
     with _on(dev):
         stats = torch.empty(2, dtype=torch.float32, device=dev)
@@ -583,6 +609,9 @@ def clip_by_global_norm(tensors, max_norm: float, out=None):
     elif not torch.is_tensor(tensors):
         tensors = list(tensors)
         out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors] if out is None else list(out)
+    stats = _calls().tensor_list(tensors, out, max_norm)
+    if stats is not None:
+        return out, stats
     rows, kept, dev = _tensor_table("clip_by_global_norm", tensors, out)
     lib = _lib.load()
     with _on(dev):

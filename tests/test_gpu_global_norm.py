@@ -131,6 +131,31 @@ def test_the_same_tensor_twice():
         engine.clip_by_global_norm(t + t, 1.0, out=t + t)
 
 
+def test_compiled_and_python_calls_agree(monkeypatch):
+    class NotPlain:
+        tensor_list = staticmethod(lambda *a: None)
+
+    ts = tensors((700, 1, 90001), (torch.float32, torch.bfloat16, torch.float16))
+    want = [engine.global_norm(ts)] + list(engine.clip_by_global_norm(ts, 0.7))
+    monkeypatch.setattr(engine, "_fast", NotPlain)
+    got = [engine.global_norm(ts)] + list(engine.clip_by_global_norm(ts, 0.7))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[2], got[2])
+    assert all(torch.equal(a, b) for a, b in zip(want[1], got[1]))
+    place = [t.clone() for t in ts]
+    out, _ = engine.clip_by_global_norm(place, 0.7, out=place)
+    assert out is not None and all(torch.equal(a, b) for a, b in zip(place, want[1]))
+    with pytest.raises(_lib.GncdeError, match="share"):
+        engine.clip_by_global_norm(ts + ts, 1.0, out=ts + ts)
+
+
+def test_tuples_and_generators():
+    ts = tensors((100, 200))
+    want = engine.global_norm(ts)
+    assert torch.equal(engine.global_norm(tuple(ts)), want) and torch.equal(engine.global_norm(t for t in ts), want)
+    out, st = engine.clip_by_global_norm(tuple(ts), 1.0)
+    assert torch.equal(st, want) and all(torch.equal(a, b) for a, b in zip(out, engine.clip_by_global_norm(ts, 1.0)[0]))
+
+
 def test_streams_and_replays():
     ts = tensors((70001, 33, 5), (torch.float32, torch.bfloat16))
     want, st = engine.clip_by_global_norm(ts, 1.0)

@@ -280,6 +280,24 @@ def test_layouts(dtype):
             assert torch.equal(a, b)
 
 
+class _NotPlain:
+    """The compiled calls turning every call down: what is left is the Python code behind them."""
+    readout_loss = readout_grad = tensor_list = staticmethod(lambda *a: None)
+
+
+@pytest.mark.parametrize("kind", ["i32", "i64", "rows"])
+def test_compiled_and_python_calls_agree(kind, monkeypatch):
+    c = make(70, 48, 400, torch.bfloat16, kind)
+    n = dict(c, b=None, mask=None)
+    want = [call(c), call(n), call(c, (True, False, False))]
+    monkeypatch.setattr(engine, "_fast", _NotPlain)
+    got = [call(c), call(n), call(c, (True, False, False))]
+    for w, o in zip(want, got):
+        assert torch.equal(w[0], o[0]) and torch.equal(w[1], o[1])
+        for a, b in zip(w[2], o[2]):
+            assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
 def test_repeatable():
     c = make(700, 64, 5000, torch.bfloat16, "rows")
     a, b = call(c), call(c)
