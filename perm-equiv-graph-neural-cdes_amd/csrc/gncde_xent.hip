@@ -6,14 +6,15 @@
 // replacing log_softmax over materialised logits [rows, classes] (trainer_tgb.py:42-60) and its reverse mode.  The
 // logits are never stored: the loss keeps, per row and tile of classes, the largest logit and the sum of exponentials
 // relative to it; the gradient makes the logits once more, a piece of the classes at a time, and stores that piece's
-// dl as bf16 matrix operands.  All four products are one kernel, C^T = B A^T over operands that lie along their
-// contraction, on v_mfma_f32_16x16x32_bf16 with fp32 accumulation:
+// dl as a bf16 matrix operand.  All four products are one kernel, C^T = B A^T on v_mfma_f32_16x16x32_bf16 with fp32
+// accumulation; where an operand's rows lie along the contraction it is read as it lies, and where they lie across it,
+// LDS reads turn it, so one stored form of x, W and dl serves every product:
 //
 //   product   A (rows of the tile)     B (columns)          contraction   epilogue
 //   logits    W       [classes, H]     x       [rows, H]    H             largest logit, sum of exponentials
-//   logits    W piece [Vc, H]          x       [rows, H]    H             dl piece, as [rows, Vc] and [Vc, rows]
-//   gx        W^T     [H, Vc]          dl      [rows, Vc]   Vc            fp32 sums / gx
-//   gW        x^T     [H, rows]        dl^T    [Vc, rows]   rows          gW
+//   logits    W piece [Vc, H]          x       [rows, H]    H             dl piece [rows, Vc]
+//   gx        W piece, turned          dl      [rows, Vc]   Vc            fp32 sums / gx
+//   gW        x, turned                dl, turned           rows          gW
 //
 // fp32 inputs are split into three bf16 parts each (8 bits of the significand a part, rounded to nearest: nothing is
 // lost) and the six products above 2^-24 of |a||b| are summed, smallest first: fp32-class results on the bf16 matrix
@@ -21,6 +22,7 @@
 #include "gncde_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace gncde {
 namespace {
@@ -95,35 +97,31 @@ __device__ __forceinline__ floatx4 four(const void* p, int64_t i, int64_t to) {
   return v;
 }
 
+// v to p[i..i+3], up to `to`.
+template <bool F32>
+__device__ __forceinline__ void put(void* p, int64_t i, int64_t to, floatx4 v) {
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+  if (i + 4 <= to) {
+    if (F32) *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = f32x4{v[0], v[1], v[2], v[3]};
+    else
+      *reinterpret_cast<u16x4u*>(static_cast<uint16_t*>(p) + i) =
+          u16x4u{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (i + q < to) {
+      if (F32) static_cast<float*>(p)[i + q] = v[q];
+      else static_cast<uint16_t*>(p)[i + q] = to_bf16(v[q]);
+    }
+}
+
 // Packed operands: rows of Kp values (zeros behind the contraction), or for three parts rows of 3 Kp with 32 values of
 // each part side by side: value k of part q at (k / 32) * 96 + q * 32 + k % 32.
 template <int NP>
 __device__ __forceinline__ int64_t packed(int64_t k, int q) {
   return NP == 1 ? k : (k >> 5) * 96 + q * 32 + (k & 31);
-}
-
-// src [R, H] -> packed [R][Kp].
-template <bool F32, int NP>
-__global__ void k_xent_pack(const void* __restrict__ src, int64_t R, int H, int Kp, uint16_t* __restrict__ dst) {
-  const int cpr = Kp / 8;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < R * cpr; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = e / cpr;
-    const int h0 = (int)(e - r * cpr) * 8;
-    u16x8 o[NP];
-    floatx4 v[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      v[i] = h0 + 4 * i < H ? four<F32>(src, r * H + h0 + 4 * i, r * H + H) : floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint16_t p[NP];
-      split<NP>(v[i >> 2][i & 3], p);
-#pragma unroll
-      for (int q = 0; q < NP; ++q) o[q][i] = p[q];
-    }
-#pragma unroll
-    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + r * NP * Kp + packed<NP>(h0, q)) = o[q];
-  }
 }
 
 // The scale of dl: the largest |g| of the rows that count (1 where that is no use).  bf16 dl is stored over it, so that
@@ -159,55 +157,41 @@ __global__ void __launch_bounds__(256) k_xent_scale(int64_t N, Rows rows, const 
   largest_cotangent(N, rows, g, scale);
 }
 
-// src [R, H] -> transposed, packed rows of stride Rp, zeros behind R up to kPad and (LEFT) in rows left out, whatever
-// they hold.  With `scale`, the first workgroup finds that instead (a launch less).
+// src [R, H] -> packed [R][Kp]; with LEFT, rows left out are zeros, whatever they hold.  With `scale`, the first
+// workgroup finds that instead (a launch less).
 template <bool F32, int NP, bool LEFT>
-__global__ void __launch_bounds__(256) k_xent_pack_t(const void* __restrict__ src, int64_t R, int H, int64_t Rp,
-                                                     Rows rows, uint16_t* __restrict__ dst,
-                                                     const float* __restrict__ g, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256) k_xent_pack(const void* __restrict__ src, int64_t R, int H, int Kp, Rows rows,
+                                                   uint16_t* __restrict__ dst, const float* __restrict__ g,
+                                                   float* __restrict__ scale) {
   if (scale && blockIdx.x == 0) {
     largest_cotangent(R, rows, g, scale);
     return;
   }
-  const int64_t block = (int64_t)blockIdx.x - (scale ? 1 : 0);
-  __shared__ float t[64][65];
-  __shared__ bool keep[64];
-  const int64_t ht = (H + 63) / 64;
-  const int64_t r0 = (block / ht) * 64;
-  const int h0 = (int)(block % ht) * 64;
-  if (LEFT && threadIdx.x < 64) keep[threadIdx.x] = r0 + threadIdx.x < R && row_counts(rows, r0 + threadIdx.x);
-  floatx4 v[4];
-  const int c = (threadIdx.x & 15) * 4, r16 = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t r = r0 + r16 + 16 * i;
-    v[i] = r < R && h0 + c < H ? four<F32>(src, r * H + h0 + c, r * H + H) : floatx4{0.f, 0.f, 0.f, 0.f};
-  }
-  if (LEFT) __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) t[r16 + 16 * i][c + q] = !LEFT || keep[r16 + 16 * i] ? v[i][q] : 0.f;
-  __syncthreads();
-  const int rc = (threadIdx.x & 7) * 8, hh = threadIdx.x >> 3;
-  for (int i = hh; i < 64; i += 32) {
-    const int h = h0 + i;
-    if (h >= H) continue;
+  const int64_t block = (int64_t)blockIdx.x - (scale ? 1 : 0), blocks = (int64_t)gridDim.x - (scale ? 1 : 0);
+  const int cpr = Kp / 8;
+  for (int64_t e = block * 256 + threadIdx.x; e < R * cpr; e += blocks * 256) {
+    const int64_t r = e / cpr;
+    const int h0 = (int)(e - r * cpr) * 8;
+    const bool keep = !LEFT || row_counts(rows, r);
     u16x8 o[NP];
+    floatx4 v[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 2; ++i)
+      v[i] = keep && h0 + 4 * i < H ? four<F32>(src, r * H + h0 + 4 * i, r * H + H) : floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       uint16_t p[NP];
-      split<NP>(t[rc + j][i], p);
+      split<NP>(v[i >> 2][i & 3], p);
 #pragma unroll
-      for (int q = 0; q < NP; ++q) o[q][j] = p[q];
+      for (int q = 0; q < NP; ++q) o[q][i] = p[q];
     }
 #pragma unroll
-    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + (int64_t)h * NP * Rp + packed<NP>(r0 + rc, q)) = o[q];
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u16x8*>(dst + r * NP * Kp + packed<NP>(h0, q)) = o[q];
   }
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------
-enum { E_LSE = 0, E_DL = 1, E_OUT = 2 };
+enum { E_LSE = 0, E_DL = 1, E_GX = 2, E_GW = 3 };
 constexpr int kLeftOut = -2;
 
 struct GemmArgs {
@@ -215,7 +199,7 @@ struct GemmArgs {
   const uint16_t* B;
   int64_t lda, ldb;          // row strides in values (of packed rows: of all parts)
   int64_t M, N;              // rows of A and of B
-  int K;                     // contraction, a multiple of 8
+  int K;                     // contraction: a multiple of 8 of the logits, the rows of turned operands
   int kt;                    // steps over K
   int per_split, splits;     // steps a workgroup of one split takes
   int64_t tm, tn;            // tiles
@@ -229,17 +213,15 @@ struct GemmArgs {
   float* hit;                // E_LSE, indices: [N] the target's logit
   const float* stats;        // E_DL
   const float* g;
-  const float* scale;        // E_DL: dl is stored over it; E_OUT: the result is multiplied by it (may be NULL: 1)
+  const float* scale;        // E_DL: dl is stored over it; E_GX, E_GW: the result is multiplied by it (may be NULL: 1)
   uint16_t* P;               // E_DL: packed [N][ldp], classes zero-padded to mp
-  uint16_t* Pt;              // packed [M][ldpt], rows zero-padded to np
-  int64_t ldp, ldpt, mp, np;
+  int64_t ldp, mp;
   float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
   // products
-  void* out;                 // E_OUT: [N][ldo]
+  void* out;                 // [N][ldo]
   float* acc;                // fp32 [split][N][lda_c]; NULL: write `out`
   int64_t ldo, ldacc;
   int32_t add;               // acc += instead of =
-  int32_t vec;               // out rows can be written four values at a time
 };
 
 // One tile of C^T.  A step brings kStep values of every row of A and B into LDS: for one part 64 values, for three parts
@@ -256,23 +238,51 @@ struct Step {
   static __device__ __forceinline__ int place(int c, int row) {
     return NP == 1 ? c ^ (row & 7) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
   }
+  // A turned operand's step is K rows of the tile's width times NP values.  Its row k's chunk c lies at c ^ turn(k): the
+  // eight rows that one LDS cycle reads 32 bytes each of then cover all banks.
+  static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
 };
 
-// The order within a half-step of MMS products: an LDS read behind every product or two, then LOADS loads of the step
-// after next, which the compiler keeps behind the reads.
-template <int MMS, int READS, int LOADS>
+// Lane l of 16 hands in the address of four values of row l / 4 and gets value l of the four rows' 16.
+__device__ __forceinline__ u16x4 read_tr(const uint16_t* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)const_cast<uint16_t*>(p)));
+}
+
+// A barrier for what went through LDS alone: stores to memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The order within a half-step of MMS products: an LDS read behind every product or two, and the LOADS loads of the
+// step after next behind them, or in front (EARLY): that hides more of their latency and is 4 % on the logits' products
+// (8192 x 4096 x 131072), but of turned operands, with twice the reads, it is 3 to 15 % slower.
+template <int MMS, int READS, int LOADS, bool EARLY>
 __device__ __forceinline__ void interleave() {
   constexpr int PER = LOADS > 0 || MMS < 2 * READS ? 1 : 2;
-  constexpr int LATER = MMS >= READS + 2 * LOADS ? 2 : 1;
+  constexpr int LATER = MMS >= READS + 2 * LOADS && !EARLY ? 2 : 1;
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < READS; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
   }
+  if constexpr (!EARLY) {
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, LATER, 0);
-    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    for (int i = 0; i < LOADS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, LATER, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
   }
   __builtin_amdgcn_sched_group_barrier(0x008, MMS, 0);
 }
@@ -293,21 +303,23 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
-template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32>
+// SOFT: the targets are label rows.
+template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32, bool SOFT>
 __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_xent_mm(GemmArgs a) {
   typedef Step<NP> S;
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
-  static_assert(IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
+  constexpr bool OUT = EPI == E_GX || EPI == E_GW;
+  constexpr bool TA = OUT, TB = EPI == E_GW;  // turned operands
+  static_assert(RT % 4 == 0 && IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
   constexpr int TILE = (BM + BN) * S::ROW;
   constexpr int PAD = 16;  // values a staged row of dl is longer
   // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
   constexpr int HALVES = BM + BN >= 512 ? 2 : 1;
-  constexpr int STAGE_P = BN / HALVES * (BM + PAD), STAGE_PT = BM / HALVES * (BN + PAD);
-  constexpr int STAGE = EPI != E_DL ? 0 : STAGE_P > STAGE_PT ? STAGE_P : STAGE_PT;
+  constexpr int STAGE = EPI != E_DL ? 0 : BN / HALVES * (BM + PAD);
   // (One LDS object: with two, the compiler waits for every load into LDS before any read of it.)
-  constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8, INFO = EPI == E_OUT ? 0 : BN;
-  constexpr int BIAS = EPI == E_OUT ? 0 : BM;
+  constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8, INFO = OUT ? 0 : BN;
+  constexpr int BIAS = OUT ? 0 : BM;
   __shared__ __attribute__((aligned(1024))) uint16_t lds[BUFS + 2 * INFO * 8 + 2 * BIAS * 2];
   uint16_t* const stage = lds + TILE;
   // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
@@ -329,6 +341,9 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   auto place_of = [&](int i, int lane) {  // this lane's chunk of the buffer
     return i < IA ? (wave * IA + i) * 64 + lane : BM * S::CH + (wave * (IT - IA) + i - IA) * 64 + lane;
   };
+  auto turned_row = [&](int i, int lane) {  // a turned operand's: its row of the step
+    return i < IA ? place_of(i, lane) / (BM * NP / 8) : (place_of(i, lane) - BM * S::CH) / (BN * NP / 8);
+  };
   // Tile `bid`: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the order: split by split, and
   // within one in blocks of eight tiles of A by all of B.  What an XCD reads at a time stays in its cache.
   auto take = [&](uint32_t bid) {
@@ -348,42 +363,59 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int slot = place_of(i, lane), row = slot / S::CH;
+      if (i < IA ? TA : TB) {
+        const int k = turned_row(i, lane), at = i < IA ? slot : slot - BM * S::CH;
+        const int c = (at - k * ((i < IA ? BM : BN) * NP / 8)) ^ S::turn(k);
+        off[i] = ((uint32_t)k * (uint32_t)(i < IA ? a.lda : a.ldb) + c * 8) * 2u;
+        continue;
+      }
       const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
       const int rr = i < IA ? row : row - BM, most = i < IA ? most_a : most_b;
       off[i] = ((uint32_t)(rr < most ? rr : most) * (uint32_t)(i < IA ? a.lda : a.ldb) + c * 8) * 2u;
     }
     k_from = split_k * a.per_split;
     k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
-    base_a = a.A + m0 * a.lda;
-    base_b = a.B + n0 * a.ldb;
+    base_a = a.A + m0 * (TA ? NP : a.lda);
+    base_b = a.B + n0 * (TB ? NP : a.ldb);
   };
 
   auto load = [&](int k, int buf) {
     const int bytes = __builtin_amdgcn_readfirstlane((k - k_to) >> 31);  // all of 2^32, or none
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
+    // of a turned operand the step's rows that there are, to the end of the last one
+    const int64_t left = a.K - k * S::K, rows = left < S::K ? left : S::K;
+    auto rows_of = [&](const uint16_t* base, int64_t ld, int64_t at) {
+      const int64_t all = (rows * ld - at * NP) * 2;
+      const int some = k < k_to && all > 0 ? (int)all : 0;
+      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k * S::K * ld), 0,
+                                               __builtin_amdgcn_readfirstlane(some), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t ra =
+        TA ? rows_of(base_a, a.lda, m0) : __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb =
+        TB ? rows_of(base_b, a.ldb, n0) : __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
     const uint32_t at = (uint32_t)k * (S::ROW * 2);
     // of a ragged last step's chunks behind the end, one that is there: zeroed below
     const uint32_t behind = k * S::K + col >= a.K ? (uint32_t)col * 2u : 0u;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
+      const bool turned = i < IA ? TA : TB;
       uint32_t o = off[i];
-      if (NP == 1) o -= behind;
+      if (NP == 1 && !turned) o -= behind;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           i < IA ? ra : rb, (__attribute__((address_space(3))) void*)(lds + buf * TILE + place_of(i, 0) * 8), 16, o,
-          at, 0, 0);
+          turned ? 0 : at, 0, 0);
     }
   };
   // The rows of x that the tile in hand has, into info[at].
   auto fetch_rows = [&](int at) {
-    if constexpr (EPI != E_OUT) {
+    if constexpr (!OUT) {
       if (a.bias)
         for (int r = fresh(threadIdx.x); r < BM; r += NW * 64)
           bias[at * BIAS + r] = m0 + r < a.M ? value<F32>(a.bias, m0 + r) : 0.f;
       for (int r = fresh(threadIdx.x); r < BN; r += NW * 64) {
         const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1;
         const bool kept = !a.rows.mask || a.rows.mask[n] != 0;
-        const int64_t c = a.rows.kind == GNCDE_TARGET_ROWS ? 0 : row_index(a.rows, n);
+        const int64_t c = SOFT ? 0 : row_index(a.rows, n);
         floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
         if (EPI == E_DL) {
           const float lse = a.stats[2 * n], mass = a.stats[2 * n + 1];
@@ -393,7 +425,7 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         const bool in = n0 + r < a.N && kept && c >= 0;
         const int64_t t = c - a.v0;
         if (!in) v = floatx4{0.f, 0.f, 0.f, 0.f};
-        v[3] = __int_as_float(!in ? kLeftOut : a.rows.kind != GNCDE_TARGET_ROWS && t >= 0 && t < a.M ? (int)t : -1);
+        v[3] = __int_as_float(!in ? kLeftOut : !SOFT && t >= 0 && t < a.M ? (int)t : -1);
         info[at * INFO + r] = v;
       }
     }
@@ -401,11 +433,12 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   // The buffer of step k is complete for every wave, and everybody has read the other one.
   auto hand_over = [&](int k, int buf) {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-    if (NP == 1 && (k + 1) * S::K > a.K) {  // chunks behind the contraction's end
-      if (k * S::K + col >= a.K)
+    if ((NP == 1 || TA || TB) && (k + 1) * S::K > a.K) {  // what lies behind the contraction's end
 #pragma unroll
-        for (int i = 0; i < IT; ++i)
-          *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i, lane) * 8) = u16x8{};
+      for (int i = 0; i < IT; ++i) {
+        const bool behind = (i < IA ? TA : TB) ? k * S::K + turned_row(i, lane) >= a.K : NP == 1 && k * S::K + col >= a.K;
+        if (behind) *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i, lane) * 8) = u16x8{};
+      }
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     }
     asm volatile("" ::: "memory");
@@ -418,13 +451,28 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   const int fr = lane & 15, fk = lane >> 4;
   const uint16_t* la = lds + (wm * (BM / WM) + fr) * S::ROW;
   const uint16_t* lb = lds + (BM + wn * (BN / WN) + fr) * S::ROW;
+  // A turned operand's: the lane's place in its first row, and which way its chunks are turned.
+  const int turn = S::turn(fk * 8 + (fr >> 2)) * 8;
+  const uint16_t* ta = lds + (fk * 8 + (fr >> 2)) * (BM * NP) + (fr & 3) * 4;
+  const uint16_t* tb = lds + BM * S::ROW + (fk * 8 + (fr >> 2)) * (BN * NP) + (fr & 3) * 4;
+  // Its 16 columns from `t` * 16 on over 32 of its rows: rows 8 fk .. 8 fk + 3 of them and the four behind.
+  auto columns = [&](const uint16_t* lane_at, int width, int t, int q, int buf) {
+    const int pair = NP == 1 ? t : (t >> 1) * 6 + q * 2 + (t & 1);
+    const uint16_t* p = lane_at + buf * TILE + (NP == 1 ? q * 32 * width : 0) + (pair * 16 ^ turn);
+    const u16x4 u = read_tr(p), v = read_tr(p + 4 * width);
+    return __builtin_bit_cast(bf16x8, u16x8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+  };
   // Fragment set q: of one part the half-step q, of three parts the part q.
+  constexpr bool EARLY = !OUT;
+  constexpr int READS = (TA ? 2 : 1) * RT + (TB ? 2 : 1) * CT;
   auto read = [&](int q, int buf, bf16x8(&fa)[RT], bf16x8(&fb)[CT]) {
     const int c = S::place(q * 4 + fk, fr) * 8 + buf * TILE;  // tile rows are multiples of 16: place() sees fr
 #pragma unroll
-    for (int j = 0; j < CT; ++j) fb[j] = *reinterpret_cast<const bf16x8*>(lb + j * 16 * S::ROW + c);
+    for (int j = 0; j < CT; ++j)
+      fb[j] = TB ? columns(tb, BN * NP, wn * CT + j, q, buf) : *reinterpret_cast<const bf16x8*>(lb + j * 16 * S::ROW + c);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) fa[i] = *reinterpret_cast<const bf16x8*>(la + i * 16 * S::ROW + c);
+    for (int i = 0; i < RT; ++i)
+      fa[i] = TA ? columns(ta, BM * NP, wm * RT + i, q, buf) : *reinterpret_cast<const bf16x8*>(la + i * 16 * S::ROW + c);
   };
   auto multiply = [&](const bf16x8(&fa)[RT], const bf16x8(&fb)[CT]) {
 #pragma unroll
@@ -441,7 +489,7 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
   const int64_t nb = n0 + wn * (BN / WN) + fr;
 
-  if constexpr (EPI == E_OUT) {
+  if constexpr (OUT) {
     const float scale = a.scale ? *a.scale : 1.f;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
@@ -457,24 +505,9 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
           if (a.add) v += *p;
           *p = v;
         } else if (F32) {
-          float* p = static_cast<float*>(a.out) + n * a.ldo + m;
-          if (a.vec) {
-            *reinterpret_cast<floatx4*>(p) = v;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (m + q < a.M) p[q] = v[q];
-          }
+          put<true>(static_cast<float*>(a.out) + n * a.ldo, m, a.M, v);
         } else {
-          uint16_t* p = static_cast<uint16_t*>(a.out) + n * a.ldo + m;
-          const u16x4 o = {to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
-          if (a.vec) {
-            *reinterpret_cast<u16x4*>(p) = o;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (m + q < a.M) p[q] = o[q];
-          }
+          put<false>(static_cast<uint16_t*>(a.out) + n * a.ldo, m, a.M, v);
         }
       }
     }
@@ -502,12 +535,84 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
       }
   }
 
+  // Hands use(i, y) the label row's values beside acc[i][j], four i at a time on their way (more would take registers
+  // that are not there); of a row that is not `in`, another's.
+  auto labels = [&](int j, bool in, auto use) {
+    typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    const float* row = static_cast<const float*>(a.rows.target) + (in ? nb + j * 16 : 0) * a.V + a.v0 + mb;
+    if (m0 + BM <= a.M) {
+#pragma unroll
+      for (int i0 = 0; i0 < RT; i0 += 4) {
+        f32x4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const f32x4*>(row + (i0 + i) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) use(i0 + i, floatx4{y[i][0], y[i][1], y[i][2], y[i][3]});
+      }
+      return;
+    }
+    const int left = fresh((int)(a.M - mb));  // of this lane's classes
+    if (a.V < 4) {
+      floatx4 y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y[q] = q < left ? row[q] : 0.f;
+      use(0, y);
+      return;
+    }
+    // four values that end with the piece's last one where they would go beyond it, moved to their places
+#pragma unroll
+    for (int i0 = 0; i0 < RT; i0 += 4) {
+      f32x4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from = (i0 + i) * 16;
+        v[i] = *reinterpret_cast<const f32x4*>(row + (from < left - 4 ? from : left - 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int by = (i0 + i) * 16 - (left - 4);
+        floatx4 y = floatx4{v[i][0], v[i][1], v[i][2], v[i][3]};
+        if (__any(by > 0)) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float s = by <= 0 ? v[i][q] : 0.f;
+#pragma unroll
+            for (int k = 1; q + k < 4; ++k) s = by == k ? v[i][q + k] : s;
+            y[q] = s;
+          }
+        }
+        use(i0 + i, y);
+      }
+    }
+  };
+
   if constexpr (EPI == E_LSE) {
     float* sm = reinterpret_cast<float*>(stage);  // [4][WM][BN]
-    float top[CT], sum[CT], dot[CT], mass[CT];
+    float top[CT], sum[CT], dot[CT] = {}, mass[CT] = {};
+    if constexpr (SOFT) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+        labels(j, in, [&](int i, floatx4 y) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float v = in ? y[q] : 0.f;
+            mass[j] += v;
+            dot[j] += v == 0.f ? 0.f : v * acc[i][j][q];  // a class at -inf without mass adds nothing
+          }
+        });
+      }
+#pragma unroll
+      for (int d = 16; d < 64; d <<= 1)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          dot[j] += __shfl_xor(dot[j], d);
+          mass[j] += __shfl_xor(mass[j], d);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
-      top[j] = -INFINITY, sum[j] = dot[j] = mass[j] = 0.f;
+      top[j] = -INFINITY, sum[j] = 0.f;
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -531,32 +636,7 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
       sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    if (a.rows.kind == GNCDE_TARGET_ROWS) {
-#pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const int64_t n = nb + j * 16;
-        if (__float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut) {
-          const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            const int64_t m = mb + i * 16;
-            const floatx4 yv = m < a.M ? four<true>(y, m, a.M) : floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              mass[j] += yv[q];
-              dot[j] += yv[q] == 0.f ? 0.f : yv[q] * acc[i][j][q];  // a class at -inf without mass adds nothing
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int d = 16; d < 64; d <<= 1)
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-          dot[j] += __shfl_xor(dot[j], d);
-          mass[j] += __shfl_xor(mass[j], d);
-        }
-    } else {
+    if constexpr (!SOFT) {
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
         const int target = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
@@ -603,35 +683,23 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         mass += sm[(3 * WM + w) * BN + col];
       }
       a.part[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(top, sum);
-      if (a.rows.kind == GNCDE_TARGET_ROWS) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
+      if (SOFT) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
     }
     return;
   }
 
   if constexpr (EPI == E_DL) {
-    const bool soft = a.rows.kind == GNCDE_TARGET_ROWS;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
-      const int64_t n = nb + j * 16;
       const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
       const int target = __float_as_int(row[3]);
-      const bool in = target != kLeftOut;
       const float off2 = row[0], gv = row[1], gs = row[2];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
-      if (soft) {
-        if (in) {
-          const float* y = static_cast<const float*>(a.rows.target) + n * a.V + a.v0;
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            const int64_t m = mb + i * 16;
-            if (m < a.M) acc[i][j] -= gv * four<true>(y, m, a.M);
-          }
-        }
-      } else {
+      if constexpr (!SOFT) {
         const int t = target - (int)mb;
         if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
@@ -640,6 +708,22 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
             for (int q = 0; q < 4; ++q) acc[i][j][q] -= target >= 0 && t == i * 16 + q ? gv : 0.f;
         }
       }
+    }
+    if constexpr (SOFT) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(acc[i][j]));  // the exponentials first: not the labels wait
+        labels(j, __float_as_int(row[3]) != kLeftOut, [&](int i, floatx4 y) {
+          acc[i][j] -= row[1] * y;
+          asm volatile("" : "+v"(acc[i][j]));
+        });
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
       if (!__all(in)) {  // rows left out, whatever their logits
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -670,26 +754,29 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         }
       }
     }
-    // dl goes out through LDS, once as rows of classes and once as classes of rows, in whole 16-byte chunks: written
-    // from the registers, its 8 and 2 byte pieces cost 31 us a 256 x 256 tile where the staged ones cost 12.
-    constexpr int THREADS = NW * 64, HN = BN / HALVES, HM = BM / HALVES;
+    // dl goes out through LDS in whole 16-byte chunks.
+    constexpr int THREADS = NW * 64, HN = BN / HALVES;
     const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
 #pragma unroll
       for (int half = 0; half < HALVES; ++half) {
-        if (s + half > 0) __syncthreads();
+        if (s + half > 0) lds_barrier();
         if (wn * (BN / WN) / HN == half) {
 #pragma unroll
           for (int j = 0; j < CT; ++j)
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-              const floatx4 v = acc[i][j];
-              *reinterpret_cast<u16x4*>(stage + (ln - half * HN + j * 16) * (BM + PAD) + lm + i * 16) =
-                  u16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+              u16x4 part;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                part[q] = to_bf16(acc[i][j][q]);
+                if (NP > 1) acc[i][j][q] -= from_bf16(part[q]);  // what the next part holds
+              }
+              *reinterpret_cast<u16x4*>(stage + (ln - half * HN + j * 16) * (BM + PAD) + lm + i * 16) = part;
             }
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll 2
         for (int e = tid; e < HN * (BM / 8); e += THREADS) {
           const int row = e / (BM / 8), c = e % (BM / 8) * 8;
@@ -697,31 +784,6 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
           if (n < a.N && m0 + c < a.mp)
             *reinterpret_cast<u16x8*>(a.P + n * NP * a.ldp + packed<NP>(m0 + c, s)) =
                 *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
-        }
-      }
-#pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        __syncthreads();
-        if (wm * (BM / WM) / HM == half) {
-#pragma unroll
-          for (int j = 0; j < CT; ++j)
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint16_t part = to_bf16(acc[i][j][q]);
-                stage[(lm - half * HM + i * 16 + q) * (BN + PAD) + ln + j * 16] = part;
-                if (NP > 1) acc[i][j][q] -= from_bf16(part);  // what the next part holds
-              }
-        }
-        __syncthreads();
-#pragma unroll 2
-        for (int e = tid; e < HM * (BN / 8); e += THREADS) {
-          const int row = e / (BN / 8), c = e % (BN / 8) * 8;
-          const int64_t m = m0 + half * HM + row;
-          if (m < a.M && n0 + c < a.np)
-            *reinterpret_cast<u16x8*>(a.Pt + m * NP * a.ldpt + packed<NP>(n0 + c, s)) =
-                *reinterpret_cast<const u16x8*>(stage + row * (BN + PAD) + c);
         }
       }
     }
@@ -747,12 +809,13 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         const int buf = (k - k_from) & 1;
         read(1, buf, fa1, fb1);
         multiply(fa0, fb0);
-        interleave<RT * CT, RT + CT, 0>();
+        interleave<RT * CT, READS, 0, EARLY>();
         hand_over(k + 1, buf ^ 1);
+        if (EARLY) load(k + 2, buf);
         read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
-        load(k + 2, buf);
+        if (!EARLY) load(k + 2, buf);
         multiply(fa1, fb1);
-        interleave<RT * CT, RT + CT, IT>();
+        interleave<RT * CT, READS, IT, EARLY>();
       }
     } else {
       bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
@@ -761,18 +824,19 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         const int buf = (k - k_from) & 1;
         read(0, buf, ha, hb);
         multiply(ma, mb);
-        interleave<RT * CT, RT + CT, 0>();
+        interleave<RT * CT, READS, 0, EARLY>();
         read(2, buf, sa, sb);
         multiply(ma, hb);
         multiply(ha, mb);
-        interleave<2 * RT * CT, RT + CT, 0>();
+        interleave<2 * RT * CT, READS, 0, EARLY>();
         hand_over(k + 1, buf ^ 1);
+        if (EARLY) load(k + 2, buf);
         read(1, buf ^ 1, ma, mb);
-        load(k + 2, buf);
+        if (!EARLY) load(k + 2, buf);
         multiply(sa, hb);
         multiply(ha, sb);
         multiply(ha, hb);
-        interleave<3 * RT * CT, RT + CT, IT>();
+        interleave<3 * RT * CT, READS, IT, EARLY>();
       }
     }
   }
@@ -1494,9 +1558,9 @@ struct PieceCfg {
 PieceCfg piece_cfg(int64_t N, int64_t H, int64_t vc, int np, int64_t most_gx) {
   PieceCfg c;
   c.dl = cover(E_DL, vc, N, steps_of(H, np), np);
-  c.gx = choose(E_OUT, H, N, steps_of(vc, np), np, most_gx);
-  c.gw = choose(E_OUT, H, vc, steps_of(N, np), np, 64);
-  c.us = c.dl.us + c.gx.us + c.gw.us + 10 + (double)H * (double)(vc * 4 * np + N * 8) / 3e6;
+  c.gx = choose(E_GX, H, N, steps_of(vc, np), np, most_gx);
+  c.gw = choose(E_GW, H, vc, steps_of(N, np), np, 64);
+  c.us = c.dl.us + c.gx.us + c.gw.us + (double)H * (double)N * 8 / 3e6;
   return c;
 }
 
@@ -1508,13 +1572,12 @@ struct Plan {
   int ks = 1, xs = 0;
   bool f32, direct_ok;  // direct_ok: sizes allow x and W as operands as they lie (the pointers decide too)
   int np;
-  int64_t Kp, Np;       // packed contraction of x and W; rows padded
-  int64_t Ns;           // row stride of x^T and dl^T
+  int64_t Kp;           // packed contraction of x and W
   int64_t piece, whole; // classes a piece; the loss's where W is used as it lies
   int64_t bytes = 0;
   // offsets
   int64_t o_x = 0, o_w = 0, o_part = 0, o_party = 0, o_hit = 0, o_run = 0;
-  int64_t o_scale = 0, o_xt = 0, o_wt = 0, o_p = 0, o_pt = 0, o_gx = 0, o_gw = 0, o_b = 0;
+  int64_t o_scale = 0, o_p = 0, o_gx = 0, o_gw = 0, o_b = 0;
   int64_t ldacc = 0;
   PieceCfg full, last;  // the gradient's products for a full piece and the last one
 
@@ -1545,8 +1608,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   p.f32 = dtype == GNCDE_DTYPE_FP32;
   p.np = p.f32 ? 3 : 1;
   p.direct_ok = !p.f32 && H % 8 == 0;
-  p.Kp = up(H, 64), p.Np = up(std::max<int64_t>(N, 1), 64);
-  p.Ns = stride_of(p.Np);
+  p.Kp = up(H, 64);
   p.small = small_fits(H, V);
   if (p.small) {
     p.o_b = p.take(grad ? 4 * small_groups(N) * (V * H + V) : 0);
@@ -1576,10 +1638,10 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   }
   const int64_t plane = 2 * p.np;
   // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
-  const int64_t per_class = grad ? plane * (p.Ns + N + H + p.Kp) : plane * p.Kp + p.Np / 8 + 16;
+  const int64_t per_class = plane * p.Kp + (grad ? plane * N : N / 8 + 24);
   const int64_t most = std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256);
   p.piece = std::min(up(V, 256), most);
-  p.whole = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / (p.Np / 8 + 16) / 256 * 256));
+  p.whole = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / (N / 8 + 24) / 256 * 256));
   if (grad && p.piece < V) {  // of several pieces: the size whose products fill the CUs best
     double best = 0;
     for (int64_t i = 0; i < 16; ++i) {
@@ -1606,10 +1668,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
     // the last one adds to the sums that the others left
     p.last = rest == vc ? p.full : piece_cfg(N, H, rest, p.np, p.full.gx.splits);
     p.o_scale = p.take(4);
-    p.o_xt = p.take(plane * H * p.Ns);
-    p.o_wt = p.take(plane * H * stride_of(p.piece));
     p.o_p = p.take(plane * N * stride_of(p.piece));
-    p.o_pt = p.take(plane * p.piece * p.Ns);
     p.ldacc = up(H, 4);
     p.o_gx = p.take(4 * std::max(p.full.gx.splits, p.last.gx.splits) * N * p.ldacc);
     const int64_t a = p.full.gw.splits > 1 ? p.full.gw.splits * vc : 0;
@@ -1631,25 +1690,27 @@ void mm(const GemmArgs& in, const Cfg& cfg, hipStream_t st) {
   a.per_split = (int)div_up(a.kt, cfg.splits);
   // a workgroup for every place the chip has (LDS: one large or two small ones a CU), each with its share of the tiles
   const dim3 grid((unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus));
-  if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32>), grid, dim3(256), 0, st, a);
-  else if constexpr (F32) hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32>), grid, dim3(512), 0, st, a);
-}
-
-template <bool F32>
-void pack(const void* src, int64_t R, const Plan& p, uint16_t* dst, hipStream_t st) {
-  const int64_t n = R * (p.Kp / 8);
-  hipLaunchKernelGGL((k_xent_pack<F32, F32 ? 3 : 1>), dim3((unsigned)std::min(div_up(n, 256), kMostBlocks)),
-                     dim3(256), 0, st, src, R,
-                     (int)p.H, (int)p.Kp, dst);
+  const auto launch = [&](auto soft) {
+    constexpr bool SOFT = decltype(soft)::value;
+    if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
+    else if constexpr (F32)
+      hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32, SOFT>), grid, dim3(512), 0, st, a);
+    else if constexpr (EPI == E_GX)  // the wave's shorter side turned, 16 LDS reads a half-step instead of 20: 5 % faster
+      hipLaunchKernelGGL((k_xent_mm<256, 256, 4, 2, EPI, NP, F32, SOFT>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_xent_mm<256, 256, 2, 4, EPI, NP, F32, SOFT>), grid, dim3(512), 0, st, a);
+  };
+  if constexpr (EPI == E_LSE || EPI == E_DL) {
+    if (a.rows.kind == GNCDE_TARGET_ROWS) return launch(std::true_type{});
+  }
+  launch(std::false_type{});
 }
 
 template <bool F32, bool LEFT>
-void pack_t(const void* src, int64_t R, int64_t stride, const Plan& p, Rows rows, uint16_t* dst, const float* g,
-            float* scale, hipStream_t st) {
-  const int64_t blocks = div_up(R, 64) * div_up(p.H, 64) + (scale ? 1 : 0);
-  hipLaunchKernelGGL((k_xent_pack_t<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)blocks), dim3(256), 0, st, src, R, (int)p.H,
-                     stride, rows, dst, g, scale);
+void pack(const void* src, int64_t R, const Plan& p, Rows rows, uint16_t* dst, const float* g, float* scale,
+          hipStream_t st) {
+  const int64_t blocks = std::min(div_up(R * (p.Kp / 8), 256), kMostBlocks) + (scale ? 1 : 0);
+  hipLaunchKernelGGL((k_xent_pack<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)blocks), dim3(256), 0, st, src, R, (int)p.H,
+                     (int)p.Kp, rows, dst, g, scale);
 }
 
 bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -1673,7 +1734,7 @@ template <bool F32>
 Operand<F32> operand(const void* src, int64_t R, const Plan& p, int64_t at, const Call& c) {
   if (p.direct_ok && aligned(src, 16)) return {static_cast<const uint16_t*>(src), p.H, (int)p.H};
   uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + at);
-  pack<F32>(src, R, p, dst, c.st);
+  pack<F32, false>(src, R, p, c.rows, dst, nullptr, nullptr, c.st);
   return {dst, p.np * p.Kp, (int)p.Kp};
 }
 
@@ -1800,17 +1861,21 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
                          (int)(p.N * p.H), 0, part, gx, nullptr);
     return;
   }
-  const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
-  uint16_t* xt = reinterpret_cast<uint16_t*>(c.ws + p.o_xt);
-  uint16_t* wt = reinterpret_cast<uint16_t*>(c.ws + p.o_wt);
+  float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);  // three parts lose nothing to it
+  // gW multiplies every row of x, by zeros where it is left out: those rows are put aside, whatever they hold
+  const bool aside = gW && (c.rows.mask || c.rows.kind != GNCDE_TARGET_ROWS);
+  Operand<F32> x = {static_cast<const uint16_t*>(c.x), p.H, (int)p.H};
+  if (aside || !p.direct_ok || !aligned(c.x, 16)) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + p.o_x);
+    pack<F32, true>(c.x, p.N, p, c.rows, dst, g, scale, c.st);
+    x = {dst, p.np * p.Kp, (int)p.Kp};
+  } else if (scale) {
+    hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(256), 0, c.st, p.N, c.rows, g, scale);
+  }
   uint16_t* P = reinterpret_cast<uint16_t*>(c.ws + p.o_p);
-  uint16_t* Pt = reinterpret_cast<uint16_t*>(c.ws + p.o_pt);
   float* acc_x = reinterpret_cast<float*>(c.ws + p.o_gx);
   float* acc_w = reinterpret_cast<float*>(c.ws + p.o_gw);
   float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
-  float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);  // three parts lose nothing to it
-  if (gW) pack_t<F32, true>(c.x, p.N, p.Ns, p, c.rows, xt, g, scale, c.st);
-  else if (scale) hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(256), 0, c.st, p.N, c.rows, g, scale);
   const bool one = p.piece >= p.V;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad), vs = stride_of(vc);
@@ -1823,7 +1888,6 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       a.stats = stats, a.g = g;
       a.scale = scale;
       a.P = P + p.np * at, a.ldp = vs, a.mp = at + len < vc ? len : vp - at;
-      a.Pt = Pt + p.np * at * p.Ns, a.ldpt = p.Ns, a.np = p.Np;
       a.part_b = gb ? part_b + bias_rows(p.N) * at : nullptr;
       const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
       mm<E_DL, F32>(a, one_cfg, c.st);
@@ -1835,17 +1899,16 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       if (at != 0) break;
     }
     if (gx) {
-      pack_t<F32, false>(wsrc, vc, vs, p, c.rows, wt, nullptr, nullptr, c.st);
       GemmArgs q = {};
       q.scale = scale;
-      q.A = wt, q.lda = p.np * vs, q.M = p.H;
+      q.A = w.p, q.lda = w.ld, q.M = p.H;
       q.B = P, q.ldb = p.np * vs, q.N = p.N;
-      q.K = (int)vp;
-      q.out = gx, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(gx, 4 * SZ);
+      q.K = (int)vc;
+      q.out = gx, q.ldo = p.H;
       // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
       const bool sums = !one || cfg.gx.splits > 1;
       if (sums) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
-      mm<E_OUT, F32>(q, cfg.gx, c.st);
+      mm<E_GX, F32>(q, cfg.gx, c.st);
       if (sums && v0 + p.piece >= p.V)
         sum_out<F32>(p.N, p.H, one ? p.last.gx.splits : p.full.gx.splits, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H,
                      c.st);
@@ -1853,14 +1916,14 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
     if (gW) {
       GemmArgs q = {};
       q.scale = scale;
-      q.A = xt, q.lda = p.np * p.Ns, q.M = p.H;
-      q.B = Pt, q.ldb = p.np * p.Ns, q.N = vc;
-      q.K = (int)p.Np;
+      q.A = x.p, q.lda = x.ld, q.M = p.H;
+      q.B = P, q.ldb = p.np * vs, q.N = vc;
+      q.K = (int)p.N;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
-      q.out = out, q.ldo = p.H, q.vec = p.H % 4 == 0 && aligned(out, 4 * SZ);
+      q.out = out, q.ldo = p.H;
       const int sp = cfg.gw.splits;
       if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
-      mm<E_OUT, F32>(q, cfg.gw, c.st);
+      mm<E_GW, F32>(q, cfg.gw, c.st);
       if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H, c.st);
     }
   }
