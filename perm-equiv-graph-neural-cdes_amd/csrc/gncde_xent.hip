@@ -224,11 +224,23 @@ struct GemmArgs {
   int32_t add;               // acc += instead of =
 };
 
-// One tile of C^T.  A step brings kStep values of every row of A and B into LDS: for one part 64 values, for three parts
-// 32 of each part, which lie side by side in the packed operands.  Two LDS buffers; a wave's fragments are read one
-// half-step (one part: a third of the products) before they are multiplied, and the barrier that hands a buffer over
-// lies between two runs of products whose fragments are in registers already, so neither LDS latency nor the barrier
-// leaves the matrix units idle while both waves of a SIMD keep up.
+// One tile of C^T.  A step brings S::K values of every row of A and B into LDS: for one part 64 values, for three parts
+// 32 of each part, which lie side by side in the packed operands; of a turned operand as many of its rows, the tile wide.
+// Two LDS buffers; a wave's fragments are read one half-step (one part: a third of the products) before they are
+// multiplied, and the barrier that hands a buffer over lies between two runs of products whose fragments are in registers
+// already.  Workgroups stay for all their tiles, and the next tile's first operands are on their way while this one's
+// products are put out.
+//
+// Tiles of 256 x 256 (three parts: 256 x 128), eight waves of 128 x 64 (64 x 64) each: what a step reads from LDS and
+// brings there (256 KB at 128 bytes a cycle) takes as long as its products, so smaller tiles are bound by LDS; four waves
+// of 128 x 128 read a third less and were slower, with nothing to run while one waits.  128 x 128 tiles, two workgroups a
+// CU, serve where the large ones leave CUs idle.
+//
+// Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.4 ms (1.38 PFLOP/s), dl 6.7 (1.32),
+// gx 7.4 (1.19), gW 8.1 (1.08), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
+// 0.94.  The logits are bound by power: their matrix units are busy 68 % of the cycles, and the clock falls to 1.65 GHz.
+// The turned products wait for LDS reads, two instructions a fragment instead of one.  Beside them, turning W, x and dl
+// in memory cost 0.5 ms of copies and 0.8 ms of dl's second form, a tenth of the gradient at 1021 x 333 x 50021.
 template <int NP>
 struct Step {
   static constexpr int K = NP == 1 ? 64 : 32;     // contraction a step
@@ -754,7 +766,7 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
         }
       }
     }
-    // dl goes out through LDS in whole 16-byte chunks.
+    // dl goes out through LDS in whole 16-byte chunks: from the registers it would be 8-byte pieces of 16 rows.
     constexpr int THREADS = NW * 64, HN = BN / HALVES;
     const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
 #pragma unroll
@@ -918,7 +930,13 @@ __global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __rest
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * M; e += (int64_t)gridDim.x * blockDim.x) {
     const int64_t n = e / M, m = e - n * M;
     float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += acc[k * stride + n * ldacc + m];
+    for (int k0 = 0; k0 < splits; k0 += 8) {  // eight loads side by side: 64 splits of 100 x 512 18 -> 6 us
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = k0 + k < splits ? acc[(k0 + k) * stride + n * ldacc + m] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
     s *= by;
     if (F32) static_cast<float*>(out)[n * ldo + m] = s;
     else static_cast<uint16_t*>(out)[n * ldo + m] = to_bf16(s);
@@ -929,7 +947,8 @@ __global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __rest
 // W (as fp32), 16 rows of x and their dl stay in LDS and all four products run on v_mfma_f32_16x16x4f32 (either type:
 // the products of bf16 values are exact there), so nothing but the results goes to memory: the loss is one launch, the
 // gradient two (the second adds the workgroups' gW and gb).  TGB's read-out (classes = nodes, hidden 32) is this size,
-// where the tiled kernels above are eleven launches of a few microseconds.
+// where the tiled kernels above are eleven launches of a few microseconds.  255 x 32 x 255 (the loss) takes 6 us and the
+// gradient of 4080 x 32 x 255 14 and 4, of which launches, the first reads and the last writes are all but a few.
 //
 // Sixteen waves a workgroup; a row tile's classes go round the waves by 16, two rounds at most.
 constexpr int kSmallLds = 20480;     // floats: W [Vp][Hs], x [16][Hs], dl [16][Vs], joins
@@ -1197,7 +1216,8 @@ __global__ void __launch_bounds__(1024) k_xent_parts_sum(int parts, int VH, int 
 // from memory into matrix operands (16 classes, 16 bytes a lane; LDS holds x alone), eight loads ahead of the products;
 // where the classes are too few for all waves, ks of them share a tile's contraction.  The gradient reads W once for dl
 // and once more, row by row, for gx, writing gW in the same loop: a VALU product, which for so few rows hides behind
-// the bytes, and needs no transposed copy of W.
+// the bytes, and needs no transposed copy of W.  One row of 4096 against 131072 classes in bf16: 205 us,
+// 5.2 TB/s, where reads alone reach 6.4.
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 16;
 constexpr int kFewLds = 147456;   // bytes of x
@@ -1480,10 +1500,6 @@ __global__ void __launch_bounds__(256) k_xent_few_out(int N, int H, int64_t V, i
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
-// Row stride of an operand in the workspace: padded to kPad, and an odd number of 128-byte lines, so that the rows of a
-// tile do not all fall on the same channels (a stride of 8 KB cost the gW product a third of its rate).
-int64_t stride_of(int64_t k) { return up(k, kPad) | kPad; }
-
 constexpr int64_t kCus = 256;
 constexpr int64_t kMostBlocks = int64_t(1) << 20;  // of the element-wise kernels: the rest by their loops
 constexpr int64_t kPieceBytes = int64_t(1) << 30;  // of a piece's operands: fewer pieces are fewer passes over gx's sums
@@ -1503,9 +1519,11 @@ struct Cfg {
 };
 
 // The model that chooses tiles, splits and pieces: rounds of workgroups over the CUs, each its steps and a fixed part,
-// and the join of splits.  Measured on one MI355X in us: a step of a 256 x 256 tile 1.45 (1.5 PFLOP/s over 256 CUs), of
-// a 128 x 128 tile 0.83 alone on its CU and 1.05 beside another; of three parts 2.2 (256 x 128) and 1.5.  The large tile
-// is 1.4 to 2.3 times faster a product and loses where it leaves CUs without one: 784 tiles are four rounds of 256.
+// and the join of splits.  In us: a step of a 256 x 256 tile 1.45 (1.5 PFLOP/s over 256 CUs), of a 128 x 128 tile 0.83
+// alone on its CU and 1.05 beside another; of three parts 2.2 (256 x 128) and 1.5.  The large tile is 1.4 to 2.3 times
+// faster a product and loses where it leaves CUs without one: 784 tiles are four rounds of 256.  Against launches with
+// either tile forced (ten shapes, 100 to 6000 rows, 1000 to 50000 classes) its choices were the faster ones or within
+// 10 %: 512 x 1024 x 32000 takes 48 us (loss) in both tiles, 59 in large and 60 in small ones alone.
 Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, bool big, int64_t splits) {
   const Tile t = tile_of(big, np);
   const int64_t groups = div_up(M, t.bm) * div_up(N, t.bn) * splits;
@@ -1668,7 +1686,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
     // the last one adds to the sums that the others left
     p.last = rest == vc ? p.full : piece_cfg(N, H, rest, p.np, p.full.gx.splits);
     p.o_scale = p.take(4);
-    p.o_p = p.take(plane * N * stride_of(p.piece));
+    p.o_p = p.take(plane * N * up(p.piece, kPad));
     p.ldacc = up(H, 4);
     p.o_gx = p.take(4 * std::max(p.full.gx.splits, p.last.gx.splits) * N * p.ldacc);
     const int64_t a = p.full.gw.splits > 1 ? p.full.gw.splits * vc : 0;
@@ -1878,7 +1896,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
   float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
   const bool one = p.piece >= p.V;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
-    const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad), vs = stride_of(vc);
+    const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad);
     const char* wsrc = static_cast<const char*>(c.W) + v0 * p.H * SZ;
     const PieceCfg& cfg = v0 + p.piece >= p.V ? p.last : p.full;
     const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
@@ -1887,7 +1905,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, len);
       a.stats = stats, a.g = g;
       a.scale = scale;
-      a.P = P + p.np * at, a.ldp = vs, a.mp = at + len < vc ? len : vp - at;
+      a.P = P + p.np * at, a.ldp = vp, a.mp = at + len < vc ? len : vp - at;
       a.part_b = gb ? part_b + bias_rows(p.N) * at : nullptr;
       const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
       mm<E_DL, F32>(a, one_cfg, c.st);
@@ -1902,7 +1920,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs q = {};
       q.scale = scale;
       q.A = w.p, q.lda = w.ld, q.M = p.H;
-      q.B = P, q.ldb = p.np * vs, q.N = p.N;
+      q.B = P, q.ldb = p.np * vp, q.N = p.N;
       q.K = (int)vc;
       q.out = gx, q.ldo = p.H;
       // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
@@ -1917,7 +1935,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs q = {};
       q.scale = scale;
       q.A = x.p, q.lda = x.ld, q.M = p.H;
-      q.B = P, q.ldb = p.np * vs, q.N = vc;
+      q.B = P, q.ldb = p.np * vp, q.N = vc;
       q.K = (int)p.N;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H;

@@ -161,6 +161,30 @@ def test_few_rows(rows):
     check(make(rows, 512, 40000, torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("classes", [1, 2, 3, 4, 5, 130, 257, 510, 515])
+def test_label_rows_at_the_last_classes(classes, dtype):
+    """A wide hidden row (tiled kernels) and label rows whose last classes end anywhere within four."""
+    check(make(40, 300, classes, dtype, "rows"))
+
+
+def test_label_rows_without_mask_are_read_as_they_lie():
+    """Rows that start on 16 bytes and of which none can be left out."""
+    check(make(70, 64, 700, torch.bfloat16, "rows", masked=False))
+
+
+@pytest.mark.parametrize("hidden", [64, 72, 333])
+def test_hidden_gradient_alone_with_rows_left_out(hidden):
+    """NaN in the rows left out, and no gradient of the weights that would put them aside."""
+    c = make(100, hidden, 700, torch.bfloat16)
+    c["mask"][5:40] = False
+    want = call(c)[2][0]
+    x = c["x"].clone()
+    x[5:40] = float("nan")
+    got = call(dict(c, x=x), (True, False, False))[2][0]
+    assert torch.equal(got, want) and bool((got[5:40] == 0).all())
+
+
 def test_large_logits():
     """Logits in the hundreds: the largest carries all the mass and nothing overflows."""
     for dtype in (torch.float32, torch.bfloat16):
