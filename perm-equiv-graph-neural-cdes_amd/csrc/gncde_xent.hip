@@ -152,27 +152,34 @@ __device__ __forceinline__ void largest_cotangent(int64_t N, const Rows& rows, c
   if (threadIdx.x == 0) *scale = m > 1e-30f && m < 1e30f ? m : 1.f;
 }
 
-__global__ void __launch_bounds__(256) k_xent_scale(int64_t N, Rows rows, const float* __restrict__ g,
-                                                    float* __restrict__ scale) {
-  largest_cotangent(N, rows, g, scale);
-}
+// src [R, H] -> packed [R][Kp]; with `left`, rows left out are zeros, whatever they hold.
+struct PackJob {
+  const void* src;
+  uint16_t* dst;
+  int64_t R;
+  int32_t left;
+  uint32_t blocks;
+};
 
-// src [R, H] -> packed [R][Kp]; with LEFT, rows left out are zeros, whatever they hold.  With `scale`, the first
-// workgroup finds that instead (a launch less).
-template <bool F32, int NP, bool LEFT>
-__global__ void __launch_bounds__(256) k_xent_pack(const void* __restrict__ src, int64_t R, int H, int Kp, Rows rows,
-                                                   uint16_t* __restrict__ dst, const float* __restrict__ g,
-                                                   float* __restrict__ scale) {
+// x and W in one launch, either may have no blocks.  With `scale`, one workgroup more in front finds that.
+template <bool F32, int NP>
+__global__ void __launch_bounds__(256) k_xent_pack(PackJob x, PackJob w, int H, int Kp, Rows rows, int64_t N,
+                                                   const float* __restrict__ g, float* __restrict__ scale) {
   if (scale && blockIdx.x == 0) {
-    largest_cotangent(R, rows, g, scale);
+    largest_cotangent(N, rows, g, scale);
     return;
   }
-  const int64_t block = (int64_t)blockIdx.x - (scale ? 1 : 0), blocks = (int64_t)gridDim.x - (scale ? 1 : 0);
+  const uint32_t at = blockIdx.x - (scale ? 1 : 0);
+  const bool is_x = at < x.blocks;
+  const int64_t block = is_x ? at : at - x.blocks, blocks = is_x ? x.blocks : w.blocks, R = is_x ? x.R : w.R;
+  const void* src = is_x ? x.src : w.src;
+  uint16_t* dst = is_x ? x.dst : w.dst;
+  const bool left = is_x ? x.left != 0 : w.left != 0;
   const int cpr = Kp / 8;
   for (int64_t e = block * 256 + threadIdx.x; e < R * cpr; e += blocks * 256) {
     const int64_t r = e / cpr;
     const int h0 = (int)(e - r * cpr) * 8;
-    const bool keep = !LEFT || row_counts(rows, r);
+    const bool keep = !left || row_counts(rows, r);
     u16x8 o[NP];
     floatx4 v[2];
 #pragma unroll
@@ -315,24 +322,31 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
-// SOFT: the targets are label rows.
+// LDS of k_xent_mm, in 16-bit values: two buffers of a step, the second one shared with the staged dl; the rows' and the
+// classes' data, twice.
+template <int BM, int BN, int EPI, int NP>
+struct Space {
+  static constexpr int TILE = (BM + BN) * Step<NP>::ROW;
+  static constexpr int PAD = 16;  // values a staged row of dl is longer
+  // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
+  static constexpr int HALVES = BM + BN >= 512 ? 2 : 1;
+  static constexpr int STAGE = EPI != E_DL ? 0 : BN / HALVES * (BM + PAD);
+  static constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8;
+  static constexpr int INFO = EPI >= E_GX ? 0 : BN, BIAS = EPI >= E_GX ? 0 : BM;
+  static constexpr int ALL = BUFS + 2 * INFO * 8 + 2 * BIAS * 2;
+};
+
+// Tiles `first`, `first` + `step`, ... of a product.  SOFT: the targets are label rows.
 template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32, bool SOFT>
-__global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_xent_mm(GemmArgs a) {
+__device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const uint32_t first, const uint32_t step) {
   typedef Step<NP> S;
+  typedef Space<BM, BN, EPI, NP> L;
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
   constexpr bool OUT = EPI == E_GX || EPI == E_GW;
   constexpr bool TA = OUT, TB = EPI == E_GW;  // turned operands
   static_assert(RT % 4 == 0 && IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
-  constexpr int TILE = (BM + BN) * S::ROW;
-  constexpr int PAD = 16;  // values a staged row of dl is longer
-  // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
-  constexpr int HALVES = BM + BN >= 512 ? 2 : 1;
-  constexpr int STAGE = EPI != E_DL ? 0 : BN / HALVES * (BM + PAD);
-  // (One LDS object: with two, the compiler waits for every load into LDS before any read of it.)
-  constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8, INFO = OUT ? 0 : BN;
-  constexpr int BIAS = OUT ? 0 : BM;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[BUFS + 2 * INFO * 8 + 2 * BIAS * 2];
+  constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
   uint16_t* const stage = lds + TILE;
   // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
   // class within the piece (-1: none there; kLeftOut).  Fetched with the tile's first operands, one tile ahead.
@@ -802,11 +816,11 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   }
   };
 
-  take(blockIdx.x);
+  take(first);
   if (k_from < k_to) load(k_from, 0);
   fetch_rows(0);
   int at = 0;
-  for (uint32_t bid = blockIdx.x; bid < all; bid += gridDim.x, at ^= 1) {
+  for (uint32_t bid = first; bid < all; bid += step, at ^= 1) {
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -858,13 +872,28 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
   // The next tile's first operands and rows are on their way while this one's products are put out.
   const int64_t m0_now = m0, n0_now = n0;
   const int tm_now = tile_m, tn_now = tile_n, split_now = split_k;
-  if (bid + gridDim.x < all) {
-    take(bid + gridDim.x);
+  if (bid + step < all) {
+    take(bid + step);
     if (k_from < k_to) load(k_from, 0);
     fetch_rows(at ^ 1);
   }
   put_out(m0_now, n0_now, tm_now, tn_now, split_now, at);
   }
+}
+
+// (One LDS object: with two, the compiler waits for every load into LDS before any read of it.)
+template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32, bool SOFT>
+__global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_xent_mm(GemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[Space<BM, BN, EPI, NP>::ALL];
+  mm_tiles<BM, BN, WM, WN, EPI, NP, F32, SOFT>(a, lds, blockIdx.x, gridDim.x);
+}
+
+// gx and gW of a piece side by side, gx's in the first `groups` workgroups.
+template <int NP, bool F32>
+__global__ void __launch_bounds__(256, NP == 1 ? 2 : 1) k_xent_both(GemmArgs x, GemmArgs w, uint32_t groups) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[Space<128, 128, E_GW, NP>::ALL];
+  if (blockIdx.x < groups) mm_tiles<128, 128, 2, 2, E_GX, NP, F32, false>(x, lds, blockIdx.x, groups);
+  else mm_tiles<128, 128, 2, 2, E_GW, NP, F32, false>(w, lds, blockIdx.x - groups, gridDim.x - groups);
 }
 
 // A pair (largest, sum of exponentials relative to it) joined with another.
@@ -922,24 +951,42 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
   stats[2 * n + 1] = counts ? mass : 0.f;
 }
 
-// out[i] = sum over splits of acc[s][i], in the split order.
+// out[i] = sum over splits of acc[s][i], in the split order, times the scale: up to four such jobs a launch.
+struct SumJob {
+  int64_t N, M;
+  int64_t ldacc, stride, ldo;
+  const float* acc;
+  const float* scale;  // may be NULL
+  void* out;
+  int32_t splits;
+  uint32_t blocks;
+};
+
+struct SumJobs {
+  SumJob job[4];
+};
+
 template <bool F32>
-__global__ void k_xent_sum(int64_t N, int64_t M, int splits, const float* __restrict__ acc, int64_t ldacc,
-                           int64_t stride, const float* __restrict__ scale, void* __restrict__ out, int64_t ldo) {
-  const float by = scale ? *scale : 1.f;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * M; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t n = e / M, m = e - n * M;
+__global__ void __launch_bounds__(256) k_xent_sum(SumJobs jobs) {
+  uint32_t at = blockIdx.x;
+  int q = 0;
+  while (q < 3 && at >= jobs.job[q].blocks) at -= jobs.job[q++].blocks;
+  const SumJob& j = jobs.job[q];
+  const float by = j.scale ? *j.scale : 1.f;
+  const int splits = j.splits;
+  for (int64_t e = (int64_t)at * 256 + threadIdx.x; e < j.N * j.M; e += (int64_t)j.blocks * 256) {
+    const int64_t n = e / j.M, m = e - n * j.M;
     float s = 0.f;
     for (int k0 = 0; k0 < splits; k0 += 8) {  // eight loads side by side: 64 splits of 100 x 512 18 -> 6 us
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k0 + k < splits ? acc[(k0 + k) * stride + n * ldacc + m] : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = k0 + k < splits ? j.acc[(k0 + k) * j.stride + n * j.ldacc + m] : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += v[k];
     }
     s *= by;
-    if (F32) static_cast<float*>(out)[n * ldo + m] = s;
-    else static_cast<uint16_t*>(out)[n * ldo + m] = to_bf16(s);
+    if (F32) static_cast<float*>(j.out)[n * j.ldo + m] = s;
+    else static_cast<uint16_t*>(j.out)[n * j.ldo + m] = to_bf16(s);
   }
 }
 
@@ -1697,17 +1744,22 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   return true;
 }
 
-template <int EPI, bool F32>
-void mm(const GemmArgs& in, const Cfg& cfg, hipStream_t st) {
-  constexpr int NP = F32 ? 3 : 1;
-  GemmArgs a = in;
+// The product's tiles and steps; returns its workgroups: one for every place the chip has (LDS: one large or two small
+// ones a CU), each with its share of the tiles.
+template <int NP>
+unsigned lay_out(GemmArgs& a, const Cfg& cfg) {
   const Tile t = tile_of(cfg.big, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
   a.kt = (int)steps_of(a.K, NP);
   a.splits = cfg.splits;
   a.per_split = (int)div_up(a.kt, cfg.splits);
-  // a workgroup for every place the chip has (LDS: one large or two small ones a CU), each with its share of the tiles
-  const dim3 grid((unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus));
+  return (unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus);
+}
+
+template <int EPI, bool F32>
+void mm(GemmArgs a, const Cfg& cfg, hipStream_t st) {
+  constexpr int NP = F32 ? 3 : 1;
+  const dim3 grid(lay_out<NP>(a, cfg));
   const auto launch = [&](auto soft) {
     constexpr bool SOFT = decltype(soft)::value;
     if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
@@ -1723,15 +1775,15 @@ void mm(const GemmArgs& in, const Cfg& cfg, hipStream_t st) {
   launch(std::false_type{});
 }
 
-template <bool F32, bool LEFT>
-void pack(const void* src, int64_t R, const Plan& p, Rows rows, uint16_t* dst, const float* g, float* scale,
-          hipStream_t st) {
-  const int64_t blocks = std::min(div_up(R * (p.Kp / 8), 256), kMostBlocks) + (scale ? 1 : 0);
-  hipLaunchKernelGGL((k_xent_pack<F32, F32 ? 3 : 1, LEFT>), dim3((unsigned)blocks), dim3(256), 0, st, src, R, (int)p.H,
-                     (int)p.Kp, rows, dst, g, scale);
-}
-
 bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Small tiles leave room for both: 2903 x 51 x 1293 takes 13 us for the two instead of 22.
+template <bool F32>
+void mm_both(GemmArgs x, const Cfg& cx, GemmArgs w, const Cfg& cw, hipStream_t st) {
+  constexpr int NP = F32 ? 3 : 1;
+  const unsigned gx = lay_out<NP>(x, cx), gw = lay_out<NP>(w, cw);
+  hipLaunchKernelGGL((k_xent_both<NP, F32>), dim3(gx + gw), dim3(256), 0, st, x, w, gx);
+}
 
 struct Call {
   const void *x, *W, *b;
@@ -1747,13 +1799,27 @@ struct Operand {
   int K;
 };
 
-// x or a piece of W as the product's operand: as it lies where its rows start on 16 bytes, else packed.
+// x and a piece of W as the products' operands: as they lie where their rows start on 16 bytes (x: and no row is to be
+// put aside), else packed, both in one launch.  With an x from an earlier piece, W alone.  The scale of dl is found
+// beside them.
 template <bool F32>
-Operand<F32> operand(const void* src, int64_t R, const Plan& p, int64_t at, const Call& c) {
-  if (p.direct_ok && aligned(src, 16)) return {static_cast<const uint16_t*>(src), p.H, (int)p.H};
-  uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + at);
-  pack<F32, false>(src, R, p, c.rows, dst, nullptr, nullptr, c.st);
-  return {dst, p.np * p.Kp, (int)p.Kp};
+void operands(const Plan& p, const Call& c, const void* W, int64_t vc, bool aside, const float* g, float* scale,
+              Operand<F32>& x, Operand<F32>& w) {
+  PackJob jx = {}, jw = {};
+  const auto job = [&](const void* src, int64_t R, int64_t at, bool left, PackJob& j, Operand<F32>& o) {
+    if (!left && p.direct_ok && aligned(src, 16)) {
+      o = {static_cast<const uint16_t*>(src), p.H, (int)p.H};
+      return;
+    }
+    j = {src, reinterpret_cast<uint16_t*>(c.ws + at), R, left, (uint32_t)std::min(div_up(R * (p.Kp / 8), 256), kMostBlocks)};
+    o = {j.dst, p.np * p.Kp, (int)p.Kp};
+  };
+  if (!x.p) job(c.x, p.N, p.o_x, aside, jx, x);
+  job(W, vc, p.o_w, false, jw, w);
+  const uint32_t blocks = jx.blocks + jw.blocks + (scale ? 1 : 0);
+  if (blocks)
+    hipLaunchKernelGGL((k_xent_pack<F32, F32 ? 3 : 1>), dim3(blocks), dim3(256), 0, c.st, jx, jw, (int)p.H, (int)p.Kp, c.rows,
+                       p.N, g, scale);
 }
 
 // The logits of classes v0 + at .. of a piece that starts at v0.
@@ -1807,12 +1873,11 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
                        dim3(kSmallThreads), 0, c.st, a);
     return;
   }
-  const Operand<F32> x = operand<F32>(c.x, p.N, p, p.o_x, c);
+  Operand<F32> x = {}, w = {};
   const int64_t piece = p.direct_ok && aligned(c.W, 16) ? p.whole : p.piece;
   for (int64_t v0 = 0; v0 < p.V; v0 += piece) {
     const int64_t vc = std::min(piece, p.V - v0);
-    const Operand<F32> w =
-        operand<F32>(static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, p, p.o_w, c);
+    operands<F32>(p, c, static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, false, nullptr, nullptr, x, w);
     const Cover cv = cover(E_LSE, vc, p.N, steps_of(std::min(w.K, x.K), p.np), p.np);
     const int64_t tiles_a = div_up(cv.first, tile_of(cv.a.big, p.np).bm);
     const int64_t tiles = tiles_a + (cv.first < vc ? div_up(vc - cv.first, tile_of(cv.b.big, p.np).bm) : 0);
@@ -1833,12 +1898,24 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
   }
 }
 
+// Sums on their way into one launch.
 template <bool F32>
-void sum_out(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t ldacc, int64_t stride, const float* scale,
-             void* out, int64_t ldo, hipStream_t st) {
-  hipLaunchKernelGGL((k_xent_sum<F32>), dim3((unsigned)std::min(div_up(N * M, 256), kMostBlocks)), dim3(256), 0, st, N,
-                     M, (int)splits, acc, ldacc, stride, scale, out, ldo);
-}
+struct Sums {
+  SumJobs jobs = {};
+  int n = 0;
+
+  void add(int64_t N, int64_t M, int64_t splits, const float* acc, int64_t ldacc, int64_t stride, const float* scale,
+           void* out, int64_t ldo) {
+    jobs.job[n++] = {N,     M,   ldacc, stride, ldo, acc, scale, out, (int32_t)splits,
+                     (uint32_t)std::min(div_up(N * M, 256), kMostBlocks)};
+  }
+  void launch(hipStream_t st) {
+    uint32_t blocks = 0;
+    for (int i = 0; i < n; ++i) blocks += jobs.job[i].blocks;
+    if (n) hipLaunchKernelGGL((k_xent_sum<F32>), dim3(blocks), dim3(256), 0, st, jobs);
+    *this = {};
+  }
+};
 
 template <bool F32>
 void backward(const Plan& p, const Call& c, const float* stats, const float* g, void* gx, void* gW, void* gb) {
@@ -1865,15 +1942,18 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
     float* part = gx ? reinterpret_cast<float*>(c.ws + p.o_gx) : nullptr;
     const int64_t per = div_up(p.V, p.few_out), runs = div_up(p.V, per);
     const dim3 grid((unsigned)runs, (unsigned)div_up(p.H, 256 * few_cols(p.N)));
-    if (p.N == 1)
-      hipLaunchKernelGGL((k_xent_few_out<F32, 1, 8>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W, c.rows,
-                         part, gW);
-    else if (p.N <= 4)
-      hipLaunchKernelGGL((k_xent_few_out<F32, 4, 8>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W, c.rows,
-                         part, gW);
-    else
-      hipLaunchKernelGGL((k_xent_few_out<F32, 16, 4>), grid, dim3(256), 0, c.st, a.N, a.H, p.V, per, a.d, c.x, c.W,
-                         c.rows, part, gW);
+    const auto out = [&](auto rows, auto cols) {
+      hipLaunchKernelGGL((k_xent_few_out<F32, decltype(rows)::value, decltype(cols)::value>), grid, dim3(256), 0, c.st, a.N,
+                         a.H, p.V, per, a.d, c.x, c.W, c.rows, part, gW);
+    };
+    // rows that are not there cost products all the same: 2 rows of 1856 against 85678 classes take 258 us as 4, 170 as 2
+    typedef std::integral_constant<int, 4> Four;
+    typedef std::integral_constant<int, 8> Eight;
+    if (p.N == 1) out(std::integral_constant<int, 1>(), Eight());
+    else if (p.N == 2) out(std::integral_constant<int, 2>(), Eight());
+    else if (p.N <= 4) out(Four(), Eight());
+    else if (p.N <= 8) out(Eight(), Four());
+    else out(std::integral_constant<int, 16>(), Four());
     if (gx)
       hipLaunchKernelGGL((k_xent_parts_sum<F32>), dim3((unsigned)div_up(p.N * p.H, 64)), dim3(1024), 0, c.st, (int)runs,
                          (int)(p.N * p.H), 0, part, gx, nullptr);
@@ -1882,24 +1962,18 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
   float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);  // three parts lose nothing to it
   // gW multiplies every row of x, by zeros where it is left out: those rows are put aside, whatever they hold
   const bool aside = gW && (c.rows.mask || c.rows.kind != GNCDE_TARGET_ROWS);
-  Operand<F32> x = {static_cast<const uint16_t*>(c.x), p.H, (int)p.H};
-  if (aside || !p.direct_ok || !aligned(c.x, 16)) {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(c.ws + p.o_x);
-    pack<F32, true>(c.x, p.N, p, c.rows, dst, g, scale, c.st);
-    x = {dst, p.np * p.Kp, (int)p.Kp};
-  } else if (scale) {
-    hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(256), 0, c.st, p.N, c.rows, g, scale);
-  }
+  Operand<F32> x = {}, w = {};
   uint16_t* P = reinterpret_cast<uint16_t*>(c.ws + p.o_p);
   float* acc_x = reinterpret_cast<float*>(c.ws + p.o_gx);
   float* acc_w = reinterpret_cast<float*>(c.ws + p.o_gw);
   float* part_b = reinterpret_cast<float*>(c.ws + p.o_b);
   const bool one = p.piece >= p.V;
+  Sums<F32> sums;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
     const int64_t vc = std::min(p.piece, p.V - v0), vp = up(vc, kPad);
     const char* wsrc = static_cast<const char*>(c.W) + v0 * p.H * SZ;
     const PieceCfg& cfg = v0 + p.piece >= p.V ? p.last : p.full;
-    const Operand<F32> w = operand<F32>(wsrc, vc, p, p.o_w, c);
+    operands<F32>(p, c, wsrc, vc, aside, g, v0 == 0 ? scale : nullptr, x, w);
     for (int64_t at = 0; at < vc; at += cfg.dl.first) {
       const int64_t len = at == 0 ? cfg.dl.first : vc - cfg.dl.first;
       GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, len);
@@ -1911,28 +1985,26 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       mm<E_DL, F32>(a, one_cfg, c.st);
       if (gb) {
         const Tile t = tile_of(one_cfg.big, p.np);
-        sum_out<F32>(1, len, div_up(p.N, t.bn) * t.wn, a.part_b, len, len, scale,
-                     static_cast<char*>(gb) + (v0 + at) * SZ, len, c.st);
+        sums.add(1, len, div_up(p.N, t.bn) * t.wn, a.part_b, len, len, scale, static_cast<char*>(gb) + (v0 + at) * SZ, len);
       }
       if (at != 0) break;
     }
+    GemmArgs to_x = {}, to_w = {};
     if (gx) {
-      GemmArgs q = {};
+      GemmArgs& q = to_x;
       q.scale = scale;
       q.A = w.p, q.lda = w.ld, q.M = p.H;
       q.B = P, q.ldb = p.np * vp, q.N = p.N;
       q.K = (int)vc;
       q.out = gx, q.ldo = p.H;
       // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
-      const bool sums = !one || cfg.gx.splits > 1;
-      if (sums) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
-      mm<E_GX, F32>(q, cfg.gx, c.st);
-      if (sums && v0 + p.piece >= p.V)
-        sum_out<F32>(p.N, p.H, one ? p.last.gx.splits : p.full.gx.splits, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H,
-                     c.st);
+      const bool kept = !one || cfg.gx.splits > 1;
+      if (kept) q.acc = acc_x, q.ldacc = p.ldacc, q.add = v0 > 0;
+      if (kept && v0 + p.piece >= p.V)
+        sums.add(p.N, p.H, one ? p.last.gx.splits : p.full.gx.splits, acc_x, p.ldacc, p.N * p.ldacc, nullptr, gx, p.H);
     }
     if (gW) {
-      GemmArgs q = {};
+      GemmArgs& q = to_w;
       q.scale = scale;
       q.A = x.p, q.lda = x.ld, q.M = p.H;
       q.B = P, q.ldb = p.np * vp, q.N = vc;
@@ -1940,10 +2012,18 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H;
       const int sp = cfg.gw.splits;
-      if (sp > 1) q.acc = acc_w, q.ldacc = p.ldacc;
-      mm<E_GW, F32>(q, cfg.gw, c.st);
-      if (sp > 1) sum_out<F32>(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H, c.st);
+      if (sp > 1) {
+        q.acc = acc_w, q.ldacc = p.ldacc;
+        sums.add(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H);
+      }
     }
+    if (gx && gW && !cfg.gx.big && !cfg.gw.big) {
+      mm_both<F32>(to_x, cfg.gx, to_w, cfg.gw, c.st);
+    } else {
+      if (gx) mm<E_GX, F32>(to_x, cfg.gx, c.st);
+      if (gW) mm<E_GW, F32>(to_w, cfg.gw, c.st);
+    }
+    sums.launch(c.st);
   }
 }
 
@@ -1999,13 +2079,13 @@ int gncde_linear_cross_entropy_grad(int64_t rows, int64_t hidden, int64_t classe
   if (!gncde::aligned(gx, sz) || !gncde::aligned(gW, sz) || !gncde::aligned(gb, sz)) return GNCDE_ERR_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows == 0) {  // no row: gradients of nothing
-    if (p.f32) {
-      if (gW) gncde::sum_out<true>(classes, hidden, 0, nullptr, 0, 0, nullptr, gW, hidden, st);
-      if (gb) gncde::sum_out<true>(1, classes, 0, nullptr, 0, 0, nullptr, gb, classes, st);
-    } else {
-      if (gW) gncde::sum_out<false>(classes, hidden, 0, nullptr, 0, 0, nullptr, gW, hidden, st);
-      if (gb) gncde::sum_out<false>(1, classes, 0, nullptr, 0, 0, nullptr, gb, classes, st);
-    }
+    const auto zeros = [&](auto sums) {
+      if (gW) sums.add(classes, hidden, 0, nullptr, 0, 0, nullptr, gW, hidden);
+      if (gb) sums.add(1, classes, 0, nullptr, 0, 0, nullptr, gb, classes);
+      sums.launch(st);
+    };
+    if (p.f32) zeros(gncde::Sums<true>());
+    else zeros(gncde::Sums<false>());
     return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
   }
   if (!stats || !g) return GNCDE_ERR_ARG;
