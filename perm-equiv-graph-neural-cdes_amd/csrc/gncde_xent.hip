@@ -243,14 +243,18 @@ struct GemmArgs {
 // of 128 x 128 read a third less and were slower, with nothing to run while one waits.  128 x 128 tiles, two workgroups a
 // CU, serve where the large ones leave CUs idle.
 //
-// Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.4 ms (1.38 PFLOP/s), dl 6.7 (1.32),
-// gx 7.4 (1.19), gW 8.1 (1.08), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
-// 0.94.  The logits are bound by power: their matrix units are busy 68 % of the cycles, and the clock falls to 1.65 GHz.
-// The turned products wait for LDS reads, two instructions a fragment instead of one.  Beside them, turning W, x and dl
-// in memory cost 0.5 ms of copies and 0.8 ms of dl's second form, a tenth of the gradient at 1021 x 333 x 50021.
-template <int NP>
+// Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.8 (1.30),
+// gx 7.5 (1.18), gW 7.1 (1.24), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
+// 0.94.  The logits are bound by power: their matrix units are busy 70 % of the cycles, and the clock falls to 1.65 GHz.
+// The turned products wait for their operands, two LDS reads a fragment instead of one.  Turning W, x and dl in memory
+// instead cost 0.5 ms of copies and 0.8 ms for dl's second form here, a tenth of the gradient at 1021 x 333 x 50021.
+//
+// The product of two turned operands in one part (gW) takes steps of half that and four buffers: its loads are then two
+// to three steps on their way instead of one, and a hand-over leaves those of two steps there (8.6 -> 7.6 ms).  Operands
+// along the contraction would be read in pieces of half a cache line (the logits' product 7.1 -> 7.6 ms).
+template <int NP, bool DEEP>
 struct Step {
-  static constexpr int K = NP == 1 ? 64 : 32;     // contraction a step
+  static constexpr int K = NP == 1 && !DEEP ? 64 : 32;  // contraction a step
   static constexpr int ROW = K * NP;              // values a row in LDS
   static constexpr int CH = ROW / 8;              // 16-byte chunks a row
   // A row's chunk c lies at place(c, row): rows that one LDS cycle reads together then differ in bank.
@@ -279,7 +283,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 // The order within a half-step of MMS products: an LDS read behind every product or two, and the LOADS loads of the
 // step after next behind them, or in front (EARLY): that hides more of their latency and is 4 % on the logits' products
-// (8192 x 4096 x 131072), but of turned operands, with twice the reads, it is 3 to 15 % slower.
+// (8192 x 4096 x 131072), but of turned operands, with twice the reads, it is 3 to 40 % slower.
 template <int MMS, int READS, int LOADS, bool EARLY>
 __device__ __forceinline__ void interleave() {
   constexpr int PER = LOADS > 0 || MMS < 2 * READS ? 1 : 2;
@@ -326,12 +330,14 @@ __device__ __forceinline__ int fresh(int x) {
 // classes' data, twice.
 template <int BM, int BN, int EPI, int NP>
 struct Space {
-  static constexpr int TILE = (BM + BN) * Step<NP>::ROW;
+  static constexpr bool DEEP = EPI == E_GW && NP == 1;
+  static constexpr int TILE = (BM + BN) * Step<NP, DEEP>::ROW;
   static constexpr int PAD = 16;  // values a staged row of dl is longer
   // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
   static constexpr int HALVES = BM + BN >= 512 ? 2 : 1;
   static constexpr int STAGE = EPI != E_DL ? 0 : BN / HALVES * (BM + PAD);
-  static constexpr int BUFS = (TILE + (TILE > STAGE ? TILE : STAGE) + 7) / 8 * 8;
+  static constexpr int HALF = (DEEP ? 2 : 1) * TILE;  // of the buffers
+  static constexpr int BUFS = (HALF + (HALF > STAGE ? HALF : STAGE) + 7) / 8 * 8;
   static constexpr int INFO = EPI >= E_GX ? 0 : BN, BIAS = EPI >= E_GX ? 0 : BM;
   static constexpr int ALL = BUFS + 2 * INFO * 8 + 2 * BIAS * 2;
 };
@@ -339,15 +345,16 @@ struct Space {
 // Tiles `first`, `first` + `step`, ... of a product.  SOFT: the targets are label rows.
 template <int BM, int BN, int WM, int WN, int EPI, int NP, bool F32, bool SOFT>
 __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const uint32_t first, const uint32_t step) {
-  typedef Step<NP> S;
   typedef Space<BM, BN, EPI, NP> L;
+  constexpr bool DEEP = L::DEEP;
+  typedef Step<NP, DEEP> S;
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
   constexpr bool OUT = EPI == E_GX || EPI == E_GW;
   constexpr bool TA = OUT, TB = EPI == E_GW;  // turned operands
   static_assert(RT % 4 == 0 && IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
   constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
-  uint16_t* const stage = lds + TILE;
+  uint16_t* const stage = lds + L::HALF;
   // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
   // class within the piece (-1: none there; kLeftOut).  Fetched with the tile's first operands, one tile ahead.
   floatx4* const info = reinterpret_cast<floatx4*>(lds + BUFS);
@@ -457,8 +464,10 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     }
   };
   // The buffer of step k is complete for every wave, and everybody has read the other one.
-  auto hand_over = [&](int k, int buf) {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  auto hand_over = [&](int k, int buf, auto on_their_way) {
+    constexpr int LEFT = decltype(on_their_way)::value;  // newer loads, which stay on their way
+    static_assert(LEFT < 16, "fits the count's low bits");
+    __builtin_amdgcn_s_waitcnt(0x0070 | LEFT);  // vmcnt(LEFT) lgkmcnt(0)
     if ((NP == 1 || TA || TB) && (k + 1) * S::K > a.K) {  // what lies behind the contraction's end
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
@@ -490,6 +499,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   };
   // Fragment set q: of one part the half-step q, of three parts the part q.
   constexpr bool EARLY = !OUT;
+  typedef std::integral_constant<int, 0> None;
   constexpr int READS = (TA ? 2 : 1) * RT + (TB ? 2 : 1) * CT;
   auto read = [&](int q, int buf, bf16x8(&fa)[RT], bf16x8(&fb)[CT]) {
     const int c = S::place(q * 4 + fk, fr) * 8 + buf * TILE;  // tile rows are multiples of 16: place() sees fr
@@ -818,6 +828,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
 
   take(first);
   if (k_from < k_to) load(k_from, 0);
+  if (DEEP && k_from < k_to) load(k_from + 1, 1);
   fetch_rows(0);
   int at = 0;
   for (uint32_t bid = first; bid < all; bid += step, at ^= 1) {
@@ -826,9 +837,27 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   if (k_from < k_to) {
-    hand_over(k_from, 0);
-    load(k_from + 1, 1);
-    if constexpr (NP == 1) {
+    hand_over(k_from, 0, None());
+    if (!DEEP) load(k_from + 1, 1);
+    if constexpr (DEEP) {
+      load(k_from + 2, 2);
+      load(k_from + 3, 3);
+      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
+      read(0, 0, fa0, fb0);
+      // step k's products; step k + 1 is read and step k + 4 sent for
+      auto go = [&](int k, const bf16x8(&fa)[RT], const bf16x8(&fb)[CT], bf16x8(&na)[RT], bf16x8(&nb)[CT]) {
+        const int buf = (k - k_from) & 3;
+        hand_over(k + 1, (buf + 1) & 3, std::integral_constant<int, 2 * IT>());
+        read(0, (buf + 1) & 3, na, nb);  // behind the last step: what lies there, never multiplied
+        load(k + 4, buf);
+        multiply(fa, fb);
+        interleave<RT * CT, READS, IT, EARLY>();
+      };
+      for (int k = k_from; k < k_to; k += 2) {
+        go(k, fa0, fb0, fa1, fb1);
+        if (k + 1 < k_to) go(k + 1, fa1, fb1, fa0, fb0);
+      }
+    } else if constexpr (NP == 1) {
       bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
       read(0, 0, fa0, fb0);
       for (int k = k_from; k < k_to; ++k) {
@@ -836,7 +865,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         read(1, buf, fa1, fb1);
         multiply(fa0, fb0);
         interleave<RT * CT, READS, 0, EARLY>();
-        hand_over(k + 1, buf ^ 1);
+        hand_over(k + 1, buf ^ 1, None());
         if (EARLY) load(k + 2, buf);
         read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
         if (!EARLY) load(k + 2, buf);
@@ -855,7 +884,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         multiply(ma, hb);
         multiply(ha, mb);
         interleave<2 * RT * CT, READS, 0, EARLY>();
-        hand_over(k + 1, buf ^ 1);
+        hand_over(k + 1, buf ^ 1, None());
         if (EARLY) load(k + 2, buf);
         read(1, buf ^ 1, ma, mb);
         if (!EARLY) load(k + 2, buf);
@@ -875,6 +904,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   if (bid + step < all) {
     take(bid + step);
     if (k_from < k_to) load(k_from, 0);
+    if (DEEP && k_from < k_to) load(k_from + 1, 1);
     fetch_rows(at ^ 1);
   }
   put_out(m0_now, n0_now, tm_now, tn_now, split_now, at);
@@ -891,6 +921,7 @@ __global__ void __launch_bounds__(WM* WN * 64, NP == 1 || BM == 256 ? 2 : 1) k_x
 // gx and gW of a piece side by side, gx's in the first `groups` workgroups.
 template <int NP, bool F32>
 __global__ void __launch_bounds__(256, NP == 1 ? 2 : 1) k_xent_both(GemmArgs x, GemmArgs w, uint32_t groups) {
+  static_assert(Space<128, 128, E_GX, NP>::ALL == Space<128, 128, E_GW, NP>::ALL, "one space for either");
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Space<128, 128, E_GW, NP>::ALL];
   if (blockIdx.x < groups) mm_tiles<128, 128, 2, 2, E_GX, NP, F32, false>(x, lds, blockIdx.x, groups);
   else mm_tiles<128, 128, 2, 2, E_GW, NP, F32, false>(w, lds, blockIdx.x - groups, gridDim.x - groups);
@@ -1557,7 +1588,7 @@ struct Tile {
 
 Tile tile_of(bool big, int np) { return big ? Tile{256, np == 1 ? 256 : 128, np == 1 ? 4 : 2} : Tile{128, 128, 2}; }
 
-int64_t steps_of(int64_t K, int np) { return np == 1 ? div_up(K, 64) : up(K, kPad) / 32; }
+int64_t steps_of(int epi, int64_t K, int np) { return np == 1 ? div_up(K, epi == E_GW ? 32 : 64) : up(K, kPad) / 32; }
 
 struct Cfg {
   bool big = true;  // 256 x 256 tiles (three parts: 256 x 128), else 128 x 128
@@ -1575,7 +1606,7 @@ Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, bool big, int64_t sp
   const Tile t = tile_of(big, np);
   const int64_t groups = div_up(M, t.bm) * div_up(N, t.bn) * splits;
   const bool two = !big && np == 1 && groups > kCus;
-  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) : (big ? 2.2 : 1.5);
+  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) * (epi == E_GW ? 0.5 : 1) : (big ? 2.2 : 1.5);
   const double fixed = epi == E_DL ? (big ? 16 : 12) : 7;
   Cfg c{big, (int)splits, (double)div_up(groups, two ? 2 * kCus : kCus) * ((double)div_up(kt, splits) * step + fixed)};
   if (splits > 1) c.us += 5 + (double)splits * (double)N * (double)M * 8 / 4.5e6;
@@ -1586,7 +1617,7 @@ Cfg choose(int epi, int64_t M, int64_t N, int64_t kt, int np, int64_t most_split
   Cfg best = cost(epi, M, N, kt, np, true, 1);
   const int64_t tiles = div_up(M, 256) * div_up(N, 256);
   for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > most_splits || s * 2 > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
+    if (s > most_splits || s * (np == 1 && epi == E_GW ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
     for (const bool big : {true, false}) {
       const Cfg c = cost(epi, M, N, kt, np, big, div_up(kt, div_up(kt, s)));  // no split without a step
       if (c.us < best.us) best = c;
@@ -1622,9 +1653,9 @@ struct PieceCfg {
 
 PieceCfg piece_cfg(int64_t N, int64_t H, int64_t vc, int np, int64_t most_gx) {
   PieceCfg c;
-  c.dl = cover(E_DL, vc, N, steps_of(H, np), np);
-  c.gx = choose(E_GX, H, N, steps_of(vc, np), np, most_gx);
-  c.gw = choose(E_GW, H, vc, steps_of(N, np), np, 64);
+  c.dl = cover(E_DL, vc, N, steps_of(E_DL, H, np), np);
+  c.gx = choose(E_GX, H, N, steps_of(E_GX, vc, np), np, most_gx);
+  c.gw = choose(E_GW, H, vc, steps_of(E_GW, N, np), np, 64);
   c.us = c.dl.us + c.gx.us + c.gw.us + (double)H * (double)N * 8 / 3e6;
   return c;
 }
@@ -1746,11 +1777,11 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
 
 // The product's tiles and steps; returns its workgroups: one for every place the chip has (LDS: one large or two small
 // ones a CU), each with its share of the tiles.
-template <int NP>
+template <int EPI, int NP>
 unsigned lay_out(GemmArgs& a, const Cfg& cfg) {
   const Tile t = tile_of(cfg.big, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
-  a.kt = (int)steps_of(a.K, NP);
+  a.kt = (int)steps_of(EPI, a.K, NP);
   a.splits = cfg.splits;
   a.per_split = (int)div_up(a.kt, cfg.splits);
   return (unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus);
@@ -1759,7 +1790,7 @@ unsigned lay_out(GemmArgs& a, const Cfg& cfg) {
 template <int EPI, bool F32>
 void mm(GemmArgs a, const Cfg& cfg, hipStream_t st) {
   constexpr int NP = F32 ? 3 : 1;
-  const dim3 grid(lay_out<NP>(a, cfg));
+  const dim3 grid(lay_out<EPI, NP>(a, cfg));
   const auto launch = [&](auto soft) {
     constexpr bool SOFT = decltype(soft)::value;
     if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
@@ -1781,7 +1812,7 @@ bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) 
 template <bool F32>
 void mm_both(GemmArgs x, const Cfg& cx, GemmArgs w, const Cfg& cw, hipStream_t st) {
   constexpr int NP = F32 ? 3 : 1;
-  const unsigned gx = lay_out<NP>(x, cx), gw = lay_out<NP>(w, cw);
+  const unsigned gx = lay_out<E_GX, NP>(x, cx), gw = lay_out<E_GW, NP>(w, cw);
   hipLaunchKernelGGL((k_xent_both<NP, F32>), dim3(gx + gw), dim3(256), 0, st, x, w, gx);
 }
 
@@ -1878,7 +1909,7 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
   for (int64_t v0 = 0; v0 < p.V; v0 += piece) {
     const int64_t vc = std::min(piece, p.V - v0);
     operands<F32>(p, c, static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, false, nullptr, nullptr, x, w);
-    const Cover cv = cover(E_LSE, vc, p.N, steps_of(std::min(w.K, x.K), p.np), p.np);
+    const Cover cv = cover(E_LSE, vc, p.N, steps_of(E_LSE, std::min(w.K, x.K), p.np), p.np);
     const int64_t tiles_a = div_up(cv.first, tile_of(cv.a.big, p.np).bm);
     const int64_t tiles = tiles_a + (cv.first < vc ? div_up(vc - cv.first, tile_of(cv.b.big, p.np).bm) : 0);
     for (int64_t at = 0; at < vc; at += cv.first) {
