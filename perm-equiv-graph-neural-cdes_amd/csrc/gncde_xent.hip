@@ -204,7 +204,7 @@ constexpr int kLeftOut = -2;
 struct GemmArgs {
   const uint16_t* A;
   const uint16_t* B;
-  int64_t lda, ldb;          // row strides in values (of packed rows: of all parts)
+  int64_t lda, ldb;          // row strides in values (of packed rows: of all parts); dl has none
   int64_t M, N;              // rows of A and of B
   int K;                     // contraction: a multiple of 8 of the logits, the rows of turned operands
   int kt;                    // steps over K
@@ -221,8 +221,8 @@ struct GemmArgs {
   const float* stats;        // E_DL
   const float* g;
   const float* scale;        // E_DL: dl is stored over it; E_GX, E_GW: the result is multiplied by it (may be NULL: 1)
-  uint16_t* P;               // E_DL: packed [N][ldp], classes zero-padded to mp
-  int64_t ldp, mp;
+  uint16_t* P;               // E_DL: [class / 32][N][part][32], classes zero-padded to mp
+  int64_t mp;
   float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
   // products
   void* out;                 // [N][ldo]
@@ -244,14 +244,15 @@ struct GemmArgs {
 // CU, serve where the large ones leave CUs idle.
 //
 // Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.8 (1.30),
-// gx 7.5 (1.18), gW 7.1 (1.24), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
+// gx 6.9 (1.27), gW 7.2 (1.22), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
 // 0.94.  The logits are bound by power: their matrix units are busy 70 % of the cycles, and the clock falls to 1.65 GHz.
 // The turned products wait for their operands, two LDS reads a fragment instead of one.  Turning W, x and dl in memory
 // instead cost 0.5 ms of copies and 0.8 ms for dl's second form here, a tenth of the gradient at 1021 x 333 x 50021.
 //
-// The product of two turned operands in one part (gW) takes steps of half that and four buffers: its loads are then two
-// to three steps on their way instead of one, and a hand-over leaves those of two steps there (8.6 -> 7.6 ms).  Operands
-// along the contraction would be read in pieces of half a cache line (the logits' product 7.1 -> 7.6 ms).
+// The one-part products with turned operands (gx, gW) take steps of half that and four buffers (DEEP): their loads are
+// then two to three steps on their way instead of one, and a hand-over leaves those of two steps there (gW 8.6 -> 7.6 ms,
+// gx 7.5 -> 6.9).  dl lies in blocks of 32 classes for that, [class / 32][row][part][32]: a step's rows of it are one run
+// of memory.  The logits' operands lie as their rows do and would be read in pieces of half a cache line (7.1 -> 7.6 ms).
 template <int NP, bool DEEP>
 struct Step {
   static constexpr int K = NP == 1 && !DEEP ? 64 : 32;  // contraction a step
@@ -259,11 +260,13 @@ struct Step {
   static constexpr int CH = ROW / 8;              // 16-byte chunks a row
   // A row's chunk c lies at place(c, row): rows that one LDS cycle reads together then differ in bank.
   static __device__ __forceinline__ int place(int c, int row) {
-    return NP == 1 ? c ^ (row & 7) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
+    return NP == 1 ? (DEEP ? c ^ ((row >> 2) & 3) : c ^ (row & 7)) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
   }
   // A turned operand's step is K rows of the tile's width times NP values.  Its row k's chunk c lies at c ^ turn(k): the
   // eight rows that one LDS cycle reads 32 bytes each of then cover all banks.
   static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
+  // dl's, in blocks of 32 columns: [block][row][32 values of every part].
+  static __device__ __forceinline__ int turn_dl(int k) { return ((k >> 3) & 1) << 1; }
 };
 
 // Lane l of 16 hands in the address of four values of row l / 4 and gets value l of the four rows' 16.
@@ -330,7 +333,7 @@ __device__ __forceinline__ int fresh(int x) {
 // classes' data, twice.
 template <int BM, int BN, int EPI, int NP>
 struct Space {
-  static constexpr bool DEEP = EPI == E_GW && NP == 1;
+  static constexpr bool DEEP = EPI >= E_GX && NP == 1;
   static constexpr int TILE = (BM + BN) * Step<NP, DEEP>::ROW;
   static constexpr int PAD = 16;  // values a staged row of dl is longer
   // dl is staged beside the first buffer, which already takes the next tile: in two halves where one does not fit
@@ -375,7 +378,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     return i < IA ? (wave * IA + i) * 64 + lane : BM * S::CH + (wave * (IT - IA) + i - IA) * 64 + lane;
   };
   auto turned_row = [&](int i, int lane) {  // a turned operand's: its row of the step
-    return i < IA ? place_of(i, lane) / (BM * NP / 8) : (place_of(i, lane) - BM * S::CH) / (BN * NP / 8);
+    return i < IA ? place_of(i, lane) / (BM * NP / 8) : (place_of(i, lane) - BM * S::CH) / S::CH % 32;
   };
   // Tile `bid`: consecutive workgroups go round the eight XCDs, so each XCD takes a run of the order: split by split, and
   // within one in blocks of eight tiles of A by all of B.  What an XCD reads at a time stays in its cache.
@@ -396,47 +399,60 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int slot = place_of(i, lane), row = slot / S::CH;
-      if (i < IA ? TA : TB) {
-        const int k = turned_row(i, lane), at = i < IA ? slot : slot - BM * S::CH;
-        const int c = (at - k * ((i < IA ? BM : BN) * NP / 8)) ^ S::turn(k);
-        off[i] = ((uint32_t)k * (uint32_t)(i < IA ? a.lda : a.ldb) + c * 8) * 2u;
+      if (i < IA && TA) {
+        const int k = turned_row(i, lane);
+        const int c = (slot - k * (BM * NP / 8)) ^ S::turn(k);
+        off[i] = ((uint32_t)k * (uint32_t)a.lda + c * 8) * 2u;
+        continue;
+      }
+      if (i >= IA && TB) {
+        const int at = slot - BM * S::CH, block = at / (32 * S::CH), k = turned_row(i, lane);
+        const int c = (at % S::CH) ^ S::turn_dl(k);
+        off[i] = ((uint32_t)(block * a.K + k) * (uint32_t)S::ROW + c * 8) * 2u;
         continue;
       }
       const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
       const int rr = i < IA ? row : row - BM, most = i < IA ? most_a : most_b;
-      off[i] = ((uint32_t)(rr < most ? rr : most) * (uint32_t)(i < IA ? a.lda : a.ldb) + c * 8) * 2u;
+      off[i] = ((uint32_t)(rr < most ? rr : most) * (uint32_t)(i < IA ? a.lda : OUT ? S::ROW : a.ldb) + c * 8) * 2u;
     }
     k_from = split_k * a.per_split;
     k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
     base_a = a.A + m0 * (TA ? NP : a.lda);
-    base_b = a.B + n0 * (TB ? NP : a.ldb);
+    base_b = a.B + n0 * (TB ? (int64_t)a.K * NP : OUT ? S::ROW : a.ldb);
   };
 
   auto load = [&](int k, int buf) {
     const int bytes = __builtin_amdgcn_readfirstlane((k - k_to) >> 31);  // all of 2^32, or none
-    // of a turned operand the step's rows that there are, to the end of the last one
-    const int64_t left = a.K - k * S::K, rows = left < S::K ? left : S::K;
-    auto rows_of = [&](const uint16_t* base, int64_t ld, int64_t at) {
-      const int64_t all = (rows * ld - at * NP) * 2;
+    __amdgpu_buffer_rsrc_t ra, rb;
+    if constexpr (TA) {  // the step's rows that there are, to the end of the last one
+      const int64_t left = (int64_t)a.K - (int64_t)k * S::K, rows = left < S::K ? left : S::K;
+      const int64_t all = (rows * a.lda - m0 * NP) * 2;
       const int some = k < k_to && all > 0 ? (int)all : 0;
-      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k * S::K * ld), 0,
-                                               __builtin_amdgcn_readfirstlane(some), 0x00020000);
-    };
-    const __amdgpu_buffer_rsrc_t ra =
-        TA ? rows_of(base_a, a.lda, m0) : __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb =
-        TB ? rows_of(base_b, a.ldb, n0) : __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
+      ra = __builtin_amdgcn_make_buffer_rsrc((void*)(base_a + (int64_t)k * S::K * a.lda), 0,
+                                             __builtin_amdgcn_readfirstlane(some), 0x00020000);
+    } else {
+      ra = __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
+    }
+    if constexpr (TB) {  // to the end of dl
+      const int64_t all = ((((a.N + 63) / 64 * 64 - n0) / 32) * a.K - (int64_t)k * 32) * S::ROW * 2;
+      const int64_t most = all < 0xffffffffll ? all : 0xffffffffll;
+      rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base_b + (int64_t)k * 32 * S::ROW), 0,
+                                             __builtin_amdgcn_readfirstlane(k < k_to ? (int)(uint32_t)most : 0), 0x00020000);
+    } else if constexpr (OUT) {
+      rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base_b + (int64_t)k * a.N * S::ROW), 0, bytes, 0x00020000);
+    } else {
+      rb = __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
+    }
     const uint32_t at = (uint32_t)k * (S::ROW * 2);
     // of a ragged last step's chunks behind the end, one that is there: zeroed below
     const uint32_t behind = k * S::K + col >= a.K ? (uint32_t)col * 2u : 0u;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const bool turned = i < IA ? TA : TB;
       uint32_t o = off[i];
-      if (NP == 1 && !turned) o -= behind;
+      if (NP == 1 && !OUT) o -= behind;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           i < IA ? ra : rb, (__attribute__((address_space(3))) void*)(lds + buf * TILE + place_of(i, 0) * 8), 16, o,
-          turned ? 0 : at, 0, 0);
+          OUT ? 0 : at, 0, 0);
     }
   };
   // The rows of x that the tile in hand has, into info[at].
@@ -471,7 +487,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     if ((NP == 1 || TA || TB) && (k + 1) * S::K > a.K) {  // what lies behind the contraction's end
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const bool behind = (i < IA ? TA : TB) ? k * S::K + turned_row(i, lane) >= a.K : NP == 1 && k * S::K + col >= a.K;
+        const bool behind = (i < IA ? TA : TB) ? k * S::K + turned_row(i, lane) >= a.K : NP == 1 && !OUT && k * S::K + col >= a.K;
         if (behind) *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i, lane) * 8) = u16x8{};
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -489,13 +505,18 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   // A turned operand's: the lane's place in its first row, and which way its chunks are turned.
   const int turn = S::turn(fk * 8 + (fr >> 2)) * 8;
   const uint16_t* ta = lds + (fk * 8 + (fr >> 2)) * (BM * NP) + (fr & 3) * 4;
-  const uint16_t* tb = lds + BM * S::ROW + (fk * 8 + (fr >> 2)) * (BN * NP) + (fr & 3) * 4;
-  // Its 16 columns from `t` * 16 on over 32 of its rows: rows 8 fk .. 8 fk + 3 of them and the four behind.
-  auto columns = [&](const uint16_t* lane_at, int width, int t, int q, int buf) {
-    const int pair = NP == 1 ? t : (t >> 1) * 6 + q * 2 + (t & 1);
-    const uint16_t* p = lane_at + buf * TILE + (NP == 1 ? q * 32 * width : 0) + (pair * 16 ^ turn);
+  const uint16_t* tb = lds + BM * S::ROW + (fk * 8 + (fr >> 2)) * S::ROW + (fr & 3) * 4;
+  // Its 16 columns from `t` * 16 on over 32 rows: rows 8 fk .. 8 fk + 3 of them and the four behind.
+  auto columns = [&](const uint16_t* p, int width) {
     const u16x4 u = read_tr(p), v = read_tr(p + 4 * width);
     return __builtin_bit_cast(bf16x8, u16x8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+  };
+  auto columns_a = [&](int t, int q, int buf) {
+    const int pair = NP == 1 ? t : (t >> 1) * 6 + q * 2 + (t & 1);
+    return columns(ta + buf * TILE + (pair * 16 ^ turn), BM * NP);
+  };
+  auto columns_b = [&](int t, int q, int buf) {
+    return columns(tb + buf * TILE + (t >> 1) * (32 * S::ROW) + q * 32 + ((t & 1) * 16 ^ S::turn_dl(fk * 8) * 8), S::ROW);
   };
   // Fragment set q: of one part the half-step q, of three parts the part q.
   constexpr bool EARLY = !OUT;
@@ -505,10 +526,10 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     const int c = S::place(q * 4 + fk, fr) * 8 + buf * TILE;  // tile rows are multiples of 16: place() sees fr
 #pragma unroll
     for (int j = 0; j < CT; ++j)
-      fb[j] = TB ? columns(tb, BN * NP, wn * CT + j, q, buf) : *reinterpret_cast<const bf16x8*>(lb + j * 16 * S::ROW + c);
+      fb[j] = TB ? columns_b(wn * CT + j, q, buf) : *reinterpret_cast<const bf16x8*>(lb + j * 16 * S::ROW + c);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
-      fa[i] = TA ? columns(ta, BM * NP, wm * RT + i, q, buf) : *reinterpret_cast<const bf16x8*>(la + i * 16 * S::ROW + c);
+      fa[i] = TA ? columns_a(wm * RT + i, q, buf) : *reinterpret_cast<const bf16x8*>(la + i * 16 * S::ROW + c);
   };
   auto multiply = [&](const bf16x8(&fa)[RT], const bf16x8(&fb)[CT]) {
 #pragma unroll
@@ -814,11 +835,11 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         }
         lds_barrier();
 #pragma unroll 2
-        for (int e = tid; e < HN * (BM / 8); e += THREADS) {
-          const int row = e / (BM / 8), c = e % (BM / 8) * 8;
+        for (int e = tid; e < HN * (BM / 8); e += THREADS) {  // 16 rows of a block a wave: 1 KB
+          const int row = (e >> 2) % HN, c = (e >> 2) / HN * 32 + (e & 3) * 8;
           const int64_t n = n0 + half * HN + row;
           if (n < a.N && m0 + c < a.mp)
-            *reinterpret_cast<u16x8*>(a.P + n * NP * a.ldp + packed<NP>(m0 + c, s)) =
+            *reinterpret_cast<u16x8*>(a.P + ((m0 + c) / 32 * a.N + n) * (32 * NP) + s * 32 + (c & 31)) =
                 *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
         }
       }
@@ -1588,7 +1609,7 @@ struct Tile {
 
 Tile tile_of(bool big, int np) { return big ? Tile{256, np == 1 ? 256 : 128, np == 1 ? 4 : 2} : Tile{128, 128, 2}; }
 
-int64_t steps_of(int epi, int64_t K, int np) { return np == 1 ? div_up(K, epi == E_GW ? 32 : 64) : up(K, kPad) / 32; }
+int64_t steps_of(int epi, int64_t K, int np) { return np == 1 ? div_up(K, epi == E_GX || epi == E_GW ? 32 : 64) : up(K, kPad) / 32; }
 
 struct Cfg {
   bool big = true;  // 256 x 256 tiles (three parts: 256 x 128), else 128 x 128
@@ -1606,7 +1627,7 @@ Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, bool big, int64_t sp
   const Tile t = tile_of(big, np);
   const int64_t groups = div_up(M, t.bm) * div_up(N, t.bn) * splits;
   const bool two = !big && np == 1 && groups > kCus;
-  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) * (epi == E_GW ? 0.5 : 1) : (big ? 2.2 : 1.5);
+  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) * (epi == E_GX || epi == E_GW ? 0.5 : 1) : (big ? 2.2 : 1.5);
   const double fixed = epi == E_DL ? (big ? 16 : 12) : 7;
   Cfg c{big, (int)splits, (double)div_up(groups, two ? 2 * kCus : kCus) * ((double)div_up(kt, splits) * step + fixed)};
   if (splits > 1) c.us += 5 + (double)splits * (double)N * (double)M * 8 / 4.5e6;
@@ -1617,7 +1638,7 @@ Cfg choose(int epi, int64_t M, int64_t N, int64_t kt, int np, int64_t most_split
   Cfg best = cost(epi, M, N, kt, np, true, 1);
   const int64_t tiles = div_up(M, 256) * div_up(N, 256);
   for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > most_splits || s * (np == 1 && epi == E_GW ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
+    if (s > most_splits || s * (np == 1 && (epi == E_GX || epi == E_GW) ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
     for (const bool big : {true, false}) {
       const Cfg c = cost(epi, M, N, kt, np, big, div_up(kt, div_up(kt, s)));  // no split without a step
       if (c.us < best.us) best = c;
@@ -2010,7 +2031,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, len);
       a.stats = stats, a.g = g;
       a.scale = scale;
-      a.P = P + p.np * at, a.ldp = vp, a.mp = at + len < vc ? len : vp - at;
+      a.P = P + p.np * at * p.N, a.mp = at + len < vc ? len : vp - at;
       a.part_b = gb ? part_b + bias_rows(p.N) * at : nullptr;
       const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
       mm<E_DL, F32>(a, one_cfg, c.st);
@@ -2025,7 +2046,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs& q = to_x;
       q.scale = scale;
       q.A = w.p, q.lda = w.ld, q.M = p.H;
-      q.B = P, q.ldb = p.np * vp, q.N = p.N;
+      q.B = P, q.N = p.N;
       q.K = (int)vc;
       q.out = gx, q.ldo = p.H;
       // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
@@ -2038,7 +2059,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs& q = to_w;
       q.scale = scale;
       q.A = x.p, q.lda = x.ld, q.M = p.H;
-      q.B = P, q.ldb = p.np * vp, q.N = vc;
+      q.B = P, q.N = vc;
       q.K = (int)p.N;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H;
