@@ -150,10 +150,11 @@ def test_large_tiles(size, kind, dtype):
     check(make(*size, dtype, kind))
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_classes_in_several_pieces(dtype):
-    """8200 rows: the gradient takes the classes in pieces (the last one ragged)."""
-    check(make(8200, 40, 17001, dtype))
+@pytest.mark.parametrize("rows,dtype,kind", [(12000, torch.float32, "i64"), (12000, torch.float32, "rows"),
+                                             (33000, torch.bfloat16, "i64"), (33000, torch.bfloat16, "rows")])
+def test_classes_in_several_pieces(rows, dtype, kind):
+    """So many rows that dl of all classes passes 1 GiB: the gradient takes the classes in pieces, the last one ragged."""
+    check(make(rows, 40, 17001, dtype, kind))
 
 
 @pytest.mark.parametrize("rows", [1, 2, 16, 17, 40])
@@ -166,6 +167,14 @@ def test_few_rows(rows):
 def test_label_rows_at_the_last_classes(classes, dtype):
     """A wide hidden row (tiled kernels) and label rows whose last classes end anywhere within four."""
     check(make(40, 300, classes, dtype, "rows"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,classes", [(31, 513), (32, 545), (33, 543), (63, 608), (64, 577), (65, 639), (97, 640),
+                                          (129, 1025), (255, 1055), (256, 1056), (257, 1057)])
+def test_rows_and_classes_around_the_steps(rows, classes, dtype):
+    """Contractions that end anywhere within the steps of gx (classes) and gW (rows)."""
+    check(make(rows, 136, classes, dtype))
 
 
 def test_label_rows_without_mask_are_read_as_they_lie():
