@@ -241,7 +241,7 @@ struct GemmArgs {
 // Tiles of 256 x 256 (three parts: 256 x 128), eight waves of 128 x 64 (64 x 64) each: what a step reads from LDS and
 // brings there (256 KB at 128 bytes a cycle) takes as long as its products, so smaller tiles are bound by LDS; four waves
 // of 128 x 128 read a third less and were slower, with nothing to run while one waits.  128 x 128 tiles, two workgroups a
-// CU, serve where the large ones leave CUs idle.
+// CU, and 128 x 64 ones (the logits) serve where larger ones leave CUs idle.
 //
 // Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.8 (1.30),
 // gx 6.9 (1.27), gW 7.2 (1.22), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
@@ -1607,40 +1607,55 @@ struct Tile {
   int64_t bm, bn, wn;
 };
 
-Tile tile_of(bool big, int np) { return big ? Tile{256, np == 1 ? 256 : 128, np == 1 ? 4 : 2} : Tile{128, 128, 2}; }
+enum { T_LARGE, T_SMALL, T_HALF };  // 256 x 256 (three parts: 256 x 128); 128 x 128; 128 x 64, of the logits alone
+
+Tile tile_of(int tile, int np) {
+  if (tile == T_LARGE) return Tile{256, np == 1 ? 256 : 128, np == 1 ? 4 : 2};
+  return Tile{128, tile == T_SMALL ? 128 : 64, 2};
+}
+
+// Workgroups of a tile that a CU holds at once, by their LDS.
+int64_t places(int tile, int np) { return tile == T_LARGE || (tile == T_SMALL && np == 3) ? 1 : np == 1 && tile == T_HALF ? 3 : 2; }
+
 
 int64_t steps_of(int epi, int64_t K, int np) { return np == 1 ? div_up(K, epi == E_GX || epi == E_GW ? 32 : 64) : up(K, kPad) / 32; }
 
 struct Cfg {
-  bool big = true;  // 256 x 256 tiles (three parts: 256 x 128), else 128 x 128
+  int tile = T_LARGE;
   int splits = 1;   // of the contraction
   double us = 0;    // what the model below says
 };
 
 // The model that chooses tiles, splits and pieces: rounds of workgroups over the CUs, each its steps and a fixed part,
 // and the join of splits.  In us: a step of a 256 x 256 tile 1.45 (1.5 PFLOP/s over 256 CUs), of a 128 x 128 tile 0.83
-// alone on its CU and 1.05 beside another; of three parts 2.2 (256 x 128) and 1.5.  The large tile is 1.4 to 2.3 times
-// faster a product and loses where it leaves CUs without one: 784 tiles are four rounds of 256.  Against launches with
-// either tile forced (ten shapes, 100 to 6000 rows, 1000 to 50000 classes) its choices were the faster ones or within
-// 10 %: 512 x 1024 x 32000 takes 48 us (loss) in both tiles, 59 in large and 60 in small ones alone.
-Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, bool big, int64_t splits) {
-  const Tile t = tile_of(big, np);
+// alone on its CU and 1.05 beside another, of a 128 x 64 tile 0.55, 0.65 and 0.95 beside two; of three parts 2.2 (256 x
+// 128), 1.5 and 0.85 or 1.35 beside another.  The large tile is 1.4 to 2.3 times faster a product and loses where it
+// leaves CUs without one: 784 tiles are four rounds of 256.  Against launches with one tile forced (ten shapes each, 100
+// to 6000 rows, 500 to 50000 classes) the choices were the faster ones or within 10 %: the loss of 512 x 1024 x 32000
+// takes 33 us in 256 x 256 tiles, 39 in 128 x 128 and 49 in 128 x 64; of 299 x 960 x 4333 in fp32 44 us in 128 x 128 and
+// 30 in 128 x 64.
+Cfg cost(int epi, int64_t M, int64_t N, int64_t kt, int np, int tile, int64_t splits) {
+  const Tile t = tile_of(tile, np);
+  const bool out = epi == E_GX || epi == E_GW;
   const int64_t groups = div_up(M, t.bm) * div_up(N, t.bn) * splits;
-  const bool two = !big && np == 1 && groups > kCus;
-  const double step = np == 1 ? (big ? 1.45 : two ? 1.05 : 0.83) * (epi == E_GX || epi == E_GW ? 0.5 : 1) : (big ? 2.2 : 1.5);
-  const double fixed = epi == E_DL ? (big ? 16 : 12) : 7;
-  Cfg c{big, (int)splits, (double)div_up(groups, two ? 2 * kCus : kCus) * ((double)div_up(kt, splits) * step + fixed)};
+  const int64_t beside = std::min(places(tile, np), div_up(groups, kCus));  // workgroups that share a CU
+  static const double kStep[2][3][3] = {{{1.45}, {0.83, 1.05}, {0.55, 0.65, 0.95}}, {{2.2}, {1.5}, {0.85, 1.35}}};
+  const double step = kStep[np == 1 ? 0 : 1][tile][beside - 1] * (np == 1 && out ? 0.5 : 1);
+  static const double kFixed[2][3] = {{7, 7, 5}, {16, 12, 7}};
+  const double fixed = kFixed[epi == E_DL][tile];
+  Cfg c{tile, (int)splits, (double)div_up(groups, beside * kCus) * ((double)div_up(kt, splits) * step + fixed)};
   if (splits > 1) c.us += 5 + (double)splits * (double)N * (double)M * 8 / 4.5e6;
   return c;
 }
 
 Cfg choose(int epi, int64_t M, int64_t N, int64_t kt, int np, int64_t most_splits) {
-  Cfg best = cost(epi, M, N, kt, np, true, 1);
+  const bool out = epi == E_GX || epi == E_GW;
+  Cfg best = cost(epi, M, N, kt, np, T_LARGE, 1);
   const int64_t tiles = div_up(M, 256) * div_up(N, 256);
   for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > most_splits || s * (np == 1 && (epi == E_GX || epi == E_GW) ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
-    for (const bool big : {true, false}) {
-      const Cfg c = cost(epi, M, N, kt, np, big, div_up(kt, div_up(kt, s)));  // no split without a step
+    if (s > most_splits || s * (np == 1 && out ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
+    for (int tile = T_LARGE; tile <= (out ? T_SMALL : T_HALF); ++tile) {
+      const Cfg c = cost(epi, M, N, kt, np, tile, div_up(kt, div_up(kt, s)));  // no split without a step
       if (c.us < best.us) best = c;
     }
   }
@@ -1657,10 +1672,10 @@ struct Cover {
 Cover cover(int epi, int64_t vc, int64_t N, int64_t kt, int np) {
   Cover c;
   c.first = vc, c.a = choose(epi, vc, N, kt, np, 1), c.us = c.a.us;
-  const int64_t tn = div_up(N, tile_of(true, np).bn), rounds = div_up(vc, 256) * tn / kCus;
+  const int64_t tn = div_up(N, tile_of(T_LARGE, np).bn), rounds = div_up(vc, 256) * tn / kCus;
   const int64_t first = rounds * kCus / tn * 256;
   if (first > 0 && first < vc) {
-    const Cfg a = cost(epi, first, N, kt, np, true, 1), b = choose(epi, vc - first, N, kt, np, 1);
+    const Cfg a = cost(epi, first, N, kt, np, T_LARGE, 1), b = choose(epi, vc - first, N, kt, np, 1);
     if (a.us + b.us + 3 < c.us) c.first = first, c.a = a, c.b = b, c.us = a.us + b.us + 3;
   }
   return c;
@@ -1800,12 +1815,12 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
 // ones a CU), each with its share of the tiles.
 template <int EPI, int NP>
 unsigned lay_out(GemmArgs& a, const Cfg& cfg) {
-  const Tile t = tile_of(cfg.big, NP);
+  const Tile t = tile_of(cfg.tile, NP);
   a.tm = div_up(a.M, t.bm), a.tn = div_up(a.N, t.bn);
   a.kt = (int)steps_of(EPI, a.K, NP);
   a.splits = cfg.splits;
   a.per_split = (int)div_up(a.kt, cfg.splits);
-  return (unsigned)std::min(a.tm * a.tn * cfg.splits, !cfg.big && NP == 1 ? 2 * kCus : kCus);
+  return (unsigned)std::min(a.tm * a.tn * cfg.splits, places(cfg.tile, NP) * kCus);
 }
 
 template <int EPI, bool F32>
@@ -1814,8 +1829,17 @@ void mm(GemmArgs a, const Cfg& cfg, hipStream_t st) {
   const dim3 grid(lay_out<EPI, NP>(a, cfg));
   const auto launch = [&](auto soft) {
     constexpr bool SOFT = decltype(soft)::value;
-    if (!cfg.big) hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
-    else if constexpr (F32)
+    if (cfg.tile == T_SMALL) {
+      hipLaunchKernelGGL((k_xent_mm<128, 128, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
+      return;
+    }
+    if constexpr (EPI == E_LSE || EPI == E_DL) {
+      if (cfg.tile == T_HALF) {
+        hipLaunchKernelGGL((k_xent_mm<128, 64, 2, 2, EPI, NP, F32, SOFT>), grid, dim3(256), 0, st, a);
+        return;
+      }
+    }
+    if constexpr (F32)
       hipLaunchKernelGGL((k_xent_mm<256, 128, 4, 2, EPI, NP, F32, SOFT>), grid, dim3(512), 0, st, a);
     else if constexpr (EPI == E_GX)  // the wave's shorter side turned, 16 LDS reads a half-step instead of 20: 5 % faster
       hipLaunchKernelGGL((k_xent_mm<256, 256, 4, 2, EPI, NP, F32, SOFT>), grid, dim3(512), 0, st, a);
@@ -1931,8 +1955,8 @@ void forward(const Plan& p, const Call& c, float* loss, float* stats) {
     const int64_t vc = std::min(piece, p.V - v0);
     operands<F32>(p, c, static_cast<const char*>(c.W) + v0 * p.H * (F32 ? 4 : 2), vc, false, nullptr, nullptr, x, w);
     const Cover cv = cover(E_LSE, vc, p.N, steps_of(E_LSE, std::min(w.K, x.K), p.np), p.np);
-    const int64_t tiles_a = div_up(cv.first, tile_of(cv.a.big, p.np).bm);
-    const int64_t tiles = tiles_a + (cv.first < vc ? div_up(vc - cv.first, tile_of(cv.b.big, p.np).bm) : 0);
+    const int64_t tiles_a = div_up(cv.first, tile_of(cv.a.tile, p.np).bm);
+    const int64_t tiles = tiles_a + (cv.first < vc ? div_up(vc - cv.first, tile_of(cv.b.tile, p.np).bm) : 0);
     for (int64_t at = 0; at < vc; at += cv.first) {
       GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, at == 0 ? cv.first : vc - cv.first);
       a.part = reinterpret_cast<float2*>(c.ws + p.o_part);
@@ -2036,7 +2060,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
       mm<E_DL, F32>(a, one_cfg, c.st);
       if (gb) {
-        const Tile t = tile_of(one_cfg.big, p.np);
+        const Tile t = tile_of(one_cfg.tile, p.np);
         sums.add(1, len, div_up(p.N, t.bn) * t.wn, a.part_b, len, len, scale, static_cast<char*>(gb) + (v0 + at) * SZ, len);
       }
       if (at != 0) break;
@@ -2069,7 +2093,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
         sums.add(vc, p.H, sp, acc_w, p.ldacc, vc * p.ldacc, nullptr, out, p.H);
       }
     }
-    if (gx && gW && !cfg.gx.big && !cfg.gw.big) {
+    if (gx && gW && cfg.gx.tile == T_SMALL && cfg.gw.tile == T_SMALL) {
       mm_both<F32>(to_x, cfg.gx, to_w, cfg.gw, c.st);
     } else {
       if (gx) mm<E_GX, F32>(to_x, cfg.gx, c.st);
