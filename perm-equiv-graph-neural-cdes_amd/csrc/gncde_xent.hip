@@ -221,8 +221,9 @@ struct GemmArgs {
   const float* stats;        // E_DL
   const float* g;
   const float* scale;        // E_DL: dl is stored over it; E_GX, E_GW: the result is multiplied by it (may be NULL: 1)
-  uint16_t* P;               // E_DL: [class / 32][N][part][32], classes zero-padded to mp
+  uint16_t* P;               // E_DL: [class / 32][block][part][32], classes zero-padded to mp
   int64_t mp;
+  int64_t block;             // rows of a block of dl, the rows of x or more
   float* part_b;             // E_DL: [tn * WN][M] sums over this tile's rows of dl (may be NULL)
   // products
   void* out;                 // [N][ldo]
@@ -244,14 +245,14 @@ struct GemmArgs {
 // CU, and 128 x 64 ones (the logits) serve where larger ones leave CUs idle.
 //
 // Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.8 (1.30),
-// gx 6.9 (1.27), gW 7.2 (1.22), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
+// gx 6.6 (1.34), gW 7.3 (1.20), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
 // 0.94.  The logits are bound by power: their matrix units are busy 70 % of the cycles, and the clock falls to 1.65 GHz.
 // The turned products wait for their operands, two LDS reads a fragment instead of one.  Turning W, x and dl in memory
 // instead cost 0.5 ms of copies and 0.8 ms for dl's second form here, a tenth of the gradient at 1021 x 333 x 50021.
 //
 // The one-part products with turned operands (gx, gW) take steps of half that and four buffers (DEEP): their loads are
 // then two to three steps on their way instead of one, and a hand-over leaves those of two steps there (gW 8.6 -> 7.6 ms,
-// gx 7.5 -> 6.9).  dl lies in blocks of 32 classes for that, [class / 32][row][part][32]: a step's rows of it are one run
+// gx 7.5 -> 6.6).  dl lies in blocks of 32 classes for that, [class / 32][row][part][32]: a step's rows of it are one run
 // of memory.  The logits' operands lie as their rows do and would be read in pieces of half a cache line (7.1 -> 7.6 ms).
 template <int NP, bool DEEP>
 struct Step {
@@ -260,7 +261,7 @@ struct Step {
   static constexpr int CH = ROW / 8;              // 16-byte chunks a row
   // A row's chunk c lies at place(c, row): rows that one LDS cycle reads together then differ in bank.
   static __device__ __forceinline__ int place(int c, int row) {
-    return NP == 1 ? (DEEP ? c ^ ((row >> 2) & 3) : c ^ (row & 7)) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
+    return NP == 1 ? (DEEP ? c ^ (-(row >> 2) & 3) : c ^ (row & 7)) : (c & ~3) | ((c & 3) ^ ((row >> 1) & 3));
   }
   // A turned operand's step is K rows of the tile's width times NP values.  Its row k's chunk c lies at c ^ turn(k): the
   // eight rows that one LDS cycle reads 32 bytes each of then cover all banks.
@@ -408,7 +409,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       if (i >= IA && TB) {
         const int at = slot - BM * S::CH, block = at / (32 * S::CH), k = turned_row(i, lane);
         const int c = (at % S::CH) ^ S::turn_dl(k);
-        off[i] = ((uint32_t)(block * a.K + k) * (uint32_t)S::ROW + c * 8) * 2u;
+        off[i] = (((uint32_t)block * (uint32_t)a.block + k) * (uint32_t)S::ROW + c * 8) * 2u;
         continue;
       }
       const int c = S::place(slot - row * S::CH, row);  // place() is its own inverse
@@ -418,7 +419,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     k_from = split_k * a.per_split;
     k_to = k_from + a.per_split < a.kt ? k_from + a.per_split : a.kt;
     base_a = a.A + m0 * (TA ? NP : a.lda);
-    base_b = a.B + n0 * (TB ? (int64_t)a.K * NP : OUT ? S::ROW : a.ldb);
+    base_b = a.B + n0 * (TB ? a.block * NP : OUT ? S::ROW : a.ldb);
   };
 
   auto load = [&](int k, int buf) {
@@ -434,12 +435,12 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       ra = __builtin_amdgcn_make_buffer_rsrc((void*)base_a, 0, bytes, 0x00020000);
     }
     if constexpr (TB) {  // to the end of dl
-      const int64_t all = ((((a.N + 63) / 64 * 64 - n0) / 32) * a.K - (int64_t)k * 32) * S::ROW * 2;
+      const int64_t all = ((((a.N + 63) / 64 * 64 - n0) / 32) * a.block - (int64_t)k * 32) * S::ROW * 2;
       const int64_t most = all < 0xffffffffll ? all : 0xffffffffll;
       rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base_b + (int64_t)k * 32 * S::ROW), 0,
                                              __builtin_amdgcn_readfirstlane(k < k_to ? (int)(uint32_t)most : 0), 0x00020000);
     } else if constexpr (OUT) {
-      rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base_b + (int64_t)k * a.N * S::ROW), 0, bytes, 0x00020000);
+      rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base_b + (int64_t)k * a.block * S::ROW), 0, bytes, 0x00020000);
     } else {
       rb = __builtin_amdgcn_make_buffer_rsrc((void*)base_b, 0, bytes, 0x00020000);
     }
@@ -839,7 +840,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
           const int row = (e >> 2) % HN, c = (e >> 2) / HN * 32 + (e & 3) * 8;
           const int64_t n = n0 + half * HN + row;
           if (n < a.N && m0 + c < a.mp)
-            *reinterpret_cast<u16x8*>(a.P + ((m0 + c) / 32 * a.N + n) * (32 * NP) + s * 32 + (c & 31)) =
+            *reinterpret_cast<u16x8*>(a.P + ((m0 + c) / 32 * a.block + n) * (32 * NP) + s * 32 + (c & 31)) =
                 *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
         }
       }
@@ -1705,6 +1706,9 @@ struct Plan {
   bool f32, direct_ok;  // direct_ok: sizes allow x and W as operands as they lie (the pointers decide too)
   int np;
   int64_t Kp;           // packed contraction of x and W
+  // rows of a block of dl: an odd multiple of 16, so that a tile's blocks do not all start on the same channels (8192
+  // rows: dl and gW 2 to 3 % faster)
+  int64_t block;
   int64_t piece, whole; // classes a piece; the loss's where W is used as it lies
   int64_t bytes = 0;
   // offsets
@@ -1741,6 +1745,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   p.np = p.f32 ? 3 : 1;
   p.direct_ok = !p.f32 && H % 8 == 0;
   p.Kp = up(H, 64);
+  p.block = up(std::max<int64_t>(N, 1), 16) | 16;
   p.small = small_fits(H, V);
   if (p.small) {
     p.o_b = p.take(grad ? 4 * small_groups(N) * (V * H + V) : 0);
@@ -1770,7 +1775,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   }
   const int64_t plane = 2 * p.np;
   // Classes a piece: what the piece puts into the workspace stays within kPieceBytes.
-  const int64_t per_class = plane * p.Kp + (grad ? plane * N : N / 8 + 24);
+  const int64_t per_class = plane * p.Kp + (grad ? plane * p.block : N / 8 + 24);
   const int64_t most = std::max<int64_t>(256, kPieceBytes / per_class / 256 * 256);
   p.piece = std::min(up(V, 256), most);
   p.whole = std::min(up(V, 256), std::max<int64_t>(256, kPieceBytes / (N / 8 + 24) / 256 * 256));
@@ -1800,7 +1805,7 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
     // the last one adds to the sums that the others left
     p.last = rest == vc ? p.full : piece_cfg(N, H, rest, p.np, p.full.gx.splits);
     p.o_scale = p.take(4);
-    p.o_p = p.take(plane * N * up(p.piece, kPad));
+    p.o_p = p.take(plane * p.block * up(p.piece, kPad));
     p.ldacc = up(H, 4);
     p.o_gx = p.take(4 * std::max(p.full.gx.splits, p.last.gx.splits) * N * p.ldacc);
     const int64_t a = p.full.gw.splits > 1 ? p.full.gw.splits * vc : 0;
@@ -2055,7 +2060,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs a = logits_args<F32>(w, x, p, c, v0, at, len);
       a.stats = stats, a.g = g;
       a.scale = scale;
-      a.P = P + p.np * at * p.N, a.mp = at + len < vc ? len : vp - at;
+      a.P = P + p.np * at * p.block, a.block = p.block, a.mp = at + len < vc ? len : vp - at;
       a.part_b = gb ? part_b + bias_rows(p.N) * at : nullptr;
       const Cfg& one_cfg = at == 0 ? cfg.dl.a : cfg.dl.b;
       mm<E_DL, F32>(a, one_cfg, c.st);
@@ -2070,7 +2075,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs& q = to_x;
       q.scale = scale;
       q.A = w.p, q.lda = w.ld, q.M = p.H;
-      q.B = P, q.N = p.N;
+      q.B = P, q.block = p.block, q.N = p.N;
       q.K = (int)vc;
       q.out = gx, q.ldo = p.H;
       // every piece's splits fill the same sums; the last piece may have fewer, and leaves the others as they are
@@ -2083,7 +2088,7 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
       GemmArgs& q = to_w;
       q.scale = scale;
       q.A = x.p, q.lda = x.ld, q.M = p.H;
-      q.B = P, q.N = vc;
+      q.B = P, q.block = p.block, q.N = vc;
       q.K = (int)p.N;
       char* out = static_cast<char*>(gW) + v0 * p.H * SZ;
       q.out = out, q.ldo = p.H;
