@@ -356,7 +356,8 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   constexpr int IA = BM * S::CH / 64 / NW, IT = IA + BN * S::CH / 64 / NW;  // 1 KB loads a wave: A's, then B's
   constexpr bool OUT = EPI == E_GX || EPI == E_GW;
   constexpr bool TA = OUT, TB = EPI == E_GW;  // turned operands
-  static_assert(RT % 4 == 0 && IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH, "chunks divide over the waves");
+  static_assert(RT % 4 == 0 && IA * 64 * NW == BM * S::CH && IT * 64 * NW == (BM + BN) * S::CH,
+                "chunks divide over the waves");
   constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
   uint16_t* const stage = lds + L::HALF;
   // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
@@ -488,7 +489,8 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     if ((NP == 1 || TA || TB) && (k + 1) * S::K > a.K) {  // what lies behind the contraction's end
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const bool behind = (i < IA ? TA : TB) ? k * S::K + turned_row(i, lane) >= a.K : NP == 1 && !OUT && k * S::K + col >= a.K;
+        const bool turned = i < IA ? TA : TB;
+        const bool behind = turned ? k * S::K + turned_row(i, lane) >= a.K : NP == 1 && !OUT && k * S::K + col >= a.K;
         if (behind) *reinterpret_cast<u16x8*>(lds + buf * TILE + place_of(i, lane) * 8) = u16x8{};
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -543,309 +545,309 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   // Puts out the products of tile (m0, n0); info[at] has its rows.
   auto put_out = [&](const int64_t m0, const int64_t n0, const int tile_m, const int tile_n, const int split_k,
                      const int at) {
-  const int tid = fresh(threadIdx.x), lane = tid & 63, fr = lane & 15, fk = lane >> 4;
-  const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
-  const int64_t nb = n0 + wn * (BN / WN) + fr;
+    const int tid = fresh(threadIdx.x), lane = tid & 63, fr = lane & 15, fk = lane >> 4;
+    const int64_t mb = m0 + wm * (BM / WM) + fk * 4;  // first of this lane's four rows of A in tile row 0
+    const int64_t nb = n0 + wn * (BN / WN) + fr;
 
-  if constexpr (OUT) {
-    const float scale = a.scale ? *a.scale : 1.f;
+    if constexpr (OUT) {
+      const float scale = a.scale ? *a.scale : 1.f;
 #pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      const int64_t n = nb + j * 16;
-      if (n >= a.N) continue;
+      for (int j = 0; j < CT; ++j) {
+        const int64_t n = nb + j * 16;
+        if (n >= a.N) continue;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const int64_t m = mb + i * 16;
+          if (m >= a.M) continue;
+          floatx4 v = acc[i][j] * scale;
+          if (a.acc) {
+            floatx4* p = reinterpret_cast<floatx4*>(a.acc + ((int64_t)split_k * a.N + n) * a.ldacc + m);
+            if (a.add) v += *p;
+            *p = v;
+          } else if (F32) {
+            put<true>(static_cast<float*>(a.out) + n * a.ldo, m, a.M, v);
+          } else {
+            put<false>(static_cast<uint16_t*>(a.out) + n * a.ldo, m, a.M, v);
+          }
+        }
+      }
+      return;
+    }
+
+    // logits: the bias, and classes behind the last at -inf
+    if (a.bias) {
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        const int64_t m = mb + i * 16;
-        if (m >= a.M) continue;
-        floatx4 v = acc[i][j] * scale;
-        if (a.acc) {
-          floatx4* p = reinterpret_cast<floatx4*>(a.acc + ((int64_t)split_k * a.N + n) * a.ldacc + m);
-          if (a.add) v += *p;
-          *p = v;
-        } else if (F32) {
-          put<true>(static_cast<float*>(a.out) + n * a.ldo, m, a.M, v);
-        } else {
-          put<false>(static_cast<uint16_t*>(a.out) + n * a.ldo, m, a.M, v);
+        const floatx4 bv = *reinterpret_cast<const floatx4*>(bias + at * BIAS + wm * (BM / WM) + fk * 4 + i * 16);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) acc[i][j] += bv;
+      }
+    }
+    if (m0 + BM > a.M) {
+      const int left = (int)(a.M - mb);  // of this lane's rows of A
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool in = i * 16 + q < left;
+#pragma unroll
+          for (int j = 0; j < CT; ++j) acc[i][j][q] = in ? acc[i][j][q] : -INFINITY;
         }
-      }
     }
-    return;
-  }
 
-  // logits: the bias, and classes behind the last at -inf
-  if (a.bias) {
+    // Hands use(i, y) the label row's values beside acc[i][j], four i at a time on their way (more would take registers
+    // that are not there); of a row that is not `in`, another's.
+    auto labels = [&](int j, bool in, auto use) {
+      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+      const float* row = static_cast<const float*>(a.rows.target) + (in ? nb + j * 16 : 0) * a.V + a.v0 + mb;
+      if (m0 + BM <= a.M) {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const floatx4 bv = *reinterpret_cast<const floatx4*>(bias + at * BIAS + wm * (BM / WM) + fk * 4 + i * 16);
+        for (int i0 = 0; i0 < RT; i0 += 4) {
+          f32x4 y[4];
 #pragma unroll
-      for (int j = 0; j < CT; ++j) acc[i][j] += bv;
-    }
-  }
-  if (m0 + BM > a.M) {
-    const int left = (int)(a.M - mb);  // of this lane's rows of A
+          for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const f32x4*>(row + (i0 + i) * 16);
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool in = i * 16 + q < left;
-#pragma unroll
-        for (int j = 0; j < CT; ++j) acc[i][j][q] = in ? acc[i][j][q] : -INFINITY;
+          for (int i = 0; i < 4; ++i) use(i0 + i, floatx4{y[i][0], y[i][1], y[i][2], y[i][3]});
+        }
+        return;
       }
-  }
-
-  // Hands use(i, y) the label row's values beside acc[i][j], four i at a time on their way (more would take registers
-  // that are not there); of a row that is not `in`, another's.
-  auto labels = [&](int j, bool in, auto use) {
-    typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-    const float* row = static_cast<const float*>(a.rows.target) + (in ? nb + j * 16 : 0) * a.V + a.v0 + mb;
-    if (m0 + BM <= a.M) {
+      const int left = fresh((int)(a.M - mb));  // of this lane's classes
+      if (a.V < 4) {
+        floatx4 y;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q] = q < left ? row[q] : 0.f;
+        use(0, y);
+        return;
+      }
+      // four values that end with the piece's last one where they would go beyond it, moved to their places
 #pragma unroll
       for (int i0 = 0; i0 < RT; i0 += 4) {
-        f32x4 y[4];
+        f32x4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const f32x4*>(row + (i0 + i) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) use(i0 + i, floatx4{y[i][0], y[i][1], y[i][2], y[i][3]});
-      }
-      return;
-    }
-    const int left = fresh((int)(a.M - mb));  // of this lane's classes
-    if (a.V < 4) {
-      floatx4 y;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) y[q] = q < left ? row[q] : 0.f;
-      use(0, y);
-      return;
-    }
-    // four values that end with the piece's last one where they would go beyond it, moved to their places
-#pragma unroll
-    for (int i0 = 0; i0 < RT; i0 += 4) {
-      f32x4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int from = (i0 + i) * 16;
-        v[i] = *reinterpret_cast<const f32x4*>(row + (from < left - 4 ? from : left - 4));
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int by = (i0 + i) * 16 - (left - 4);
-        floatx4 y = floatx4{v[i][0], v[i][1], v[i][2], v[i][3]};
-        if (__any(by > 0)) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float s = by <= 0 ? v[i][q] : 0.f;
-#pragma unroll
-            for (int k = 1; q + k < 4; ++k) s = by == k ? v[i][q + k] : s;
-            y[q] = s;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int from = (i0 + i) * 16;
+          v[i] = *reinterpret_cast<const f32x4*>(row + (from < left - 4 ? from : left - 4));
         }
-        use(i0 + i, y);
-      }
-    }
-  };
-
-  if constexpr (EPI == E_LSE) {
-    float* sm = reinterpret_cast<float*>(stage);  // [4][WM][BN]
-    float top[CT], sum[CT], dot[CT] = {}, mass[CT] = {};
-    if constexpr (SOFT) {
 #pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
-        labels(j, in, [&](int i, floatx4 y) {
+        for (int i = 0; i < 4; ++i) {
+          const int by = (i0 + i) * 16 - (left - 4);
+          floatx4 y = floatx4{v[i][0], v[i][1], v[i][2], v[i][3]};
+          if (__any(by > 0)) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float v = in ? y[q] : 0.f;
-            mass[j] += v;
-            dot[j] += v == 0.f ? 0.f : v * acc[i][j][q];  // a class at -inf without mass adds nothing
+            for (int q = 0; q < 4; ++q) {
+              float s = by <= 0 ? v[i][q] : 0.f;
+#pragma unroll
+              for (int k = 1; q + k < 4; ++k) s = by == k ? v[i][q + k] : s;
+              y[q] = s;
+            }
           }
-        });
+          use(i0 + i, y);
+        }
       }
-#pragma unroll
-      for (int d = 16; d < 64; d <<= 1)
+    };
+
+    if constexpr (EPI == E_LSE) {
+      float* sm = reinterpret_cast<float*>(stage);  // [4][WM][BN]
+      float top[CT], sum[CT], dot[CT] = {}, mass[CT] = {};
+      if constexpr (SOFT) {
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          dot[j] += __shfl_xor(dot[j], d);
-          mass[j] += __shfl_xor(mass[j], d);
+          const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+          labels(j, in, [&](int i, floatx4 y) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float v = in ? y[q] : 0.f;
+              mass[j] += v;
+              dot[j] += v == 0.f ? 0.f : v * acc[i][j][q];  // a class at -inf without mass adds nothing
+            }
+          });
         }
-    }
 #pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      top[j] = -INFINITY, sum[j] = 0.f;
+        for (int d = 16; d < 64; d <<= 1)
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) top[j] = fmaxf(top[j], acc[i][j][q]);
-    }
-#pragma unroll
-    for (int d = 16; d < 64; d <<= 1) {
-      float other[CT];
-#pragma unroll
-      for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(top[j], d);
-#pragma unroll
-      for (int j = 0; j < CT; ++j) top[j] = fmaxf(top[j], other[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      const float off2 = top[j] == -INFINITY ? 0.f : -top[j] * kLog2e;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
-      sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
-    }
-    if constexpr (!SOFT) {
+          for (int j = 0; j < CT; ++j) {
+            dot[j] += __shfl_xor(dot[j], d);
+            mass[j] += __shfl_xor(mass[j], d);
+          }
+      }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
-        const int target = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
-        if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (target >= 0 && t == i * 16 + q) a.hit[nb + j * 16] = acc[i][j][q];
-        }
-      }
-    }
-#pragma unroll
-    for (int d = 16; d < 64; d <<= 1) {
-      float other[CT];
-#pragma unroll
-      for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(sum[j], d);
-#pragma unroll
-      for (int j = 0; j < CT; ++j) sum[j] += other[j];
-    }
-    if (fk == 0) {
-#pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const int c = wn * (BN / WN) + j * 16 + fr;
-        sm[wm * BN + c] = top[j];
-        sm[(WM + wm) * BN + c] = sum[j];
-        sm[(2 * WM + wm) * BN + c] = dot[j];
-        sm[(3 * WM + wm) * BN + c] = mass[j];
-      }
-    }
-    __syncthreads();
-    for (int col = tid; col < BN; col += NW * 64) {
-      if (n0 + col >= a.N) break;
-      float top = sm[col];
-#pragma unroll
-      for (int w = 1; w < WM; ++w) top = fmaxf(top, sm[w * BN + col]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, dot = 0.f, mass = 0.f;
-#pragma unroll
-      for (int w = 0; w < WM; ++w) {
-        const float tw = sm[w * BN + col];
-        sum += sm[(WM + w) * BN + col] * (tw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((tw - ref) * kLog2e));
-        dot += sm[(2 * WM + w) * BN + col];
-        mass += sm[(3 * WM + w) * BN + col];
-      }
-      a.part[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(top, sum);
-      if (SOFT) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
-    }
-    return;
-  }
-
-  if constexpr (EPI == E_DL) {
-#pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
-      const int target = __float_as_int(row[3]);
-      const float off2 = row[0], gv = row[1], gs = row[2];
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
-      if constexpr (!SOFT) {
-        const int t = target - (int)mb;
-        if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[i][j][q] -= target >= 0 && t == i * 16 + q ? gv : 0.f;
-        }
-      }
-    }
-    if constexpr (SOFT) {
-#pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(acc[i][j]));  // the exponentials first: not the labels wait
-        labels(j, __float_as_int(row[3]) != kLeftOut, [&](int i, floatx4 y) {
-          acc[i][j] -= row[1] * y;
-          asm volatile("" : "+v"(acc[i][j]));
-        });
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
-      if (!__all(in)) {  // rows left out, whatever their logits
+        top[j] = -INFINITY, sum[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = in ? acc[i][j][q] : 0.f;
+          for (int q = 0; q < 4; ++q) top[j] = fmaxf(top[j], acc[i][j][q]);
       }
-    }
-    if (m0 + BM > a.M) {  // classes behind the last: an lse of NaN must not reach them
-      const int left = (int)(a.M - mb);
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
+      for (int d = 16; d < 64; d <<= 1) {
+        float other[CT];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(top[j], d);
 #pragma unroll
-          for (int j = 0; j < CT; ++j) acc[i][j][q] = i * 16 + q < left ? acc[i][j][q] : 0.f;
-    }
-    if (a.part_b) {
+        for (int j = 0; j < CT; ++j) top[j] = fmaxf(top[j], other[j]);
+      }
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        floatx4 s = acc[i][0];
+      for (int j = 0; j < CT; ++j) {
+        const float off2 = top[j] == -INFINITY ? 0.f : -top[j] * kLog2e;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 1; j < CT; ++j) s += acc[i][j];
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float r = sum16(s[q]);
-          const int64_t m = mb + i * 16 + q;
-          if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = r;
+          for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+        sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
+      }
+      if constexpr (!SOFT) {
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          const int target = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
+          if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (target >= 0 && t == i * 16 + q) a.hit[nb + j * 16] = acc[i][j][q];
+          }
         }
       }
+#pragma unroll
+      for (int d = 16; d < 64; d <<= 1) {
+        float other[CT];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) other[j] = __shfl_xor(sum[j], d);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) sum[j] += other[j];
+      }
+      if (fk == 0) {
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          const int c = wn * (BN / WN) + j * 16 + fr;
+          sm[wm * BN + c] = top[j];
+          sm[(WM + wm) * BN + c] = sum[j];
+          sm[(2 * WM + wm) * BN + c] = dot[j];
+          sm[(3 * WM + wm) * BN + c] = mass[j];
+        }
+      }
+      __syncthreads();
+      for (int col = tid; col < BN; col += NW * 64) {
+        if (n0 + col >= a.N) break;
+        float top = sm[col];
+#pragma unroll
+        for (int w = 1; w < WM; ++w) top = fmaxf(top, sm[w * BN + col]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, dot = 0.f, mass = 0.f;
+#pragma unroll
+        for (int w = 0; w < WM; ++w) {
+          const float tw = sm[w * BN + col];
+          sum += sm[(WM + w) * BN + col] * (tw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((tw - ref) * kLog2e));
+          dot += sm[(2 * WM + w) * BN + col];
+          mass += sm[(3 * WM + w) * BN + col];
+        }
+        a.part[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(top, sum);
+        if (SOFT) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
+      }
+      return;
     }
-    // dl goes out through LDS in whole 16-byte chunks: from the registers it would be 8-byte pieces of 16 rows.
-    constexpr int THREADS = NW * 64, HN = BN / HALVES;
-    const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
+
+    if constexpr (EPI == E_DL) {
 #pragma unroll
-    for (int s = 0; s < NP; ++s) {
+      for (int j = 0; j < CT; ++j) {
+        const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
+        const int target = __float_as_int(row[3]);
+        const float off2 = row[0], gv = row[1], gs = row[2];
 #pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        if (s + half > 0) lds_barrier();
-        if (wn * (BN / WN) / HN == half) {
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int j = 0; j < CT; ++j)
+          for (int q = 0; q < 4; ++q)
+            acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+        if constexpr (!SOFT) {
+          const int t = target - (int)mb;
+          if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              u16x4 part;
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                part[q] = to_bf16(acc[i][j][q]);
-                if (NP > 1) acc[i][j][q] -= from_bf16(part[q]);  // what the next part holds
+              for (int q = 0; q < 4; ++q) acc[i][j][q] -= target >= 0 && t == i * 16 + q ? gv : 0.f;
+          }
+        }
+      }
+      if constexpr (SOFT) {
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
+#pragma unroll
+          for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(acc[i][j]));  // the exponentials first: not the labels wait
+          labels(j, __float_as_int(row[3]) != kLeftOut, [&](int i, floatx4 y) {
+            acc[i][j] -= row[1] * y;
+            asm volatile("" : "+v"(acc[i][j]));
+          });
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+        if (!__all(in)) {  // rows left out, whatever their logits
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] = in ? acc[i][j][q] : 0.f;
+        }
+      }
+      if (m0 + BM > a.M) {  // classes behind the last: an lse of NaN must not reach them
+        const int left = (int)(a.M - mb);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) acc[i][j][q] = i * 16 + q < left ? acc[i][j][q] : 0.f;
+      }
+      if (a.part_b) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          floatx4 s = acc[i][0];
+#pragma unroll
+          for (int j = 1; j < CT; ++j) s += acc[i][j];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float r = sum16(s[q]);
+            const int64_t m = mb + i * 16 + q;
+            if (fr == 0 && m < a.M) a.part_b[(int64_t)(tile_n * WN + wn) * a.M + m] = r;
+          }
+        }
+      }
+      // dl goes out through LDS in whole 16-byte chunks: from the registers it would be 8-byte pieces of 16 rows.
+      constexpr int THREADS = NW * 64, HN = BN / HALVES;
+      const int lm = wm * (BM / WM) + fk * 4, ln = wn * (BN / WN) + fr;
+#pragma unroll
+      for (int s = 0; s < NP; ++s) {
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          if (s + half > 0) lds_barrier();
+          if (wn * (BN / WN) / HN == half) {
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+#pragma unroll
+              for (int i = 0; i < RT; ++i) {
+                u16x4 part;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  part[q] = to_bf16(acc[i][j][q]);
+                  if (NP > 1) acc[i][j][q] -= from_bf16(part[q]);  // what the next part holds
+                }
+                *reinterpret_cast<u16x4*>(stage + (ln - half * HN + j * 16) * (BM + PAD) + lm + i * 16) = part;
               }
-              *reinterpret_cast<u16x4*>(stage + (ln - half * HN + j * 16) * (BM + PAD) + lm + i * 16) = part;
-            }
-        }
-        lds_barrier();
+          }
+          lds_barrier();
 #pragma unroll 2
-        for (int e = tid; e < HN * (BM / 8); e += THREADS) {  // 16 rows of a block a wave: 1 KB
-          const int row = (e >> 2) % HN, c = (e >> 2) / HN * 32 + (e & 3) * 8;
-          const int64_t n = n0 + half * HN + row;
-          if (n < a.N && m0 + c < a.mp)
-            *reinterpret_cast<u16x8*>(a.P + ((m0 + c) / 32 * a.block + n) * (32 * NP) + s * 32 + (c & 31)) =
-                *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
+          for (int e = tid; e < HN * (BM / 8); e += THREADS) {  // 16 rows of a block a wave: 1 KB
+            const int row = (e >> 2) % HN, c = (e >> 2) / HN * 32 + (e & 3) * 8;
+            const int64_t n = n0 + half * HN + row;
+            if (n < a.N && m0 + c < a.mp)
+              *reinterpret_cast<u16x8*>(a.P + ((m0 + c) / 32 * a.block + n) * (32 * NP) + s * 32 + (c & 31)) =
+                  *reinterpret_cast<const u16x8*>(stage + row * (BM + PAD) + c);
+          }
         }
       }
     }
-  }
   };
 
   take(first);
@@ -855,81 +857,81 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   int at = 0;
   for (uint32_t bid = first; bid < all; bid += step, at ^= 1) {
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  if (k_from < k_to) {
-    hand_over(k_from, 0, None());
-    if (!DEEP) load(k_from + 1, 1);
-    if constexpr (DEEP) {
-      load(k_from + 2, 2);
-      load(k_from + 3, 3);
-      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
-      read(0, 0, fa0, fb0);
-      // step k's products; step k + 1 is read and step k + 4 sent for
-      auto go = [&](int k, const bf16x8(&fa)[RT], const bf16x8(&fb)[CT], bf16x8(&na)[RT], bf16x8(&nb)[CT]) {
-        const int buf = (k - k_from) & 3;
-        hand_over(k + 1, (buf + 1) & 3, std::integral_constant<int, 2 * IT>());
-        read(0, (buf + 1) & 3, na, nb);  // behind the last step: what lies there, never multiplied
-        load(k + 4, buf);
-        multiply(fa, fb);
-        interleave<RT * CT, READS, IT, EARLY>();
-      };
-      for (int k = k_from; k < k_to; k += 2) {
-        go(k, fa0, fb0, fa1, fb1);
-        if (k + 1 < k_to) go(k + 1, fa1, fb1, fa0, fb0);
-      }
-    } else if constexpr (NP == 1) {
-      bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
-      read(0, 0, fa0, fb0);
-      for (int k = k_from; k < k_to; ++k) {
-        const int buf = (k - k_from) & 1;
-        read(1, buf, fa1, fb1);
-        multiply(fa0, fb0);
-        interleave<RT * CT, READS, 0, EARLY>();
-        hand_over(k + 1, buf ^ 1, None());
-        if (EARLY) load(k + 2, buf);
-        read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
-        if (!EARLY) load(k + 2, buf);
-        multiply(fa1, fb1);
-        interleave<RT * CT, READS, IT, EARLY>();
-      }
-    } else {
-      bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
-      read(1, 0, ma, mb);
-      for (int k = k_from; k < k_to; ++k) {
-        const int buf = (k - k_from) & 1;
-        read(0, buf, ha, hb);
-        multiply(ma, mb);
-        interleave<RT * CT, READS, 0, EARLY>();
-        read(2, buf, sa, sb);
-        multiply(ma, hb);
-        multiply(ha, mb);
-        interleave<2 * RT * CT, READS, 0, EARLY>();
-        hand_over(k + 1, buf ^ 1, None());
-        if (EARLY) load(k + 2, buf);
-        read(1, buf ^ 1, ma, mb);
-        if (!EARLY) load(k + 2, buf);
-        multiply(sa, hb);
-        multiply(ha, sb);
-        multiply(ha, hb);
-        interleave<3 * RT * CT, READS, IT, EARLY>();
+      for (int j = 0; j < CT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (k_from < k_to) {
+      hand_over(k_from, 0, None());
+      if (!DEEP) load(k_from + 1, 1);
+      if constexpr (DEEP) {
+        load(k_from + 2, 2);
+        load(k_from + 3, 3);
+        bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
+        read(0, 0, fa0, fb0);
+        // step k's products; step k + 1 is read and step k + 4 sent for
+        auto go = [&](int k, const bf16x8(&fa)[RT], const bf16x8(&fb)[CT], bf16x8(&na)[RT], bf16x8(&nb)[CT]) {
+          const int buf = (k - k_from) & 3;
+          hand_over(k + 1, (buf + 1) & 3, std::integral_constant<int, 2 * IT>());
+          read(0, (buf + 1) & 3, na, nb);  // behind the last step: what lies there, never multiplied
+          load(k + 4, buf);
+          multiply(fa, fb);
+          interleave<RT * CT, READS, IT, EARLY>();
+        };
+        for (int k = k_from; k < k_to; k += 2) {
+          go(k, fa0, fb0, fa1, fb1);
+          if (k + 1 < k_to) go(k + 1, fa1, fb1, fa0, fb0);
+        }
+      } else if constexpr (NP == 1) {
+        bf16x8 fa0[RT], fb0[CT], fa1[RT], fb1[CT];
+        read(0, 0, fa0, fb0);
+        for (int k = k_from; k < k_to; ++k) {
+          const int buf = (k - k_from) & 1;
+          read(1, buf, fa1, fb1);
+          multiply(fa0, fb0);
+          interleave<RT * CT, READS, 0, EARLY>();
+          hand_over(k + 1, buf ^ 1, None());
+          if (EARLY) load(k + 2, buf);
+          read(0, buf ^ 1, fa0, fb0);  // behind the last step: what lies there, never multiplied
+          if (!EARLY) load(k + 2, buf);
+          multiply(fa1, fb1);
+          interleave<RT * CT, READS, IT, EARLY>();
+        }
+      } else {
+        bf16x8 ha[RT], hb[CT], ma[RT], mb[CT], sa[RT], sb[CT];
+        read(1, 0, ma, mb);
+        for (int k = k_from; k < k_to; ++k) {
+          const int buf = (k - k_from) & 1;
+          read(0, buf, ha, hb);
+          multiply(ma, mb);
+          interleave<RT * CT, READS, 0, EARLY>();
+          read(2, buf, sa, sb);
+          multiply(ma, hb);
+          multiply(ha, mb);
+          interleave<2 * RT * CT, READS, 0, EARLY>();
+          hand_over(k + 1, buf ^ 1, None());
+          if (EARLY) load(k + 2, buf);
+          read(1, buf ^ 1, ma, mb);
+          if (!EARLY) load(k + 2, buf);
+          multiply(sa, hb);
+          multiply(ha, sb);
+          multiply(ha, hb);
+          interleave<3 * RT * CT, READS, IT, EARLY>();
+        }
       }
     }
-  }
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  __syncthreads();
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __syncthreads();
 
-  // The next tile's first operands and rows are on their way while this one's products are put out.
-  const int64_t m0_now = m0, n0_now = n0;
-  const int tm_now = tile_m, tn_now = tile_n, split_now = split_k;
-  if (bid + step < all) {
-    take(bid + step);
-    if (k_from < k_to) load(k_from, 0);
-    if (DEEP && k_from < k_to) load(k_from + 1, 1);
-    fetch_rows(at ^ 1);
-  }
-  put_out(m0_now, n0_now, tm_now, tn_now, split_now, at);
+    // The next tile's first operands and rows are on their way while this one's products are put out.
+    const int64_t m0_now = m0, n0_now = n0;
+    const int tm_now = tile_m, tn_now = tile_n, split_now = split_k;
+    if (bid + step < all) {
+      take(bid + step);
+      if (k_from < k_to) load(k_from, 0);
+      if (DEEP && k_from < k_to) load(k_from + 1, 1);
+      fetch_rows(at ^ 1);
+    }
+    put_out(m0_now, n0_now, tm_now, tn_now, split_now, at);
   }
 }
 
@@ -1616,10 +1618,15 @@ Tile tile_of(int tile, int np) {
 }
 
 // Workgroups of a tile that a CU holds at once, by their LDS.
-int64_t places(int tile, int np) { return tile == T_LARGE || (tile == T_SMALL && np == 3) ? 1 : np == 1 && tile == T_HALF ? 3 : 2; }
+int64_t places(int tile, int np) {
+  if (tile == T_LARGE) return 1;
+  return (tile == T_HALF ? 2 : 1) + (np == 1 ? 1 : 0);
+}
 
 
-int64_t steps_of(int epi, int64_t K, int np) { return np == 1 ? div_up(K, epi == E_GX || epi == E_GW ? 32 : 64) : up(K, kPad) / 32; }
+int64_t steps_of(int epi, int64_t K, int np) {
+  return np == 1 ? div_up(K, epi == E_GX || epi == E_GW ? 32 : 64) : up(K, kPad) / 32;
+}
 
 struct Cfg {
   int tile = T_LARGE;
