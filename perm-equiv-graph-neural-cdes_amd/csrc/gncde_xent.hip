@@ -1732,7 +1732,7 @@ struct Plan {
 };
 
 // Workgroups of the small gradient: one for each CU, each with its share of the row tiles and one part of gW.
-int64_t small_groups(int64_t N) { return std::min(div_up(std::max<int64_t>(N, 1), 16), kCus); }
+int64_t small_groups(int64_t N) { return std::min(div_up(N, 16), kCus); }
 
 // Rows of the bias's sums: tile columns times waves across, of either tile size.
 int64_t bias_rows(int64_t N) { return 4 * div_up(N, 128); }
@@ -1752,13 +1752,17 @@ bool make_plan(int64_t N, int64_t H, int64_t V, int32_t dtype, bool grad, Plan& 
   p.np = p.f32 ? 3 : 1;
   p.direct_ok = !p.f32 && H % 8 == 0;
   p.Kp = up(H, 64);
-  p.block = up(std::max<int64_t>(N, 1), 16) | 16;
+  p.block = up(N, 16) | 16;
+  if (N == 0) {  // nothing to plan: the gradient writes zeros
+    p.take(0);
+    return true;
+  }
   p.small = small_fits(H, V);
   if (p.small) {
     p.o_b = p.take(grad ? 4 * small_groups(N) * (V * H + V) : 0);
     return true;
   }
-  if (N > 0 && N <= kFewRows) {
+  if (N <= kFewRows) {
     const int64_t sz = p.f32 ? 4 : 2, step = p.f32 ? 16 : 32;
     const int64_t xs = up(H, step) + 16 / sz;  // rows of x start in different banks
     if (N * xs * sz <= kFewLds) {
