@@ -54,6 +54,16 @@ __device__ __forceinline__ void split(float x, uint16_t (&p)[NP]) {
   }
 }
 
+// exp(l - top) as exp2(l by + off), one fused product a logit.  From 2^31 on, where off rounds by more than the exponential
+// takes and ends past fp32's range, logits lie at least 128 apart: their difference as the exponent of two tells equal ones
+// from smaller ones just as well.
+struct Exponent {
+  float by, off;
+  __device__ __forceinline__ static bool far(float top) { return fabsf(top) >= 0x1p31f && fabsf(top) < INFINITY; }
+  __device__ __forceinline__ explicit Exponent(float top)
+      : by(far(top) ? 1.f : kLog2e), off(top == -INFINITY ? 0.f : -top * by) {}
+};
+
 // ---- targets and rows left out ----------------------------------------------------------------------------------
 struct Rows {
   const void* target;
@@ -200,6 +210,11 @@ __global__ void __launch_bounds__(256) k_xent_pack(PackJob x, PackJob w, int H, 
 // ---- the product ------------------------------------------------------------------------------------------------
 enum { E_LSE = 0, E_DL = 1, E_GX = 2, E_GW = 3 };
 constexpr int kLeftOut = -2;
+
+// A row's target within the piece (-1: none there; kLeftOut) and whether its logits are far, in one word.
+__device__ __forceinline__ float row_word(int target, bool far) { return __int_as_float((target + 2) | (far ? 1 << 30 : 0)); }
+__device__ __forceinline__ int word_target(float w) { return (__float_as_int(w) & ~(1 << 30)) - 2; }
+__device__ __forceinline__ bool word_far(float w) { return __float_as_int(w) & (1 << 30); }
 
 struct GemmArgs {
   const uint16_t* A;
@@ -360,8 +375,8 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
                 "chunks divide over the waves");
   constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
   uint16_t* const stage = lds + L::HALF;
-  // What the logits' epilogues need of a row of x: -lse log2 e, g over the scale, the same times S, and the target's
-  // class within the piece (-1: none there; kLeftOut).  Fetched with the tile's first operands, one tile ahead.
+  // What the logits' epilogues need of a row of x: lse's Exponent, g over the scale, the same times S, and the row's word.
+  // Fetched with the tile's first operands, one tile ahead.
   floatx4* const info = reinterpret_cast<floatx4*>(lds + BUFS);
   float* const bias = reinterpret_cast<float*>(lds + BUFS + 2 * INFO * 8);  // of the tile's classes, likewise
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -471,12 +486,12 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         if (EPI == E_DL) {
           const float lse = a.stats[2 * n], mass = a.stats[2 * n + 1];
           const float gv = a.g[n] / (a.scale ? *a.scale : 1.f);
-          v = floatx4{-lse * kLog2e, gv, gv * mass, 0.f};
+          v = floatx4{Exponent(lse).off, gv, gv * mass, lse};
         }
         const bool in = n0 + r < a.N && kept && c >= 0;
         const int64_t t = c - a.v0;
         if (!in) v = floatx4{0.f, 0.f, 0.f, 0.f};
-        v[3] = __int_as_float(!in ? kLeftOut : !SOFT && t >= 0 && t < a.M ? (int)t : -1);
+        v[3] = row_word(!in ? kLeftOut : !SOFT && t >= 0 && t < a.M ? (int)t : -1, Exponent::far(v[3]));
         info[at * INFO + r] = v;
       }
     }
@@ -652,7 +667,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       if constexpr (SOFT) {
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+          const bool in = word_target(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
           labels(j, in, [&](int i, floatx4 y) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -688,18 +703,18 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
-        const float off2 = top[j] == -INFINITY ? 0.f : -top[j] * kLog2e;
+        const Exponent e(top[j]);
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+          for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], e.by, e.off));
         sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
       }
       if constexpr (!SOFT) {
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          const int target = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
+          const int target = word_target(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]), t = target - (int)mb;
           if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
 #pragma unroll
             for (int i = 0; i < RT; ++i)
@@ -752,13 +767,13 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
         const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
-        const int target = __float_as_int(row[3]);
-        const float off2 = row[0], gv = row[1], gs = row[2];
+        const int target = word_target(row[3]);
+        const float by = word_far(row[3]) ? 1.f : kLog2e, off = row[0], gv = row[1], gs = row[2];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], kLog2e, off2));
+            acc[i][j][q] = gs * __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], by, off));
         if constexpr (!SOFT) {
           const int t = target - (int)mb;
           if (__any(target >= 0 && t >= 0 && t < RT * 16)) {  // few tiles hold a target
@@ -775,7 +790,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
           const floatx4 row = info[at * INFO + wn * (BN / WN) + j * 16 + fr];
 #pragma unroll
           for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(acc[i][j]));  // the exponentials first: not the labels wait
-          labels(j, __float_as_int(row[3]) != kLeftOut, [&](int i, floatx4 y) {
+          labels(j, word_target(row[3]) != kLeftOut, [&](int i, floatx4 y) {
             acc[i][j] -= row[1] * y;
             asm volatile("" : "+v"(acc[i][j]));
           });
@@ -783,7 +798,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
-        const bool in = __float_as_int(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+        const bool in = word_target(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
         if (!__all(in)) {  // rows left out, whatever their logits
 #pragma unroll
           for (int i = 0; i < RT; ++i)

@@ -1,0 +1,72 @@
+"""The read-out's cross-entropy where every logit is a whole number that all its sums hold exactly: what is left is the
+softmax, far from zero.
+
+Inputs: x and W whole numbers up to 3, W for a few of the hidden values only, the bias a constant B and whole numbers up to
+8: |l - B| <= D, every partial sum a whole number below 2^24, exact in any order and in either type.  With the logits exact,
+u = 2^-24:
+  exponent's argument  (l - top) log2 e within 2 u of itself, l - top and top - lse' being exact or rounded once
+  sum of exponentials  relative error <= (4 D + 4 + 256) u: the arguments', the exponential's own (2 u each time it is
+                       taken, twice here) and those of 256 additions; an error as large in its logarithm
+  loss                 S times that, + (V / 64 + 64) u sum |y| (top - l), + half a step of the largest term: nothing that
+                       grows with B
+  dl                   |g| S p times the above, once for the sum and once for the exponential, + 4 u (|g| S p + |g y|)
+  gb                   fp32: the sums' (R + 64) u sum |dl| more, and half a step of its type
+A loss that subtracts two numbers of B's size is off by u B = 2^-8 at B = 65536, a thousand times the bound."""
+import pytest
+import torch
+
+from gncde import engine
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def make(rows, hidden, classes, dtype, kind, base, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=g, device="cuda").float()
+
+    W = whole(-3, 3, classes, hidden)
+    W[:, 4:] = 0
+    c = {"x": whole(-3, 3, rows, hidden), "W": W, "b": base * torch.ones(classes, device="cuda")}
+    # bf16 holds 65536 and 1024 and few numbers beside them: the small part of the bias goes into a hidden value of one
+    c["x"][:, 0] = 1
+    c["W"][:, 0] = whole(-8, 8, classes)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    c["x"][::2, 1:4] = c["W"][t[::2], 1:4].sign() * 3  # every other row is fairly sure of its class
+    if kind == "rows":
+        y = torch.rand(rows, classes, generator=g, device="cuda") ** 8
+        y *= torch.rand(rows, 1, generator=g, device="cuda") * 2 / y.sum(1, keepdim=True)
+        y[::2] = 0
+        y[torch.arange(0, rows, 2, device="cuda"), t[::2]] = 1.0
+        t = y
+    c = {k: v.to(dtype) for k, v in c.items()}
+    c["t"], c["g"] = t, torch.rand(rows, generator=g, device="cuda") * 2 - 0.5
+    return c
+
+
+CASES = [(40, 8, 30), (300, 32, 255),                       # few classes
+         (1, 40, 700), (5, 300, 700), (16, 64, 5000),      # few rows
+         (40, 136, 513), (300, 64, 2000), (700, 200, 9001)]  # tiles
+
+
+@pytest.mark.parametrize("base", [0.0, 1024.0, -65536.0, 65536.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["i64", "rows"])
+@pytest.mark.parametrize("size", CASES)
+def test_loss_far_from_zero(size, kind, dtype, base):
+    c = make(*size, dtype, kind, base)
+    R, H, V = size
+    l = c["x"].double() @ c["W"].double().T + c["b"].double()
+    assert bool((l == l.round()).all()) and float(l.abs().max()) < 2 ** 17
+    y = c["t"].double() if kind == "rows" else torch.zeros_like(l).scatter_(1, c["t"][:, None], 1.0)
+    S, top = y.sum(1), l.amax(1, keepdim=True)
+    D = float((top - l).max())
+    d_log = (4 * D + 260) * U
+    want = S * torch.logsumexp(l - top, 1) + (y * (top - l)).sum(1)
+    tol = S * d_log + (V / 64 + 64) * U * (y * (top - l)).sum(1) + U * (S * torch.logsumexp(l - top, 1) + want)
+    loss, _ = engine.linear_cross_entropy(c["x"], c["W"], c["b"], c["t"])
+    off = (loss.double() - want).abs()
+    assert bool((off <= tol).all()), f"{float((off / tol).max()):.3g} of the bound"
+    assert bool((loss >= 0).all())
