@@ -54,15 +54,31 @@ __device__ __forceinline__ void split(float x, uint16_t (&p)[NP]) {
   }
 }
 
-// exp(l - top) as exp2(l by + off), one fused product a logit.  From 2^31 on, where off rounds by more than the exponential
-// takes and ends past fp32's range, logits lie at least 128 apart: their difference as the exponent of two tells equal ones
-// from smaller ones just as well.
+// ---- logits far from zero ---------------------------------------------------------------------------------------
+// A row's logits count relative to its largest before anything is rounded: loss = S log sum - sum y (l - top).  top + log sum
+// and sum y l would each carry the rounding of a number of the logits' size: 3e-5 near 1000, where a row sure of its class
+// has a loss of 1e-9.
+
+// What logits are taken relative to: their largest, 0 where there is none.
+__device__ __forceinline__ float reference(float top) { return top == -INFINITY ? 0.f : top; }
+
+// exp(l - top) as exp2(l by + off) rest, one fused product a logit: off is -top log2 e rounded, and rest, a factor of the
+// whole row, what that rounding took from the exponent (the constant's own error meets l - top alone).  From 2^30 on, where
+// off rounds by more than the exponential takes and ends past fp32's range, logits lie at least 64 apart: their difference
+// as the exponent of two tells equal ones from smaller ones just as well.
 struct Exponent {
   float by, off;
-  __device__ __forceinline__ static bool far(float top) { return fabsf(top) >= 0x1p31f && fabsf(top) < INFINITY; }
-  __device__ __forceinline__ explicit Exponent(float top)
-      : by(far(top) ? 1.f : kLog2e), off(top == -INFINITY ? 0.f : -top * by) {}
+  __device__ __forceinline__ static bool far(float top) { return fabsf(top) >= 0x1p30f && fabsf(top) < INFINITY; }
+  __device__ __forceinline__ explicit Exponent(float top) : by(far(top) ? 1.f : kLog2e), off(-reference(top) * by) {}
+  __device__ __forceinline__ float rest(float top) const {
+    return __builtin_amdgcn_exp2f(fmaf(-reference(top), by, -off));
+  }
 };
+
+// sum y (l - top) relative to another logit, mass being sum y.
+__device__ __forceinline__ float moved(float dot, float mass, float top, float to) {
+  return mass == 0.f ? dot : fmaf(mass, reference(top) - to, dot);
+}
 
 // ---- targets and rows left out ----------------------------------------------------------------------------------
 struct Rows {
@@ -230,7 +246,7 @@ struct GemmArgs {
   const void* bias;          // this piece's
   int64_t v0, V;             // first class of the piece, classes in all
   float2* part;              // E_LSE: [N][part_ld] (largest, sum of exponentials), this launch's tiles from part_at
-  float2* part_y;            // E_LSE, label rows: likewise (sum y l, sum y)
+  float2* part_y;            // E_LSE, label rows: likewise (sum y (l - largest), sum y)
   int64_t part_ld, part_at;
   float* hit;                // E_LSE, indices: [N] the target's logit
   const float* stats;        // E_DL
@@ -664,27 +680,6 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
     if constexpr (EPI == E_LSE) {
       float* sm = reinterpret_cast<float*>(stage);  // [4][WM][BN]
       float top[CT], sum[CT], dot[CT] = {}, mass[CT] = {};
-      if constexpr (SOFT) {
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-          const bool in = word_target(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
-          labels(j, in, [&](int i, floatx4 y) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float v = in ? y[q] : 0.f;
-              mass[j] += v;
-              dot[j] += v == 0.f ? 0.f : v * acc[i][j][q];  // a class at -inf without mass adds nothing
-            }
-          });
-        }
-#pragma unroll
-        for (int d = 16; d < 64; d <<= 1)
-#pragma unroll
-          for (int j = 0; j < CT; ++j) {
-            dot[j] += __shfl_xor(dot[j], d);
-            mass[j] += __shfl_xor(mass[j], d);
-          }
-      }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
         top[j] = -INFINITY, sum[j] = 0.f;
@@ -701,6 +696,28 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
 #pragma unroll
         for (int j = 0; j < CT; ++j) top[j] = fmaxf(top[j], other[j]);
       }
+      if constexpr (SOFT) {
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          const bool in = word_target(info[at * INFO + wn * (BN / WN) + j * 16 + fr][3]) != kLeftOut;
+          const float ref = reference(top[j]);
+          labels(j, in, [&](int i, floatx4 y) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float v = in ? y[q] : 0.f;
+              mass[j] += v;
+              dot[j] += v == 0.f ? 0.f : v * (acc[i][j][q] - ref);  // a class at -inf without mass adds nothing
+            }
+          });
+        }
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1)
+#pragma unroll
+          for (int j = 0; j < CT; ++j) {
+            dot[j] += __shfl_xor(dot[j], d);
+            mass[j] += __shfl_xor(mass[j], d);
+          }
+      }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
         const Exponent e(top[j]);
@@ -709,7 +726,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], e.by, e.off));
-        sum[j] = (part[0] + part[1]) + (part[2] + part[3]);
+        sum[j] = ((part[0] + part[1]) + (part[2] + part[3])) * e.rest(top[j]);
       }
       if constexpr (!SOFT) {
 #pragma unroll
@@ -748,14 +765,14 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         float top = sm[col];
 #pragma unroll
         for (int w = 1; w < WM; ++w) top = fmaxf(top, sm[w * BN + col]);
-        const float ref = top == -INFINITY ? 0.f : top;
+        const float ref = reference(top);
         float sum = 0.f, dot = 0.f, mass = 0.f;
 #pragma unroll
         for (int w = 0; w < WM; ++w) {
-          const float tw = sm[w * BN + col];
+          const float tw = sm[w * BN + col], mw = sm[(3 * WM + w) * BN + col];
           sum += sm[(WM + w) * BN + col] * (tw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((tw - ref) * kLog2e));
-          dot += sm[(2 * WM + w) * BN + col];
-          mass += sm[(3 * WM + w) * BN + col];
+          dot += moved(sm[(2 * WM + w) * BN + col], mw, tw, ref);
+          mass += mw;
         }
         a.part[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(top, sum);
         if (SOFT) a.part_y[(n0 + col) * a.part_ld + a.part_at + tile_m] = make_float2(dot, mass);
@@ -968,10 +985,19 @@ __global__ void __launch_bounds__(256, NP == 1 ? 2 : 1) k_xent_both(GemmArgs x, 
 
 // A pair (largest, sum of exponentials relative to it) joined with another.
 __device__ __forceinline__ void join_pair(float& top, float& sum, float top2, float sum2) {
-  const float nt = fmaxf(top, top2), ref = nt == -INFINITY ? 0.f : nt;
+  const float nt = fmaxf(top, top2), ref = reference(nt);
   sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - ref) * kLog2e)) +
         sum2 * (top2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top2 - ref) * kLog2e));
   top = nt;
+}
+
+// Likewise with (sum y (l - largest), sum y).
+__device__ __forceinline__ void join_row(float& top, float& sum, float& dot, float& mass, float top2, float sum2, float dot2,
+                                         float mass2) {
+  const float ref = reference(fmaxf(top, top2));
+  dot = moved(dot, mass, top, ref) + moved(dot2, mass2, top2, ref);
+  mass += mass2;
+  join_pair(top, sum, top2, sum2);
 }
 
 // ---- joins ------------------------------------------------------------------------------------------------------
@@ -990,33 +1016,27 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
   }
   for (int64_t i = lane; i < tiles; i += 64) {
     const float2 p = part[n * tiles + i];
-    join_pair(top, sum, p.x, p.y);
-    if (part_y) {
-      const float2 q = part_y[n * tiles + i];
-      dot += q.x;
-      mass += q.y;
-    }
+    const float2 q = part_y ? part_y[n * tiles + i] : make_float2(0.f, 0.f);
+    join_row(top, sum, dot, mass, p.x, p.y, q.x, q.y);
   }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    join_pair(top, sum, __shfl_xor(top, d), __shfl_xor(sum, d));
-    dot += __shfl_xor(dot, d);
-    mass += __shfl_xor(mass, d);
-  }
+  for (int d = 1; d < 64; d <<= 1)
+    join_row(top, sum, dot, mass, __shfl_xor(top, d), __shfl_xor(sum, d), __shfl_xor(dot, d), __shfl_xor(mass, d));
   if (lane != 0) return;
   if (!last) {
     run[n] = make_float4(top, sum, dot, mass);
     return;
   }
   const bool counts = row_counts(rows, n);
-  float lse = top + logf(sum);
+  const float ls = logf(sum);
+  float lse = top + ls;
   if (rows.kind != GNCDE_TARGET_ROWS && counts) {
     const bool in = row_index(rows, n) < V;
     lse = in ? lse : NAN;
-    dot = in ? hit[n] : NAN;
+    dot = in ? hit[n] - top : NAN;
     mass = 1.f;
   }
-  loss[n] = counts ? mass * lse - dot : 0.f;
+  loss[n] = counts ? mass * ls - dot : 0.f;
   stats[2 * n] = counts ? lse : 0.f;
   stats[2 * n + 1] = counts ? mass : 0.f;
 }
@@ -1183,28 +1203,22 @@ __global__ void __launch_bounds__(kSmallThreads) k_xent_small(SmallArgs a) {
         }
         *reinterpret_cast<floatx4*>(d + fr * z.Vs + v) = dv;
       } else {
-        const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = tt == -INFINITY ? 0.f : tt;
-        float ts = 0.f;
+        const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = reference(tt);
+        float ts = 0.f, td = 0.f, tm = 0.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           ts += __builtin_amdgcn_exp2f((l[q] - ref) * kLog2e);
-          if (soft) {
-            mass += y[i][q];
-            dot += y[i][q] == 0.f ? 0.f : y[i][q] * l[q];  // a class at -inf without mass adds nothing
-          } else if (hit == v + q) {
-            dot = l[q];
-          }
+          const float yq = soft ? y[i][q] : hit == v + q ? 1.f : 0.f;
+          tm += yq;
+          td += yq == 0.f ? 0.f : yq * (l[q] - ref);  // a class at -inf without mass adds nothing
         }
-        join_pair(top, sum, tt, ts);
+        join_row(top, sum, dot, mass, tt, ts, td, tm);
       }
     }
     if (!GRAD) {
 #pragma unroll
-      for (int s = 16; s < 64; s <<= 1) {
-        join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
-        dot += __shfl_xor(dot, s);
-        mass += __shfl_xor(mass, s);
-      }
+      for (int s = 16; s < 64; s <<= 1)
+        join_row(top, sum, dot, mass, __shfl_xor(top, s), __shfl_xor(sum, s), __shfl_xor(dot, s), __shfl_xor(mass, s));
       if (fk == 0) *reinterpret_cast<floatx4*>(join + (wave * 16 + fr) * 4) = floatx4{top, sum, dot, mass};
       __syncthreads();
       if (wave == 0) {  // four of the waves' joins a lane, then the four lanes of a row
@@ -1212,23 +1226,19 @@ __global__ void __launch_bounds__(kSmallThreads) k_xent_small(SmallArgs a) {
 #pragma unroll
         for (int i = 0; i < kSmallWaves / 4; ++i) {
           const floatx4 q = *reinterpret_cast<const floatx4*>(join + ((fk * 4 + i) * 16 + fr) * 4);
-          join_pair(top, sum, q[0], q[1]);
-          dot += q[2];
-          mass += q[3];
+          join_row(top, sum, dot, mass, q[0], q[1], q[2], q[3]);
         }
 #pragma unroll
-        for (int s = 16; s < 64; s <<= 1) {
-          join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
-          dot += __shfl_xor(dot, s);
-          mass += __shfl_xor(mass, s);
-        }
+        for (int s = 16; s < 64; s <<= 1)
+          join_row(top, sum, dot, mass, __shfl_xor(top, s), __shfl_xor(sum, s), __shfl_xor(dot, s), __shfl_xor(mass, s));
         if (fk == 0 && n < a.N) {
-          lse = top + logf(sum);
+          const float ls = logf(sum);
+          lse = top + ls;
           if (!soft) {
             mass = 1.f;
             if (in && hit >= a.V) lse = dot = NAN;
           }
-          a.loss[n] = in ? mass * lse - dot : 0.f;
+          a.loss[n] = in ? mass * ls - dot : 0.f;
           a.stats[2 * n] = in ? lse : 0.f;
           a.stats[2 * n + 1] = in ? mass : 0.f;
         }
@@ -1495,29 +1505,26 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_xent_few(FewArgs a) {
         }
       }
     } else {
-      const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = tt == -INFINITY ? 0.f : tt;
-      float ts = 0.f;
+      const float tt = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), ref = reference(tt);
+      float ts = 0.f, td = 0.f, tm = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         ts += __builtin_amdgcn_exp2f((l[q] - ref) * kLog2e);
         if (soft) {
           const float yv = in && v + q < a.V ? y[v + q] : 0.f;
-          mass += yv;
-          dot += yv == 0.f ? 0.f : yv * l[q];  // a class at -inf without mass adds nothing
+          tm += yv;
+          td += yv == 0.f ? 0.f : yv * (l[q] - ref);  // a class at -inf without mass adds nothing
         } else if (hit == v + q) {
           a.hit[n] = l[q];
         }
       }
-      join_pair(top, sum, tt, ts);
+      join_row(top, sum, dot, mass, tt, ts, td, tm);
     }
   }
   if (GRAD) return;
 #pragma unroll
-  for (int s = 16; s < 64; s <<= 1) {
-    join_pair(top, sum, __shfl_xor(top, s), __shfl_xor(sum, s));
-    dot += __shfl_xor(dot, s);
-    mass += __shfl_xor(mass, s);
-  }
+  for (int s = 16; s < 64; s <<= 1)
+    join_row(top, sum, dot, mass, __shfl_xor(top, s), __shfl_xor(sum, s), __shfl_xor(dot, s), __shfl_xor(mass, s));
   __syncthreads();
   if (fk == 0) *reinterpret_cast<floatx4*>(join + (wave * 16 + fr) * 4) = floatx4{top, sum, dot, mass};
   __syncthreads();
@@ -1525,9 +1532,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_xent_few(FewArgs a) {
     top = -INFINITY, sum = dot = mass = 0.f;
     for (int w = 0; w < kFewWaves; ++w) {
       const floatx4 q = *reinterpret_cast<const floatx4*>(join + (w * 16 + threadIdx.x) * 4);
-      join_pair(top, sum, q[0], q[1]);
-      dot += q[2];
-      mass += q[3];
+      join_row(top, sum, dot, mass, q[0], q[1], q[2], q[3]);
     }
     a.part[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(top, sum);
     if (soft) a.part_y[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(dot, mass);

@@ -70,3 +70,21 @@ def test_loss_far_from_zero(size, kind, dtype, base):
     off = (loss.double() - want).abs()
     assert bool((off <= tol).all()), f"{float((off / tol).max()):.3g} of the bound"
     assert bool((loss >= 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("base", ["lowest", -2.0 ** 100, -2.0 ** 40, -2.0 ** 32, 2.0 ** 32, 1.5 * 2.0 ** 33, 2.0 ** 100, "most"])
+@pytest.mark.parametrize("kind", ["i64", "rows"])
+@pytest.mark.parametrize("size", [(40, 8, 256), (5, 300, 512), (40, 136, 1024), (300, 64, 32768)])
+def test_loss_of_equal_logits(size, kind, base, dtype):
+    """The products, below 2^7, vanish in fp32's rounding of the bias (half a step of 2^8 and more): all V logits are the
+    same number, the sum of exponentials is V exactly and the loss S log V, within the logarithm's 2 u, one product's
+    rounding, and that of S: V / 64 + 64 additions in the kernel, 64 bits here."""
+    c = make(*size, dtype, kind, 0.0)
+    fi = torch.finfo(dtype)
+    c["b"][:] = fi.min if base == "lowest" else fi.max if base == "most" else base
+    assert float((c["x"].float().abs() @ c["W"].float().abs().T).max()) < 2 ** 7
+    S = c["t"].double().sum(1) if kind == "rows" else torch.ones(size[0], dtype=torch.float64, device="cuda")
+    want = S * torch.log(torch.tensor(float(size[2]), dtype=torch.float64))
+    loss, _ = engine.linear_cross_entropy(c["x"], c["W"], c["b"], c["t"])
+    assert bool(((loss.double() - want).abs() <= (size[2] / 64 + 68) * U * want).all())
