@@ -314,13 +314,15 @@ int gncde_clip_by_global_norm(int32_t count, const GncdeTensor* tensors, float m
  * With l_rv = sum_h x_rh W_vh + b_v, lse_r = log sum_v exp l_rv and S_r = sum_v y_rv:
  *   loss_r = S_r lse_r - sum_v y_rv l_rv                     (trainer_tgb.cross_entropy_loss, trainer_tgb.py:42-60)
  * without the logits [rows, classes] in memory: they are made tile by tile, and once more for the gradient.
- * Both terms are taken relative to the row's largest logit, so the loss carries no rounding of the logits' own size.
+ * Both terms are taken relative to the row's largest logit, and the gradient's softmax likewise: neither carries a rounding
+ * of the logits' own size.
  *   x [rows, hidden], W [classes, hidden], b [classes] (may be NULL): dtype GNCDE_DTYPE_FP32 or _BF16, all the same
  *   target by target_kind: INDEX32 / INDEX64 [rows] class indices (y_r one-hot, S_r = 1; a NEGATIVE index leaves the
  *          row out; an index >= classes makes the row's loss, and every gradient it enters, NaN), or ROWS
  *          [rows, classes] fp32 y
  *   mask [rows] bytes, 0 leaves the row out (may be NULL)
- *   loss [rows] fp32, 0 for rows left out; stats [rows, 2] fp32 (lse_r, S_r), read by the gradient
+ *   loss [rows] fp32, 0 for rows left out; stats [rows, 2] fp32, read by the gradient: lse_r rounded, and S_r times
+ *        exp(lse_r rounded - lse_r), so that the gradient's softmax is not off by that rounding
  * A row left out changes nothing, whatever its values.  b may hold -inf (a class nothing can be); non-finite values in
  * x (of a row that counts) or W make losses NaN or inf.  Sums, maxima and logits are fp32 (bf16 inputs: exact products,
  * fp32 accumulation; fp32 inputs: each value as three bf16 parts, whose six leading products leave ~2^-24 of |x||W|;

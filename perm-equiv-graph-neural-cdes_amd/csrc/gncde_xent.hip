@@ -62,18 +62,23 @@ __device__ __forceinline__ void split(float x, uint16_t (&p)[NP]) {
 // What logits are taken relative to: their largest, 0 where there is none.
 __device__ __forceinline__ float reference(float top) { return top == -INFINITY ? 0.f : top; }
 
-// exp(l - top) as exp2(l by + off) rest, one fused product a logit: off is -top log2 e rounded, and rest, a factor of the
+// exp(l - top), or exp(l - lse), as exp2(l by + off) rest, one fused product a logit: off is -top log2 e rounded, and rest, a factor of the
 // whole row, what that rounding took from the exponent (the constant's own error meets l - top alone).  From 2^30 on, where
 // off rounds by more than the exponential takes and ends past fp32's range, logits lie at least 64 apart: their difference
 // as the exponent of two tells equal ones from smaller ones just as well.
 struct Exponent {
   float by, off;
   __device__ __forceinline__ static bool far(float top) { return fabsf(top) >= 0x1p30f && fabsf(top) < INFINITY; }
-  __device__ __forceinline__ explicit Exponent(float top) : by(far(top) ? 1.f : kLog2e), off(-reference(top) * by) {}
-  __device__ __forceinline__ float rest(float top) const {
-    return __builtin_amdgcn_exp2f(fmaf(-reference(top), by, -off));
-  }
+  __device__ __forceinline__ explicit Exponent(float top) : by(far(top) ? 1.f : kLog2e), off(-top * by) {}
+  __device__ __forceinline__ float rest(float top) const { return __builtin_amdgcn_exp2f(fmaf(-top, by, -off)); }
 };
+
+// The mass that goes with lse = top + log sum, as rounded, into the gradient: S exp(lse - (top + log sum)).  exp(l - lse) by
+// itself has the rounding of a number of the logits' size: 6e-5 of a probability near 1000.
+__device__ __forceinline__ float mass_beside(float lse, float top, float log_sum, float mass) {
+  const float b = lse - top, lost = (top - (lse - b)) + (log_sum - b);  // exactly what the sum's rounding dropped
+  return lost == lost ? mass * expf(-lost) : mass;
+}
 
 // sum y (l - top) relative to another logit, mass being sum y.
 __device__ __forceinline__ float moved(float dot, float mass, float top, float to) {
@@ -391,7 +396,8 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
                 "chunks divide over the waves");
   constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
   uint16_t* const stage = lds + L::HALF;
-  // What the logits' epilogues need of a row of x: lse's Exponent, g over the scale, the same times S, and the row's word.
+  // What the logits' epilogues need of a row of x: lse's exponent, g over the scale, the same times the mass and the
+  // exponent's rest, and the row's word.
   // Fetched with the tile's first operands, one tile ahead.
   floatx4* const info = reinterpret_cast<floatx4*>(lds + BUFS);
   float* const bias = reinterpret_cast<float*>(lds + BUFS + 2 * INFO * 8);  // of the tile's classes, likewise
@@ -502,7 +508,8 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
         if (EPI == E_DL) {
           const float lse = a.stats[2 * n], mass = a.stats[2 * n + 1];
           const float gv = a.g[n] / (a.scale ? *a.scale : 1.f);
-          v = floatx4{Exponent(lse).off, gv, gv * mass, lse};
+          const Exponent e(lse);
+          v = floatx4{e.off, gv, gv * mass * e.rest(lse), lse};
         }
         const bool in = n0 + r < a.N && kept && c >= 0;
         const int64_t t = c - a.v0;
@@ -720,13 +727,14 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
       }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
-        const Exponent e(top[j]);
+        const float ref = reference(top[j]);
+        const Exponent e(ref);
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q) part[q] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], e.by, e.off));
-        sum[j] = ((part[0] + part[1]) + (part[2] + part[3])) * e.rest(top[j]);
+        sum[j] = ((part[0] + part[1]) + (part[2] + part[3])) * e.rest(ref);
       }
       if constexpr (!SOFT) {
 #pragma unroll
@@ -1038,7 +1046,7 @@ __global__ void __launch_bounds__(256) k_xent_join(int64_t N, int64_t tiles, con
   }
   loss[n] = counts ? mass * ls - dot : 0.f;
   stats[2 * n] = counts ? lse : 0.f;
-  stats[2 * n + 1] = counts ? mass : 0.f;
+  stats[2 * n + 1] = counts ? mass_beside(lse, top, ls, mass) : 0.f;
 }
 
 // out[i] = sum over splits of acc[s][i], in the split order, times the scale: up to four such jobs a launch.
@@ -1240,7 +1248,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_xent_small(SmallArgs a) {
           }
           a.loss[n] = in ? mass * ls - dot : 0.f;
           a.stats[2 * n] = in ? lse : 0.f;
-          a.stats[2 * n + 1] = in ? mass : 0.f;
+          a.stats[2 * n + 1] = in ? mass_beside(lse, top, ls, mass) : 0.f;
         }
       }
     } else {

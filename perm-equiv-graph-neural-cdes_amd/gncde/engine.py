@@ -461,8 +461,8 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, b: torch.Tensor | Non
     x [..., hidden], W [classes, hidden], b [classes] or None: fp32 or bf16, all the same.  target: class indices [...]
     (int32 / int64; a negative one leaves its row out, one past the last class makes the row NaN) or label rows
     [..., classes] fp32, of any mass.  mask [...] bool: False leaves the row out; its loss is 0 and its values change
-    nothing.  ``stats`` holds each row's (log of the summed exponentials, label mass) for
-    ``linear_cross_entropy_grad``."""
+    nothing.  ``stats`` holds each row's (log of the summed exponentials, label mass over what the
+    first's rounding changes) for ``linear_cross_entropy_grad``."""
     done = _calls().readout_loss(x, W, b, target, mask)
     if done is not None:
         return done

@@ -88,3 +88,66 @@ def test_loss_of_equal_logits(size, kind, base, dtype):
     want = S * torch.log(torch.tensor(float(size[2]), dtype=torch.float64))
     loss, _ = engine.linear_cross_entropy(c["x"], c["W"], c["b"], c["t"])
     assert bool(((loss.double() - want).abs() <= (size[2] / 64 + 68) * U * want).all())
+
+
+def _grads(c, need=(True, True, True)):
+    _, stats = engine.linear_cross_entropy(c["x"], c["W"], c["b"], c["t"])
+    return engine.linear_cross_entropy_grad(c["x"], c["W"], c["b"], c["t"], stats, c["g"], None, *need)
+
+
+def _check_grads(c, l, y, p, D):
+    """gx, gW and gb against the formula: of dl, |g| S p carries (8 D + 360) u: the sum's (4 D + 260) u, the exponent's 4 u of
+    l - lse, which is below D + log V, 6 u of three exponentials and 4 u of the products; then the operand's rounding (bf16:
+    half a step of dl) and the sums'."""
+    R, V = l.shape
+    bf = c["x"].dtype == torch.bfloat16
+    half = 2.0 ** -8 if bf else U
+    g, S, x, W = c["g"].double()[:, None], y.sum(1, keepdim=True), c["x"].double(), c["W"].double()
+    gp, d = (g * S).abs() * p, g * (S * p - y)
+    t_d = gp * (8 * D + 360) * U + 4 * U * (gp + g.abs() * y)
+    t_op = t_d + max(half, 4 * U) * (d.abs() + t_d) + 2.0 ** -134
+    for name, got, v, t in zip(("gx", "gW", "gb"), _grads(c), (d @ W, d.T @ x, d.sum(0)),
+                               (t_op @ W.abs() + (V + 64) * U * (d.abs() @ W.abs()),
+                                t_op.T @ x.abs() + (R + 64) * U * (d.abs().T @ x.abs()),
+                                t_d.sum(0) + (R + 64) * U * d.abs().sum(0))):
+        off, tol = (got.double() - v).abs(), 1.01 * t + half * (v.abs() + t) + 2.0 ** -126
+        assert bool((off <= tol).all()), f"{name}: {float((off / tol).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("base", [0.0, 1024.0, -65536.0, 65536.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["i64", "rows"])
+@pytest.mark.parametrize("size", CASES)
+def test_gradients_far_from_zero(size, kind, dtype, base):
+    c = make(*size, dtype, kind, base)
+    l = c["x"].double() @ c["W"].double().T + c["b"].double()
+    y = c["t"].double() if kind == "rows" else torch.zeros_like(l).scatter_(1, c["t"][:, None], 1.0)
+    top = l.amax(1, keepdim=True)
+    _check_grads(c, l, y, torch.softmax(l - top, 1), float((top - l).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("base", ["lowest", -2.0 ** 100, -2.0 ** 32, 2.0 ** 32, 1.5 * 2.0 ** 33, 2.0 ** 100, "most"])
+@pytest.mark.parametrize("kind", ["i64", "rows"])
+@pytest.mark.parametrize("size", [(40, 8, 256), (5, 300, 512), (40, 136, 1024), (300, 64, 32768)])
+def test_gradients_of_equal_logits(size, kind, base, dtype):
+    """All V logits the same far number: p = 1 / V, which lse, rounded to a step of that number, does not hold by itself."""
+    c = make(*size, dtype, kind, 0.0)
+    fi = torch.finfo(dtype)
+    c["b"][:] = fi.min if base == "lowest" else fi.max if base == "most" else base
+    R, H, V = size
+    l = torch.zeros(R, V, dtype=torch.float64, device="cuda")
+    y = c["t"].double() if kind == "rows" else torch.zeros_like(l).scatter_(1, c["t"][:, None], 1.0)
+    _check_grads(c, l, y, torch.full_like(l, 1 / V), 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["i64", "rows"])
+@pytest.mark.parametrize("size", [(40, 8, 30), (5, 300, 700), (40, 136, 513)])
+def test_rows_that_nothing_can_be(size, kind, dtype):
+    """-inf in the whole bias: the softmax of no class is not a number, and neither is what it enters."""
+    c = make(*size, dtype, kind, 0.0)
+    c["b"][:] = -float("inf")
+    assert bool(torch.isnan(engine.linear_cross_entropy(c["x"], c["W"], c["b"], c["t"])[0]).all())
+    gx, gW, gb = _grads(c)
+    assert bool(torch.isnan(gx).all()) and bool(torch.isnan(gb).all()) and bool(torch.isnan(gW).all())
