@@ -206,10 +206,21 @@ __global__ void __launch_bounds__(kThreads) k_norm_total(const Part* __restrict_
   }
 }
 
+// t c / n as t half (c / n) half: below 2^-126 fp32 would hold few bits of c / n, or none, though t c / n is an ordinary
+// value for t near n.  There half is 2^-64 (t loses nothing to it that the result would hold) and c / n taken 2^128 times.
+struct Scale {
+  float by, half;
+  __device__ __forceinline__ Scale() {}
+  __device__ __forceinline__ Scale(float norm, float c) : by(c / norm), half(1.f) {
+    if (by < 0x1p-126f && norm < INFINITY) by = (c * 0x1p64f) / (norm * 0x1p-64f), half = 0x1p-64f;
+  }
+  __device__ __forceinline__ float operator()(float t) const { return t * half * by * half; }
+};
+
 // The chunk's first values are on their way while `scale_of`, which the whole workgroup takes part in, adds up the norm
 // (200 tensors of 30 million values: 86.3 -> 84.4 us); it says false where nothing is to be written.
-template <int DT, bool STREAM, typename Scale>
-__device__ __forceinline__ void apply(const void* p, void* q, int64_t from, int64_t to, Scale scale_of) {
+template <int DT, bool STREAM, typename Find>
+__device__ __forceinline__ void apply(const void* p, void* q, int64_t from, int64_t to, Find scale_of) {
   typedef Kind<DT> K;
   const typename K::T* x = static_cast<const typename K::T*>(p);
   typename K::T* y = static_cast<typename K::T*>(q);
@@ -226,14 +237,14 @@ __device__ __forceinline__ void apply(const void* p, void* q, int64_t from, int6
     }
   };
   load(from);
-  float scale;
+  Scale scale;
   if (!scale_of(scale)) return;
   for (int64_t at = from; at < to;) {
     const bool whole = at + kUnroll * step <= to;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
-      for (int i = 0; i < K::N; ++i) v[u][i] = K::put(K::get(v[u][i]) * scale);
+      for (int i = 0; i < K::N; ++i) v[u][i] = K::put(scale(K::get(v[u][i])));
       const int64_t w = at + threadIdx.x * K::N + u * step;
       if (whole || w + K::N <= to) {
         if (STREAM) __builtin_nontemporal_store(v[u], reinterpret_cast<typename K::V*>(y + w));
@@ -256,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_apply(Table t, const Part* __
   const int chunk = (int)gridDim.x - 1 - (int)blockIdx.x;
   const int k = entry_of(t, chunk);
   const Entry e = t.e[k];
-  const auto scale_of = [&](float& scale) {
+  const auto scale_of = [&](Scale& scale) {
     float norm, top;
     total(parts, nparts, norm, top);
     if (t.base == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_apply(Table t, const Part* __
       stats[1] = top;
     }
     const bool keep = norm < max_norm;
-    scale = keep ? 1.f : max_norm / norm;
+    scale = keep ? Scale(1.f, 1.f) : Scale(norm, max_norm);
     return !(keep && e.in == e.out);
   };
   const int dt = (int)(e.n_dtype & 3);
