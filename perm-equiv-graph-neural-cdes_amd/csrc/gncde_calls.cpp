@@ -65,7 +65,8 @@ bool checked(int rc) {
   return false;
 }
 
-// Runs f; a C++ exception (out of memory above all) becomes a Python error.
+// Runs f; a C++ exception becomes a Python error.  Every look at a tensor belongs in here: memory runs out, and tensors
+// without sizes or memory of their own throw where they are asked for them.
 template <class F>
 PyObject* guarded(F f) {
   try {
@@ -126,9 +127,9 @@ bool readout(PyObject* const* a, Readout& r) {
 void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
 PyObject* py_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  Readout r;
-  if (n != 5 || !readout(a, r)) Py_RETURN_NONE;
   return guarded([&]() -> PyObject* {
+    Readout r;
+    if (n != 5 || !readout(a, r)) Py_RETURN_NONE;
     const auto opt = r.x->options().dtype(at::kFloat).requires_grad(false);
     const auto lead = r.x->sizes().slice(0, r.x->dim() - 1);
     at::Tensor loss = at::empty(lead, opt);
@@ -154,19 +155,19 @@ PyObject* wrap(const at::Tensor& t) {
 
 PyObject* py_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // (x, W, b, target, mask, stats, g, need_x, need_w, need_b)
-  Readout r;
-  if (n != 10 || !readout(a, r)) Py_RETURN_NONE;
-  const at::Tensor *stats = tensor(a[5]), *cot = tensor(a[6]);
-  if (!plain(stats, *r.x) || !plain(cot, *r.x) || stats->scalar_type() != at::kFloat ||
-      cot->scalar_type() != at::kFloat)
-    Py_RETURN_NONE;
-  const auto lead = r.x->sizes().slice(0, r.x->dim() - 1);
-  if (cot->sizes() != lead || stats->dim() != r.x->dim() || stats->sizes().back() != 2 ||
-      stats->sizes().slice(0, lead.size()) != lead)
-    Py_RETURN_NONE;
-  const int nx = PyObject_IsTrue(a[7]), nw = PyObject_IsTrue(a[8]), nb = PyObject_IsTrue(a[9]);
-  if (nx < 0 || nw < 0 || nb < 0) return nullptr;
   return guarded([&]() -> PyObject* {
+    Readout r;
+    if (n != 10 || !readout(a, r)) Py_RETURN_NONE;
+    const at::Tensor *stats = tensor(a[5]), *cot = tensor(a[6]);
+    if (!plain(stats, *r.x) || !plain(cot, *r.x) || stats->scalar_type() != at::kFloat ||
+        cot->scalar_type() != at::kFloat)
+      Py_RETURN_NONE;
+    const auto lead = r.x->sizes().slice(0, r.x->dim() - 1);
+    if (cot->sizes() != lead || stats->dim() != r.x->dim() || stats->sizes().back() != 2 ||
+        stats->sizes().slice(0, lead.size()) != lead)
+      Py_RETURN_NONE;
+    const int nx = PyObject_IsTrue(a[7]), nw = PyObject_IsTrue(a[8]), nb = PyObject_IsTrue(a[9]);
+    if (nx < 0 || nw < 0 || nb < 0) return nullptr;
     const auto opt = r.x->options().requires_grad(false);
     at::Tensor gx, gW, gb;
     if (nx) gx = at::empty(r.x->sizes(), opt);
