@@ -3,7 +3,8 @@
 // which the Python wrappers of the same operators (gncde/engine.py) then take: they lay out, switch devices or refuse.
 // A call costs 7 us instead of 13 (read-out loss), a list of 200 tensors 20 instead of 110.
 //
-// Host code only: it fills the arguments of the C entry points of include/gncde.h, whose addresses Python hands over.
+// Host code only: it fills the arguments of the C entry points of include/gncde.h, whose addresses Python hands over.  The
+// module says which sources it was compiled from (this file and that header), and Python refuses it beside others.
 #include <Python.h>
 
 #include <ATen/Functions.h>
@@ -18,14 +19,12 @@
 namespace {
 
 struct Entry {
-  size_t (*loss_bytes)(int64_t, int64_t, int64_t, int32_t, int32_t);
-  int (*loss)(int64_t, int64_t, int64_t, int32_t, const void*, const void*, const void*, int32_t, const void*,
-              const uint8_t*, float*, float*, void*, size_t, void*);
-  int (*grad)(int64_t, int64_t, int64_t, int32_t, const void*, const void*, const void*, int32_t, const void*,
-              const uint8_t*, const float*, const float*, void*, void*, void*, void*, size_t, void*);
-  size_t (*list_bytes)(int32_t);
-  int (*norm)(int32_t, const GncdeTensor*, float*, void*, size_t, void*);
-  int (*clip)(int32_t, const GncdeTensor*, float, float*, void*, size_t, void*);
+  decltype(&gncde_linear_cross_entropy_workspace_bytes) loss_bytes;
+  decltype(&gncde_linear_cross_entropy) loss;
+  decltype(&gncde_linear_cross_entropy_grad) grad;
+  decltype(&gncde_global_norm_workspace_bytes) list_bytes;
+  decltype(&gncde_global_norm) norm;
+  decltype(&gncde_clip_by_global_norm) clip;
   PyObject* get_stream;  // device index -> raw stream
   PyObject* check;       // error code -> None, or raises
   PyObject* no_memory;   // the error class of an allocation that failed
@@ -298,4 +297,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "source_sha256", GNCDE_CALLS_SHA256) < 0) Py_CLEAR(m);
+  return m;
+}

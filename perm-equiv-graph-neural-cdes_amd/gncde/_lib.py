@@ -138,9 +138,15 @@ def source_files() -> list[str]:
     return files + [os.path.join(os.path.dirname(_PKG_ROOT), "include", "gncde.h")]
 
 
-def source_sha256() -> str:
-    """sha256 of the kernel sources in this tree (what `make` compiles into gncde_source_sha256())."""
-    files = source_files()
+def calls_source_files() -> list[str]:
+    """The files whose bytes the compiled calls' sha covers, in the Makefile's order."""
+    return [os.path.join(_PKG_ROOT, "csrc", "gncde_calls.cpp"),
+            os.path.join(os.path.dirname(_PKG_ROOT), "include", "gncde.h")]
+
+
+def source_sha256(files: list[str] | None = None) -> str:
+    """sha256 of the kernel sources in this tree (what `make` compiles into gncde_source_sha256()), or of ``files``."""
+    files = source_files() if files is None else files
     missing = [f for f in files if not os.path.exists(f)]
     if len(files) < 2 or missing:
         raise GncdeError(f"kernel sources not found ({missing or 'csrc/'}): cannot verify the library's build")
@@ -170,6 +176,18 @@ def verify_provenance(lib) -> str:
         raise GncdeError(f"{LIB_PATH} was built from kernel sources {built[:16]}..., this tree's are "
                          f"{tree[:16]}...: rebuild with `make -C perm-equiv-graph-neural-cdes_amd`")
     return built
+
+
+def verify_calls(module) -> None:
+    """Refuse compiled calls (gncde/_calls.so) that were not built from this tree's sources: they call the library's entry
+    points by address, with the signatures they were compiled with.  An explicit experiment build is not checked, as in
+    ``verify_provenance``."""
+    if os.environ.get("GNCDE_LIB") and os.environ.get("GNCDE_LIB_UNVERIFIED") == "1":
+        return
+    built, tree = getattr(module, "source_sha256", "unknown"), source_sha256(calls_source_files())
+    if built != tree:
+        raise GncdeError(f"gncde/_calls.so was built from sources {built[:16]}..., this tree's are {tree[:16]}...: rebuild "
+                         f"with `make -C perm-equiv-graph-neural-cdes_amd`")
 
 
 _lib = None

@@ -409,6 +409,7 @@ def _calls():
             from . import _calls as module
         except ImportError as e:
             raise _lib.GncdeError(f"gncde/_calls.so: {e}: build it with `make -C perm-equiv-graph-neural-cdes_amd`") from e
+        _lib.verify_calls(module)
         module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             lib.gncde_linear_cross_entropy_workspace_bytes, lib.gncde_linear_cross_entropy,
             lib.gncde_linear_cross_entropy_grad, lib.gncde_global_norm_workspace_bytes, lib.gncde_global_norm,
