@@ -176,7 +176,7 @@ class ClippedOptimiser:
         off = 0
         for p in self.params:
             k = p.numel()
-            p.grad = flat_grad[off:off + k].view_as(p).to(p.dtype)
+            p.grad = flat_grad[off:off + k].view_as(p).to(p.dtype, copy=True)
             off += k
         stats = self.clip()
         before = [p.detach().clone() for p in self.params]
