@@ -136,6 +136,11 @@ class ClipAdamW:
                                  self.eps, self.wd, self.max_norm)
 
 
+def _in_memory_order(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its axes in the order of its memory: contiguous where its values lie without gaps."""
+    return t if t.is_contiguous() else t.permute(sorted(range(t.dim()), key=t.stride, reverse=True))
+
+
 class ClippedOptimiser:
     """``optax.chain(optax.clip_by_global_norm(max_norm), <optimiser>)`` for any ``torch.optim.Optimizer`` (the
     reference's OptimiserCfg.build wraps adam, adamw and sgd alike, optimiser_configs.py:70-88), with ``ClipAdamW``'s
@@ -163,12 +168,19 @@ class ClippedOptimiser:
 
     def clip(self) -> torch.Tensor:
         """Clip the parameters' gradients in place; device stats (global norm, max|grad|) of what they were."""
-        grads = [p.grad for p in self.params if p.grad is not None]
+        grads = [_in_memory_order(p.grad) for p in self.params if p.grad is not None]
         if not grads:
             return torch.zeros(2, dtype=torch.float32, device=self.params[0].device)
         if self.max_norm is None:
             return engine.global_norm(grads)
-        return engine.clip_by_global_norm(grads, self.max_norm, out=grads)[1]
+        gaps = [i for i, g in enumerate(grads) if not g.is_contiguous()]  # clipped in a copy
+        lie = list(grads)
+        for i in gaps:
+            grads[i] = grads[i].contiguous()
+        stats = engine.clip_by_global_norm(grads, self.max_norm, out=grads)[1]
+        for i in gaps:
+            lie[i].copy_(grads[i])
+        return stats
 
     def step(self, flat_grad: torch.Tensor) -> torch.Tensor:
         """Apply one update from the (reduced) flat gradient; returns device stats (global grad norm, max|grad|,
