@@ -145,7 +145,8 @@ class ClippedOptimiser:
     """``optax.chain(optax.clip_by_global_norm(max_norm), <optimiser>)`` for any ``torch.optim.Optimizer`` (the
     reference's OptimiserCfg.build wraps adam, adamw and sgd alike, optimiser_configs.py:70-88), with ``ClipAdamW``'s
     interface for ``make_step``.  The parameters stay where they are, in their own types; the norm and the clipping run
-    on gncde_clip_by_global_norm over the parameters' gradients as they lie (``max_norm`` None: the norm alone)."""
+    on gncde_clip_by_global_norm over the parameters' gradients as they lie (``max_norm`` None: the norm alone).  Several
+    ranks reduce one flat fp32 gradient first, as for ``ClipAdamW``, and each parameter gets its piece of it."""
 
     def __init__(self, optimiser: torch.optim.Optimizer, max_norm: float | None = 1.0):
         self.optimiser = optimiser
@@ -182,20 +183,26 @@ class ClippedOptimiser:
             lie[i].copy_(grads[i])
         return stats
 
-    def step(self, flat_grad: torch.Tensor) -> torch.Tensor:
-        """Apply one update from the (reduced) flat gradient; returns device stats (global grad norm, max|grad|,
-        max|update|)."""
+    def step(self, flat_grad: torch.Tensor | None = None) -> torch.Tensor:
+        """Apply one update from the parameters' own gradients (a missing one counts as zeros), or from the (reduced) flat
+        gradient; returns device stats (global grad norm, max|grad|, max|update|)."""
         off = 0
         for p in self.params:
             k = p.numel()
-            p.grad = flat_grad[off:off + k].view_as(p).to(p.dtype, copy=True)
+            if flat_grad is not None:
+                p.grad = flat_grad[off:off + k].view_as(p).to(p.dtype, copy=True)
+            elif p.grad is None:
+                p.grad = torch.zeros_like(p)
             off += k
         stats = self.clip()
-        before = [p.detach().clone() for p in self.params]
+        types: dict = {}
+        for p in self.params:
+            types.setdefault(p.dtype, []).append(p.detach())
+        moved = [torch._foreach_neg(ps) for ps in types.values()]
         self.optimiser.step()
-        update = torch.stack([(p.detach() - q).abs().amax().to(torch.float32) if p.numel() else stats.new_zeros(())
-                              for p, q in zip(self.params, before)]).amax()
-        return torch.cat([stats, update.reshape(1)])
+        for m, ps in zip(moved, types.values()):
+            torch._foreach_add_(m, ps)
+        return torch.cat([stats, engine.global_norm([t for m in moved for t in m])[1:]])
 
 
 def make_step(opt: ClipAdamW | ClippedOptimiser, loss_terms, *args, **kwargs):
@@ -204,6 +211,10 @@ def make_step(opt: ClipAdamW | ClippedOptimiser, loss_terms, *args, **kwargs):
     max|update|) like trainer.py:327 (device scalars)."""
     opt.zero_grad()
     sse, count = loss_terms(*args, **kwargs)
+    if isinstance(opt, ClippedOptimiser) and dist_world()[1] == 1:  # nothing to reduce: the mean's gradients as they lie
+        (sse / count).backward()
+        stats = opt.step()
+        return sse.detach().to(torch.float64) / count, stats[1], stats[2]
     sse.backward()
     g, loss = reduce_gradients(opt.flat_grad(), sse, count)
     stats = opt.step(g)

@@ -56,3 +56,54 @@ def test_clip_takes_gradients_in_any_order_of_memory():
     assert abs(float(norm) - 0.5) <= 0.5 * 2.0 ** -8
     alone = train.ClippedOptimiser(torch.optim.SGD(ps, lr=0.1), None).clip()
     assert bool(((alone - engine.global_norm(grads)).abs() <= 2.0 ** -23 * alone).all())
+
+
+def loss_terms(ps, x):
+    """A sum of squares over parameters of both types, and its element count on the device; the last one takes no part."""
+    y = (x @ ps[0])[:, :8].to(torch.bfloat16) @ ps[1]
+    return (y.float() ** 2).sum() + ((x[:, :1] * ps[2].sum(0)) ** 2).sum(), torch.tensor(5 * 7, device="cuda")
+
+
+@pytest.mark.parametrize("kind", ["sgd", "adamw"])
+@pytest.mark.parametrize("max_norm", [0.05, 1e4, None])
+def test_make_step_clips_gradients_as_they_lie(kind, max_norm, monkeypatch):
+    """One process: the mean loss's gradients reach the clip in the parameters' own tensors, with no flat copy on the way; a
+    parameter without one counts as zeros (weight decay applies to it), as in the flat gradient."""
+    make = {"sgd": lambda ps: torch.optim.SGD(ps, lr=0.1), "adamw": lambda ps: torch.optim.AdamW(ps, lr=0.1, weight_decay=0.1)}
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(5, 20, generator=g, device="cuda")
+    a, b = params(), params()
+    opt = train.ClippedOptimiser(make[kind](a), max_norm)
+    monkeypatch.setattr(opt, "flat_grad", lambda: pytest.fail("a flat gradient"))
+    got = train.make_step(opt, loss_terms, a, x)
+
+    sse, count = loss_terms(b, x)
+    (sse / count).backward()
+    for p in b:
+        p.grad = torch.zeros_like(p) if p.grad is None else p.grad
+    stats = train.ClippedOptimiser(make[kind](b), max_norm).clip()
+    before = [p.detach().clone() for p in b]
+    make[kind](b).step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and torch.equal(p.grad, q.grad) and p.grad.stride() == q.grad.stride()
+    assert abs(float(got[0]) - float(sse.detach()) / 35) <= 2.0 ** -22 * abs(float(got[0]))
+    assert torch.equal(got[1], stats[1])
+    assert float(got[2]) == max(float((p.detach() - z).abs().max()) for p, z in zip(b, before))
+    if kind == "adamw":
+        assert not torch.equal(a[3], params()[3])
+
+
+@pytest.mark.parametrize("max_norm", [0.05, None])
+def test_make_step_of_several_ranks_reduces_one_flat_gradient(max_norm, monkeypatch):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(5, 20, generator=g, device="cuda")
+    a, b = params(), params()
+    monkeypatch.setattr(train, "dist_world", lambda: (0, 2))
+    got = train.make_step(train.ClippedOptimiser(torch.optim.SGD(a, lr=0.1), max_norm), loss_terms, a, x)
+    ref = train.ClippedOptimiser(torch.optim.SGD(b, lr=0.1), max_norm)
+    sse, count = loss_terms(b, x)
+    sse.backward()
+    mean, loss = train.reduce_gradients(ref.flat_grad(), sse, count)
+    stats = ref.step(mean)
+    assert all(torch.equal(p, q) and torch.equal(p.grad, q.grad) for p, q in zip(a, b))
+    assert torch.equal(got[0], loss) and torch.equal(got[1], stats[1]) and torch.equal(got[2], stats[2])
