@@ -12,7 +12,7 @@ solves' step counts; pgt/tgb: the windows of each optimiser step), with one grad
 
 Flow (trainer.py:88-285): build the dataset (gncde.data, f2), the vector field by registry name
 (vector_field_configs.py:52) and GraphNeuralCDE (model_configs.py:46-59); full-batch training steps
-(make_step, trainer.py:288-327) with clip_by_global_norm(1) + AdamW on the GPU; every ``eval_freq`` epochs the
+(make_step, trainer.py:288-327) with clip_by_global_norm(1) + AdamW, Adam or SGD on the GPU; every ``eval_freq`` epochs the
 interpolation / extrapolation MSE with the model's own solve (Tsit5 + PIDController, SaveAt(ts)); early
 stopping with ``patience`` / ``min_epochs``; the best model saved under ``checkpoint_dir`` (safetensors).
 
@@ -54,6 +54,22 @@ def _optimiser(cfg: dict) -> dict:
         raise NotImplementedError("only constant_schedule is wired (optimiser_configs.py)")
     return {"learning_rate": float(sched.get("value", 1e-3)), "weight_decay": float(opt_cfg.get("weight_decay", 0.0)),
             "gradient_clipping": bool(opt_cfg.get("gradient_clipping", True))}
+
+
+def _build_optimiser(cfg: dict, model: torch.nn.Module):
+    """The optimiser that the ``optimiser:`` block names (adamw | adam | sgd, adamw without a name) behind its optional
+    clip_by_global_norm(1) (optimiser_configs.py:70-88)."""
+    numbers, name = _optimiser(cfg), cfg.get("optimiser", {}).get("name", "adamw")
+    if name == "adamw":
+        return train.ClipAdamW(model, **numbers)
+    kinds = {"adam": torch.optim.Adam, "sgd": torch.optim.SGD}
+    if name not in kinds:
+        raise NotImplementedError(f"optimiser {name}: adamw, adam or sgd")
+    if numbers["weight_decay"]:
+        raise ValueError(f"optimiser {name} takes no weight_decay (adamw does)")
+    params = [p for p in model.parameters() if p.requires_grad]
+    return train.ClippedOptimiser(kinds[name](params, lr=numbers["learning_rate"]),
+                                  1.0 if numbers["gradient_clipping"] else None)
 
 
 class Trainer:
@@ -115,7 +131,7 @@ class Trainer:
     def run(self) -> dict:
         ds, model = self.build()
         rank, world = train.dist_world()
-        opt = train.ClipAdamW(model, **_optimiser(self.cfg))
+        opt = _build_optimiser(self.cfg, model)
         # training control over the training knots (the reference's train_graph_path_coeffs), validation over all
         ts_tr, coef_tr, tcoef_tr = ds.graph_path(ds.id_train)
         ts_all, coef_all, tcoef_all = ds.graph_path(list(range(ds.t.shape[1])))
@@ -307,7 +323,7 @@ class WindowTrainer:
     def run(self) -> dict:
         from safetensors.torch import save_file
         ds, model = self.build()
-        opt = train.ClipAdamW(model, **_optimiser(self.cfg))
+        opt = _build_optimiser(self.cfg, model)
         # Data parallelism: each optimiser step takes `window_batch` windows (at least one per rank),
         # split over the ranks (balanced_partition by the windows' costs: the adaptive TGB solve's accepted step
         # counts from the previous epoch, else equal), with one gradient all-reduce per step (train.make_step
