@@ -8,6 +8,7 @@
 // Two launches for every 128 tensors.  k_norm_part cuts each tensor into chunks, one workgroup a chunk, and writes one
 // (sum of squares, largest magnitude) per chunk; k_norm_apply has every workgroup add up all the chunks' sums itself,
 // in the same order (so no launch in between, no atomics, and the same bits from every workgroup), and scale its chunk.
+// (Of very long lists k_norm_join adds them up, in that order too.)
 // The tensor table travels in the kernel arguments: no copy to the device, and a captured graph keeps it.
 //
 // Squares and sums are held in 64 bits: an fp32 square overflows from 1.8e19 and is lost below 1e-19, and a gradient
@@ -22,6 +23,10 @@ namespace {
 constexpr int kTensors = 128;       // table entries a launch (128 * 24 + 129 * 4 bytes of 4096 of kernel arguments)
 constexpr int kThreads = 256;
 constexpr int kChunks = 2048;       // chunks aimed at: 8 workgroups a CU, all resident at once
+// Past so many chunks (more than two thousand tensors) one workgroup adds them up first: as it is otherwise, every
+// workgroup of every table's launch does, which costs the square of the tensors (clip of 5000 tensors 522 -> 447 us, 20000
+// 3190 -> 2000, 100000 46 -> 13 ms; at 2000 the extra launch would gain nothing).
+constexpr int kJoin = 2 * kChunks;
 constexpr int64_t kMinChunk = 32768;  // bytes: one round of 8 16-byte loads for every thread
 // Past what the last-level cache (256 MB) holds, a list's reads and writes go round it: 1.5e9 bf16 values clip in 1644
 // instead of 1742 us (5.5 TB/s over both passes), 200 million mixed ones are summed in 83 instead of 94 us (6.4 TB/s).
@@ -181,19 +186,32 @@ __global__ void __launch_bounds__(kThreads) k_norm_part(Table t, Part* __restric
   if (threadIdx.x == 0) parts[t.base + blockIdx.x] = Part{s, m, 0.f};
 }
 
-// Norm and largest magnitude from all chunks, the same bits in every workgroup.  fmaxf passes over a NaN; the sum
-// does not, and says so for both.
-__device__ __forceinline__ void total(const Part* __restrict__ parts, int nparts, float& norm, float& top) {
-  double s = 0.0;
-  float m = 0.f;
+// All chunks' sum and largest magnitude, the same bits in every workgroup.
+__device__ __forceinline__ void join(const Part* __restrict__ parts, int nparts, double& s, float& m) {
+  s = 0.0;
+  m = 0.f;
   for (int i = threadIdx.x; i < nparts; i += kThreads) {
     const Part p = parts[i];
     s += p.sum;
     m = fmaxf(m, p.top);
   }
   block_sum(s, m);
+}
+
+// Norm and largest magnitude from all chunks.  fmaxf passes over a NaN; the sum does not, and says so for both.
+__device__ __forceinline__ void total(const Part* __restrict__ parts, int nparts, float& norm, float& top) {
+  double s;
+  float m;
+  join(parts, nparts, s, m);
   norm = (float)sqrt(s);
   top = s != s ? norm : m;
+}
+
+__global__ void __launch_bounds__(kThreads) k_norm_join(Part* __restrict__ parts, int nparts) {
+  double s;
+  float m;
+  join(parts, nparts, s, m);
+  if (threadIdx.x == 0) parts[nparts] = Part{s, m, 0.f};
 }
 
 __global__ void __launch_bounds__(kThreads) k_norm_total(const Part* __restrict__ parts, int nparts,
@@ -321,6 +339,7 @@ int run(int32_t count, const GncdeTensor* ts, float* stats, bool clip, float max
   Part* parts = static_cast<Part*>(workspace);
   const int64_t chunk = chunk_bytes(bytes);
   int nparts = 0;
+  const Part* sums = parts;  // what the second pass adds up
   bool applied = false;
   for (int pass = 0; pass < (clip ? 2 : 1); ++pass) {
     Table t;
@@ -345,14 +364,18 @@ int run(int32_t count, const GncdeTensor* ts, float* stats, bool clip, float max
         else hipLaunchKernelGGL(k_norm_part<false>, dim3(blocks), dim3(kThreads), 0, st, t, parts);
       } else {
         if (stream_past)
-          hipLaunchKernelGGL(k_norm_apply<true>, dim3(blocks), dim3(kThreads), 0, st, t, parts, nparts, max_norm, stats);
+          hipLaunchKernelGGL(k_norm_apply<true>, dim3(blocks), dim3(kThreads), 0, st, t, sums, nparts, max_norm, stats);
         else
-          hipLaunchKernelGGL(k_norm_apply<false>, dim3(blocks), dim3(kThreads), 0, st, t, parts, nparts, max_norm, stats);
+          hipLaunchKernelGGL(k_norm_apply<false>, dim3(blocks), dim3(kThreads), 0, st, t, sums, nparts, max_norm, stats);
         applied = true;
       }
       base += blocks;
     }
     nparts = base;
+    if (clip && pass == 0 && nparts > kJoin) {
+      hipLaunchKernelGGL(k_norm_join, dim3(1), dim3(kThreads), 0, st, parts, nparts);
+      sums = parts + nparts, nparts = 1;
+    }
   }
   if (!applied) hipLaunchKernelGGL(k_norm_total, dim3(1), dim3(kThreads), 0, st, parts, nparts, stats);
   return hipGetLastError() == hipSuccess ? GNCDE_OK : GNCDE_ERR_HIP;
