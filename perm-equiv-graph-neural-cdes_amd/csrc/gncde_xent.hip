@@ -1689,7 +1689,7 @@ Cfg choose(int epi, int64_t M, int64_t N, int64_t kt, int np, int64_t most_split
   Cfg best = cost(epi, M, N, kt, np, T_LARGE, 1);
   const int64_t tiles = div_up(M, 256) * div_up(N, 256);
   for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > most_splits || s * (np == 1 && out ? 4 : 2) > kt + 1 || (s > 1 && tiles * s > 2 * kCus)) break;
+    if (s > 1 && (s > most_splits || s * (np == 1 && out ? 4 : 2) > kt + 1 || tiles * s > 2 * kCus)) break;
     for (int tile = T_LARGE; tile <= (out ? T_SMALL : T_HALF); ++tile) {
       const Cfg c = cost(epi, M, N, kt, np, tile, div_up(kt, div_up(kt, s)));  // no split without a step
       if (c.us < best.us) best = c;

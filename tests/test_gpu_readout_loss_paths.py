@@ -20,6 +20,8 @@ F, B = torch.float32, torch.bfloat16
     ((1021, 333, 50021), F, "i64"),                                  # loss and dl of three parts in two launches
     ((4000, 64, 9000), B, "i64"), ((4000, 64, 9000), F, "rows"),     # one of them in two launches
     ((5000, 200, 6000), F, "i64"),                                   # gW in large split tiles
+    # up to 64 rows: gW's contraction has one or two steps, and small tiles beside gx's
+    ((24, 256, 2000), B, "i64"), ((50, 64, 9000), B, "rows"), ((64, 72, 700), B, "i64"), ((17, 130, 513), B, "rows"),
     ((2048, 256, 8191), B, "rows"), ((2903, 51, 1293), B, "i64"),
 ])
 def test_ways_of_dividing_the_work(size, dtype, kind):
