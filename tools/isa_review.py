@@ -9,12 +9,11 @@ VGPR / AGPR / SGPR counts, scratch (private segment) and static LDS, and llvm-ob
   python tools/isa_review.py --all      # every kernel
 
 Checks (tests/test_isa.py runs them):
-  * no instruction writes through the scalar data cache (scalar stores, scalar atomics, scalar cache write-back);
+  * every scalar memory instruction is a load: nothing writes through the scalar data cache or touches it otherwise;
   * the headline kernel k_fused<64,16,3,rk4> has no scratch, at most 128 VGPRs (four waves per SIMD), and its
     products on v_mfma_f32_16x16x4_f32;
   * every kernel's scratch is reported (spills are visible, not silent);
   * no kernel wraps a buffer access in a waterfall loop (a descriptor the compiler could not prove uniform).
-This file names scalar-store mnemonics, so it is listed in .gpurunignore (it never runs on the GPU box).
 """
 from __future__ import annotations
 
@@ -29,9 +28,10 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "perm-equiv-graph-neural-cdes_amd")
 LLVM = "/opt/rocm/lib/llvm/bin"
 TARGET = "hipv4-amdgcn-amd-amdhsa--gfx950"
-# scalar-data-cache writes: s_store_*, s_buffer_store_*, s_scratch_store_*, s_atomic_*, s_buffer_atomic_*,
-# s_dcache_wb*
-SCALAR_WRITE = re.compile(r"^\s*(s_store_|s_buffer_store_|s_scratch_store_|s_atomic_|s_buffer_atomic_|s_dcache_wb)")
+# A scalar memory instruction is told by its encoding (bits 31:26 of the first word), whatever its name; these are allowed.
+SCALAR_MEMORY = 0x30
+SCALAR_LOAD = re.compile(r"^s_(load|buffer_load|scratch_load)_dword(x\d+)?$")
+ENCODED = re.compile(r"//\s*[0-9A-Fa-f]+:\s*([0-9A-Fa-f]{8})")
 WATERFALL = re.compile(r"^v_cmp_eq_u64\S*\s+\S+,\s*s\[\d+:\d+\],\s*v\[\d+:\d+\]")
 HEADLINE = "_ZN5gncde12_GLOBAL__N_17k_fusedILi64ELi16ELi3ELi0EEEvNS0_9FusedArgsE"
 
@@ -73,10 +73,15 @@ def kernel_metadata(co: str) -> dict:
     return out
 
 
+def scalar_write(line: str) -> bool:
+    """Whether an instruction, with its encoding behind it, is one of scalar memory that is not a load."""
+    word = ENCODED.search(line)
+    return bool(word) and int(word.group(1), 16) >> 26 == SCALAR_MEMORY and not SCALAR_LOAD.match(line.split()[0])
+
+
 def disassembly(co: str) -> dict:
-    """{symbol: [instruction lines]}"""
-    txt = subprocess.run([f"{LLVM}/llvm-objdump", "-d", "--no-show-raw-insn", co], check=True, capture_output=True,
-                         text=True).stdout
+    """{symbol: [instruction lines, their encodings behind them]}"""
+    txt = subprocess.run([f"{LLVM}/llvm-objdump", "-d", co], check=True, capture_output=True, text=True).stdout
     out, cur = {}, None
     for line in txt.splitlines():
         m = re.match(r"^[0-9a-f]+ <(.+)>:$", line)
@@ -110,7 +115,7 @@ def review(objs=None) -> dict:
                 res["kernels"][k] = m
             for k, ins in dis.items():
                 for x in ins:
-                    if SCALAR_WRITE.match(x):
+                    if scalar_write(x):
                         res["scalar_writes"].append((os.path.basename(o), k, x))
     return res
 
