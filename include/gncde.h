@@ -326,7 +326,8 @@ int gncde_clip_by_global_norm(int32_t count, const GncdeTensor* tensors, float m
  * A row left out changes nothing, whatever its values.  b may hold -inf (a class nothing can be); non-finite values in
  * x (of a row that counts) or W make losses NaN or inf.  Sums, maxima and logits are fp32 (bf16 inputs: exact products,
  * fp32 accumulation; fp32 inputs: each value as three bf16 parts, whose six leading products leave ~2^-24 of |x||W|;
- * the parts end at 2^-133, so fp32 values below 2^-109 carry fewer bits). */
+ * the parts end at 2^-133, so fp32 values below 2^-109 carry fewer bits, the gradient's g (S p - y) among them: cotangents
+ * that are all below 2^-110, 8e-34, leave its entries fewer bits than their own). */
 enum { GNCDE_TARGET_INDEX32 = 0, GNCDE_TARGET_INDEX64 = 1, GNCDE_TARGET_ROWS = 2 };
 /* Workspace of the loss (grad 0) or the gradient (grad 1); 0 for sizes the entries refuse. */
 size_t gncde_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t classes, int32_t dtype,

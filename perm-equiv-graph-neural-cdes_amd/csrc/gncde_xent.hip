@@ -280,14 +280,16 @@ struct GemmArgs {
 // of 128 x 128 read a third less and were slower, with nothing to run while one waits.  128 x 128 tiles, two workgroups a
 // CU, and 128 x 64 ones (the logits) serve where larger ones leave CUs idle.
 //
-// Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.8 (1.30),
-// gx 6.6 (1.34), gW 7.3 (1.20), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
+// Measured at 8192 x 4096 x 131072 bf16 (8.8 TFLOP a product): logits of the loss 6.6 ms (1.33 PFLOP/s), dl 6.9 (1.28),
+// gx 6.6 (1.33), gW 7.5 (1.18), where a library product of such operands reaches 1.4 to 1.6 and, turned as gW's are,
 // 0.94.  The logits are bound by power: their matrix units are busy 70 % of the cycles, and the clock falls to 1.65 GHz.
-// The turned products wait for their operands, two LDS reads a fragment instead of one.  Turning W, x and dl in memory
-// instead cost 0.5 ms of copies and 0.8 ms for dl's second form here, a tenth of the gradient at 1021 x 333 x 50021.
+// The turned products wait for their operands, two LDS reads a fragment instead of one; gW's, with both turned, takes all 256
+// registers and is the one kernel here with scratch (two registers, written and read once a tile, outside the loop over
+// steps).  Turning W, x and dl in memory instead cost 0.5 ms of copies and 0.8 ms for dl's second form here, a tenth of the
+// gradient at 1021 x 333 x 50021.
 //
 // The one-part products with turned operands (gx, gW) take steps of half that and four buffers (DEEP): their loads are
-// then two to three steps on their way instead of one, and a hand-over leaves those of two steps there (gW 8.6 -> 7.6 ms,
+// then two to three steps on their way instead of one, and a hand-over leaves those of two steps there (gW 8.6 -> 7.5 ms,
 // gx 7.5 -> 6.6).  dl lies in blocks of 32 classes for that, [class / 32][row][part][32]: a step's rows of it are one run
 // of memory.  The logits' operands lie as their rows do and would be read in pieces of half a cache line (7.1 -> 7.6 ms).
 template <int NP, bool DEEP>
@@ -1351,8 +1353,8 @@ __global__ void __launch_bounds__(1024) k_xent_parts_sum(int parts, int VH, int 
 // from memory into matrix operands (16 classes, 16 bytes a lane; LDS holds x alone), eight loads ahead of the products;
 // where the classes are too few for all waves, ks of them share a tile's contraction.  The gradient reads W once for dl
 // and once more, row by row, for gx, writing gW in the same loop: a VALU product, which for so few rows hides behind
-// the bytes, and needs no transposed copy of W.  One row of 4096 against 131072 classes in bf16: 205 us,
-// 5.2 TB/s, where reads alone reach 6.4.
+// the bytes, and needs no transposed copy of W.  One row of 4096 against 131072 classes in bf16: 210 us
+// with the join's 5, 5.2 TB/s of the stream, where reads alone reach 6.4.
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 16;
 constexpr int kFewLds = 147456;   // bytes of x
@@ -2079,7 +2081,9 @@ void backward(const Plan& p, const Call& c, const float* stats, const float* g, 
                          (int)(p.N * p.H), 0, part, gx, nullptr);
     return;
   }
-  float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);  // three parts lose nothing to it
+  // Three parts take dl as it is: an entry is off by 2^-25 of itself or 2^-134, whichever is more, and with the largest
+  // cotangent at 2^-110 or above (8e-34) the latter is below 2^-24 of that.
+  float* scale = F32 ? nullptr : reinterpret_cast<float*>(c.ws + p.o_scale);
   // gW multiplies every row of x, by zeros where it is left out: those rows are put aside, whatever they hold
   const bool aside = gW && (c.rows.mask || c.rows.kind != GNCDE_TARGET_ROWS);
   Operand<F32> x = {}, w = {};
