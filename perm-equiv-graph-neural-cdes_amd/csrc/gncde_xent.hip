@@ -62,10 +62,10 @@ __device__ __forceinline__ void split(float x, uint16_t (&p)[NP]) {
 // What logits are taken relative to: their largest, 0 where there is none.
 __device__ __forceinline__ float reference(float top) { return top == -INFINITY ? 0.f : top; }
 
-// exp(l - top), or exp(l - lse), as exp2(l by + off) rest, one fused product a logit: off is -top log2 e rounded, and rest, a factor of the
-// whole row, what that rounding took from the exponent (the constant's own error meets l - top alone).  From 2^30 on, where
-// off rounds by more than the exponential takes and ends past fp32's range, logits lie at least 64 apart: their difference
-// as the exponent of two tells equal ones from smaller ones just as well.
+// exp(l - top), or exp(l - lse), as exp2(l by + off) rest, one fused product a logit: off is -top log2 e rounded, and rest,
+// a factor of the whole row, what that rounding took from the exponent (the constant's own error meets l - top alone).  From
+// 2^30 on, where off rounds by more than the exponential takes and ends past fp32's range, logits lie at least 64 apart:
+// their difference as the exponent of two tells equal ones from smaller ones just as well.
 struct Exponent {
   float by, off;
   __device__ __forceinline__ static bool far(float top) { return fabsf(top) >= 0x1p30f && fabsf(top) < INFINITY; }
@@ -399,8 +399,7 @@ __device__ __forceinline__ void mm_tiles(const GemmArgs& a, uint16_t* lds, const
   constexpr int TILE = L::TILE, PAD = L::PAD, HALVES = L::HALVES, BUFS = L::BUFS, INFO = L::INFO, BIAS = L::BIAS;
   uint16_t* const stage = lds + L::HALF;
   // What the logits' epilogues need of a row of x: lse's exponent, g over the scale, the same times the mass and the
-  // exponent's rest, and the row's word.
-  // Fetched with the tile's first operands, one tile ahead.
+  // exponent's rest, and the row's word.  Fetched with the tile's first operands, one tile ahead.
   floatx4* const info = reinterpret_cast<floatx4*>(lds + BUFS);
   float* const bias = reinterpret_cast<float*>(lds + BUFS + 2 * INFO * 8);  // of the tile's classes, likewise
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
